@@ -16,7 +16,7 @@ from dataclasses import dataclass, field, fields
 from typing import Any
 
 _IDENT = {"add": (2, 0.0), "multiply": (2, 1.0), "maximum": (2, -1e30), "minimum": (2, 1e30)}
-_ARITY1 = {"copy", "exp", "reciprocal", "relu", "sqrt", "rsqrt", "negative", "abs", "tanh", "sin", "cos"}
+_ARITY1 = {"copy", "exp", "reciprocal", "relu", "sqrt", "rsqrt", "negative", "abs", "tanh", "sin", "cos", "sigmoid"}
 
 
 @dataclass

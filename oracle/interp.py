@@ -43,7 +43,7 @@ sys.path.insert(0, str(Path(__file__).resolve().parent / "emmy_shim"))
 
 from emmy.compiler import _model as M  # noqa: E402
 
-DT = {"f32": np.float32, "f16": np.float16, "f64": np.float64}
+DT = {"f32": np.float32, "f16": np.float16, "f64": np.float64, "i32": np.int32}
 SMEM_DT = {"float": np.float32, "__half": np.float16, "double": np.float64}
 LOG2_E32 = np.float32(math.log2(math.e))
 SWZ = {"B128": (6, 7), "B64": (6, 3), "B32": (6, 1)}
@@ -264,6 +264,9 @@ class Interp:
                     raise OracleError("exp on non-f32 values")
                 t = (x * LOG2_E32).astype(np.float32)
                 return np.exp2(t.astype(np.float64)).astype(np.float32)
+            if op == "sigmoid":
+                t = (x * np.float32(-LOG2_E32)).astype(np.float32)
+                return (1.0 / (1.0 + np.exp2(t.astype(np.float64)))).astype(dt)
             if op == "rsqrt":
                 return (1.0 / np.sqrt(x.astype(np.float64))).astype(dt)
             if op in ("tanh", "sin", "cos"):

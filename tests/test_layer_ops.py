@@ -1,0 +1,163 @@
+"""The layer operators on the CPU: the packages' statement trees, run by the oracle's interpreter
+(every access bounds-checked), give the operators' float64 definitions within what f32 arithmetic
+and one rounding allow; the builders refuse what they do not take; every module assembles without
+spills; the rotary tables follow their formulas."""
+
+import re
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+from layer_cases import HEADS, LINEAR, check, heads_expected, heads_package, heads_spec, linear_expected
+from oracle.interp import run_package as oracle_run
+from thompiler import ir, load, problems, rotary, synth
+from thompiler.compiler import compile_kernel
+
+
+def _ir(d):
+    return next(d.glob("*.ir.json"))
+
+
+@pytest.mark.parametrize("case", [c for c in LINEAR if c[3] == "f16" and c[0] * c[1] * c[2] < 2 ** 24], ids=str)
+def test_linear_tree_is_the_definition(tmp_path, case):
+    M, N, K, dtype, out, bias, act, res, gated = case
+    d = synth.linear_package(tmp_path, M, N, K, dtype, out, bias, act, res, gated)
+    x = problems.make_inputs(problems.load_package(d))
+    want, allowed = linear_expected(x["x"], x["w"], x.get("bias"), x.get("res"), N, act, gated, out)
+    check(oracle_run(d)["linear"], want, allowed, "linear")
+
+
+@pytest.mark.parametrize("case", [c for c in HEADS if c[6] != "bf16" and c[1] < 200], ids=str)
+def test_heads_tree_is_the_definition(tmp_path, case):
+    spec, table = heads_spec(case), 23
+    d = heads_package(synth, tmp_path, spec, table)
+    x = problems.make_inputs(problems.load_package(d))
+    x["pos"].flat[-1] = -1                               # an empty slot, and a position past the table
+    if x["pos"].size > 2:
+        x["pos"].flat[1] = table
+    got = oracle_run(d, x)
+    zeros = {n: 0.0 for n in ("q", "k", "v")}
+    want = heads_expected(x, spec, table, zeros)
+    assert set(got) == set(want)
+    for name, (w, allowed) in want.items():
+        check(got[name], w, allowed, name)
+
+
+def test_tree_survives_the_reader(tmp_path):
+    """The written text reads back as the tree the builder made (families compare the two)."""
+    from thompiler import schedules
+    epi = schedules.linear_epilogue(70, 72, "bf16", True, "gelu_tanh", True, True)
+    tree = schedules.linear_body(70, 72, 136, "bf16", True, epi)
+    assert ir.parse_stmt(synth.to_repr(tree)) == tree
+    tree = schedules.heads_body(2, 3, 4, 2, 80, 40, 9, "f16", True, True, True, False, 1e-5)
+    assert ir.parse_stmt(synth.to_repr(tree)) == tree
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(M=0, N=64, K=64), "M = 0"), (dict(M=4, N=60, K=64), "multiples of 8"), (dict(M=4, N=64, K=60), "multiples of 8"),
+    (dict(M=4, N=64, K=64, dtype="f32"), "dtype 'f32'"), (dict(M=4, N=64, K=64, dtype="f16", out_dtype="bf16"), "dtype"),
+    (dict(M=4, N=64, K=64, activation="gelu"), "activation 'gelu'"), (dict(M=2.0, N=64, K=64), "M = 2.0"),
+    (dict(M=4, N=-8, K=64), "N = -8")])
+def test_linear_refusals(tmp_path, kw, text):
+    with pytest.raises(ValueError, match=text):
+        synth.linear_package(tmp_path, **kw)
+    assert not list(tmp_path.glob("*"))
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(rotary=33), "rotary = 33"), (dict(rotary=130), "rotary = 130"), (dict(rotary=0), "rotary = 0"),
+    (dict(dtype="f64"), "dtype 'f64'"), (dict(kv_heads=0, values=True), "values without kv_heads"),
+    (dict(kv_heads=-1), "kv_heads = -1"), (dict(S=0), "S = 0"), (dict(table=0), "table = 0"), (dict(D=0), "D = 0"),
+    (dict(heads=0), "heads = 0")])
+def test_heads_refusals(tmp_path, kw, text):
+    args = dict(B=1, S=4, heads=4, kv_heads=2, D=128)
+    for build in (synth.rope_package, synth.qk_norm_rope_package):
+        with pytest.raises(ValueError, match=re.escape(text)):
+            build(tmp_path, **dict(args, **kw))
+    assert not list(tmp_path.glob("*"))
+
+
+def test_norm_refuses_a_negative_eps(tmp_path):
+    for eps in (-1e-6, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            synth.qk_norm_rope_package(tmp_path, 1, 4, 4, 2, 128, eps=eps)
+
+
+def _ptxas(ptx, tmp_path):
+    if shutil.which("ptxas") is None:
+        pytest.skip("ptxas not on PATH")
+    f = tmp_path / "k.ptx"
+    f.write_text(ptx)
+    r = subprocess.run(["ptxas", "-arch=sm_100a", "-v", str(f), "-o", str(tmp_path / "k.cubin")],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    assert "0 bytes spill stores" in r.stderr and "0 bytes stack frame" in r.stderr, r.stderr
+
+
+@pytest.mark.parametrize("tuned", [True, False], ids=["tuned", "generic"])
+@pytest.mark.parametrize("case", [LINEAR[i] for i in (1, 3, 4, 7, 12, 16, 17)], ids=str)
+def test_linear_assembles(tmp_path, case, tuned):
+    d = synth.linear_package(tmp_path, *case)
+    _ptxas(compile_kernel(load.load(str(_ir(d))), tuned=tuned), tmp_path)
+
+
+@pytest.mark.parametrize("tuned", [True, False], ids=["tuned", "generic"])
+@pytest.mark.parametrize("case", HEADS, ids=str)
+def test_heads_assemble(tmp_path, case, tuned):
+    d = heads_package(synth, tmp_path, heads_spec(case), 64)
+    _ptxas(compile_kernel(load.load(str(_ir(d))), tuned=tuned), tmp_path)
+
+
+# ---- storage types -----------------------------------------------------------------------
+
+def test_bf16_bits_round_to_nearest_even():
+    torch = pytest.importorskip("torch")
+    x = np.random.default_rng(1).standard_normal(4096).astype(np.float32)
+    x[:9] = [0.0, -0.0, np.inf, -np.inf, 1.00390625, 1.01171875, 3.4e38, 1e-40, 65535.0]
+    bits = problems.to_bf16(x)
+    want = torch.from_numpy(x).bfloat16().view(torch.int16).numpy().view(np.uint16)
+    assert np.array_equal(bits, want)
+    assert np.isnan(problems.from_bf16(problems.to_bf16(np.float32([np.nan]))))[0]
+    assert np.array_equal(problems.from_bf16(bits), torch.from_numpy(x).bfloat16().float().numpy())
+
+
+# ---- rotary tables -------------------------------------------------------------------------
+
+def test_rotary_tables_plain_and_far():
+    cos, sin = rotary.tables(131073, 64)
+    assert cos.dtype == sin.dtype == np.float32 and cos.shape == (131073, 32)
+    from math import cos as c, sin as s
+    for p in (0, 1, 4095, 65535, 65536, 131072):
+        for i in (0, 1, 17, 31):
+            a = p * 10000.0 ** (-2 * i / 64)
+            assert abs(cos[p, i] - c(a)) <= 2.0 ** -24 and abs(sin[p, i] - s(a)) <= 2.0 ** -24
+
+
+def test_rotary_scalings():
+    R, base, f = 128, 10000.0, 4.0
+    plain = rotary.frequencies(R)
+    assert np.allclose(rotary.frequencies(R, scaling="linear", factor=f), plain / f, rtol=1e-15)
+    ntk = rotary.frequencies(R, scaling="ntk", factor=f)
+    assert ntk[0] == 1.0 and np.isclose(ntk[-1], plain[-1] / f, rtol=1e-12)
+    parts = rotary.frequencies(R, scaling="parts", factor=f, original=4096, fast=32, slow=1)
+    turns = 4096 * plain / (2 * np.pi)
+    assert np.array_equal(parts[turns > 32], plain[turns > 32])
+    assert np.allclose(parts[turns < 1], plain[turns < 1] / f, rtol=1e-15)
+    mid = (turns >= 1) & (turns <= 32)
+    g = (turns[mid] - 1) / 31
+    assert mid.any() and np.allclose(parts[mid], plain[mid] * ((1 - g) / f + g), rtol=1e-15)
+    cos, _ = rotary.tables(4, R, scaling="parts", factor=f, original=4096, scale=1.25)
+    assert np.all(cos[0] == np.float32(1.25))
+
+
+@pytest.mark.parametrize("kw", [dict(rotary=7), dict(rotary=0), dict(rotary=8, scaling="dynamic"),
+                                dict(rotary=8, scaling="parts", factor=2.0), dict(rotary=8, factor=0.5),
+                                dict(rotary=8, base=0.0),
+                                dict(rotary=8, scaling="parts", original=64, fast=1.0, slow=2.0)])
+def test_rotary_refusals(kw):
+    with pytest.raises(ValueError):
+        rotary.frequencies(**kw)
+    with pytest.raises(ValueError):
+        rotary.tables(0, 8)

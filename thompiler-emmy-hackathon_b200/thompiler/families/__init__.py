@@ -7,6 +7,7 @@ this backend has a tuned body for, else None (generic lowering).
 from __future__ import annotations
 
 from thompiler.load import KernelInfo
+from thompiler.lowering.types import BF16, I32
 
 
 def recognise(kernel: KernelInfo):
@@ -24,6 +25,10 @@ def recognise(kernel: KernelInfo):
     flat = tile is not None and all(isinstance(s, (ir.Load, ir.Assign, ir.Let, ir.Write))
                                     for s in tile.body)                  # pointwise
     simt_mm = ir.CpAsyncCopy in kinds and ir.MmaSyncPtx not in kinds    # f32 matmul on the FMA pipes
+    # storage types (a loaded bf16 is an f32 value, a loaded i32 an index), which only the generic handlers
+    # and the layer families know
+    if any(p.ty in (BF16, I32) for p in kernel.params):
+        return None
     for name, maybe in (("strided", True), ("matmul_pair", mma), ("matmul", mma), ("matmul_f32", simt_mm),
                         ("attention", top_loop), ("pointwise", flat)):
         if maybe:

@@ -8,7 +8,8 @@ CPU float math), ``exp`` as ``ex2.approx(x * log2 e)`` (the reference's
 lowering, thompiler/handlers/compute.py:77-83 of the reference), ``relu`` as
 ``max(x, 0)``, and a change of dtype (spelled ``copy``) as ``cvt``.
 f16 values compute natively where sm_100a has the instruction and through
-f32 otherwise.
+f32 otherwise.  bf16 is a storage type: its Loads widen to f32 values, its
+Writes round f32 values once.
 """
 
 from __future__ import annotations
@@ -18,7 +19,7 @@ from typing import TYPE_CHECKING
 
 from thompiler import ir
 from thompiler.lowering import address, expr, ops
-from thompiler.lowering.types import F16, F32, I32, REG_VALUE_TYPE, Ty, dtype_of
+from thompiler.lowering.types import BF16, F16, F32, I32, REG_VALUE_TYPE, Ty, dtype_of
 
 if TYPE_CHECKING:
     from thompiler.walk import Walker
@@ -42,12 +43,17 @@ def emit_load(w: "Walker", load: ir.Load) -> None:
     space, addr, ty, readonly = address.access(w, load.input, load.index)
     width = len(load.names)
     check_vector(width, ty, f"Load from {load.input}")
-    regs = [em.value(n, ty.reg) for n in load.names]
+    vals = regs = [em.value(n, F32.reg if ty is BF16 else ty.reg) for n in load.names]
+    if ty is BF16:
+        regs = em.tmps(ty.reg, width)
     op = "ld.global.nc" if (space == "global" and readonly) else f"ld.{space}"
     if width == 1:
         em.ins(f"{op}.{ty.mov} {regs[0]}, [{addr}]")
     else:
         em.ins(f"{op}.v{width}.{ty.mov} {{{', '.join(regs)}}}, [{addr}]")
+    if ty is BF16:
+        for v, r in zip(vals, regs):
+            em.ins(f"{ops.convert(BF16, F32)} {v}, {r}")
 
 
 def arg_type(w: "Walker", name: str) -> Ty:
@@ -80,6 +86,15 @@ def apply_op(w: "Walker", op: str, dst: str, args: list[str], ty: Ty) -> None:
         t = em.tmp("f32")
         em.ins(f"mul.rn.f32 {t}, {args[0]}, {F32.imm(LOG2_E)}")
         em.ins(f"ex2.approx.f32 {dst}, {t}")
+        return
+    if op == "sigmoid":
+        if ty is not F32:
+            raise NotImplementedError(f"sigmoid on {ty.name} values")
+        t, e, s = em.tmps("f32", 3)
+        em.ins(f"mul.rn.f32 {t}, {args[0]}, {F32.imm(-LOG2_E)}")
+        em.ins(f"ex2.approx.f32 {e}, {t}")
+        em.ins(f"add.rn.f32 {s}, {e}, {F32.imm(1.0)}")
+        em.ins(f"rcp.approx.f32 {dst}, {s}")
         return
     if op in ops.UNARY:
         em.ins(f"{ops.instruction(ops.UNARY, op, ty)} {dst}, {args[0]}")
@@ -123,9 +138,15 @@ def emit_write(w: "Walker", wr: ir.Write) -> None:
     space, addr, ty, _ = address.access(w, wr.output, wr.index, wr.swizzle)
     check_vector(width, ty, f"Write to {wr.output}")
     vtys = {arg_type(w, v) for v in wr.values}
-    if vtys != {ty}:
+    if ty is BF16 and vtys == {F32}:
+        values, wide = em.tmps(ty.reg, width), values
+        for r, v in zip(values, wide):
+            em.ins(f"{ops.convert(F32, BF16)} {r}, {v}")
+    elif vtys != {ty}:
         raise TypeError(f"Write to {ty.name} buffer {wr.output} of {sorted(t.name for t in vtys)} values")
     if wr.atomic:
+        if ty is BF16:
+            raise NotImplementedError(f"atomic Write to bf16 buffer {wr.output}")
         if space != "global":
             raise NotImplementedError(f"atomic Write to shared array {wr.output}")
         suffix = "noftz.f16" if ty is F16 else ty.ptx

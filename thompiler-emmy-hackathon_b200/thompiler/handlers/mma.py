@@ -37,7 +37,8 @@ from typing import TYPE_CHECKING
 
 from thompiler import ir
 from thompiler.lowering import address, expr
-from thompiler.lowering.types import E2M1, F16, F32, FRAGMENT_TYPES, UE8M0, Ty, dtype_of
+from thompiler.lowering import ops
+from thompiler.lowering.types import BF16, E2M1, F16, F32, FRAGMENT_TYPES, UE8M0, Ty, dtype_of
 
 if TYPE_CHECKING:
     from thompiler.walk import Walker
@@ -259,7 +260,7 @@ def _to(w: "Walker", reg: str, have: Ty, want: Ty) -> str:
     if have is want:
         return reg
     out = w.em.tmp(want.reg)
-    w.em.ins(f"{'cvt.rn.f16.f32' if want is F16 else 'cvt.f32.f16'} {out}, {reg}")
+    w.em.ins(f"{ops.convert(have, want)} {out}, {reg}")
     return out
 
 
@@ -345,7 +346,7 @@ def emit_reg_store(w: "Walker", st: ir.RegStore) -> None:
     p = w.kernel.param(st.dst_buffer)
     if p is None:
         raise NotImplementedError(f"RegStore to {st.dst_buffer!r}, which is not a kernel parameter")
-    if p.ty not in (F32, F16):
+    if p.ty not in (F32, F16, BF16) or (p.ty is BF16 and st.atomic):
         raise NotImplementedError(f"RegStore to a {p.ty.name} buffer")
     frag, regs = fragment_regs(w, st.frag)
     want = shape[1] // 2 if wide else 4
@@ -406,9 +407,9 @@ def emit_reg_store(w: "Walker", st: ir.RegStore) -> None:
                     continue
                 packed = em.tmp("b32")
                 if vals[0][1] is F32 and vals[1][1] is F32:
-                    em.ins(f"cvt.rn.f16x2.f32 {packed}, {vals[1][0]}, {vals[0][0]}")
+                    em.ins(f"cvt.rn.{p.ty.ptx}x2.f32 {packed}, {vals[1][0]}, {vals[0][0]}")
                 else:
-                    lo, hi = (_to(w, v, ty, F16) for v, ty in vals)
+                    lo, hi = (_to(w, v, ty, p.ty) for v, ty in vals)
                     em.ins(f"mov.b32 {packed}, {{{lo}, {hi}}}")
                 em.ins(f"st.global.b32 [{addr}], {packed}")
                 continue

@@ -6,7 +6,8 @@ explicit rounding mode also stops ptxas from contracting a mul and an add
 into one fma (which rounds once instead of twice).  The transcendental
 ops map to the SFU ``.approx`` forms, as in the reference compiler
 (thompiler/lowering/ops.py:18-99 of the reference); exp is lowered by the
-caller as 2^(x*log2 e).
+caller as 2^(x*log2 e), sigmoid as 1 / (1 + 2^(-x*log2 e)) with the
+approximate reciprocal (1 ulp).
 
 f16 values compute natively (sm_53 and later have .rn f16 add / mul /
 fma and min / max); there is no f16 division, square root or
@@ -91,6 +92,8 @@ CONVERT: dict[tuple[str, str], str] = {
     ("f16", "f32"): "cvt.f32.f16",
     ("f16", "f64"): "cvt.f64.f16",
     ("f32", "f64"): "cvt.f64.f32",
+    ("bf16", "f32"): "cvt.f32.bf16",
+    ("f32", "bf16"): "cvt.rn.bf16.f32",
 }
 
 

@@ -51,6 +51,9 @@ class Ty:
 F16 = Ty("f16", "float", "f16", "b16", "b16", 2)
 F32 = Ty("f32", "float", "f32", "f32", "f32", 4)
 F64 = Ty("f64", "float", "f64", "f64", "f64", 8)
+# bf16 is a storage type: a Load widens the element to f32 (exact) and a Write or RegStore rounds an
+# f32 value once, so no value register ever holds one (as an operand of MmaSyncPtx it stays packed)
+BF16 = Ty("bf16", "float", "bf16", "b16", "b16", 2)
 I32 = Ty("i32", "int", "s32", "s32", "b32", 4)
 I64 = Ty("i64", "int", "s64", "s64", "b64", 8)
 PRED = Ty("pred", "int", "pred", "pred", "pred", 0)
@@ -63,9 +66,11 @@ E2M1 = Ty("e2m1", "float", "e2m1", "b32", "b32", 0)
 UE8M0 = Ty("ue8m0", "int", "ue8m0", "b32", "b32", 1)
 FRAGMENT_TYPES: dict[str, Ty] = {"e2m1": E2M1, "fp4": E2M1, "ue8m0": UE8M0}
 
-# Buffer / value dtypes by IR name: the float types of the problems, and bytes for the
-# block-scaled fp4 statements' packed operands and scales.
-BUFFER_TYPES: dict[str, Ty] = {"f16": F16, "f32": F32, "f64": F64, "u8": U8, "uint8": U8}
+# Buffer / value dtypes by IR name: the float types of the problems, bytes for the block-scaled
+# fp4 statements' packed operands and scales, bf16 (storage), and 32-bit integers (positions and
+# other indices: a loaded element is an index value).
+BUFFER_TYPES: dict[str, Ty] = {"f16": F16, "f32": F32, "f64": F64, "u8": U8, "uint8": U8, "bf16": BF16,
+                               "i32": I32, "int32": I32}
 
 # Smem.dtype is the C element type emmy renders, not an IR dtype.
 SMEM_TYPES: dict[str, Ty] = {"__half": F16, "half": F16, "float": F32, "double": F64,

@@ -31,7 +31,23 @@ from thompiler.compiler import compile_kernel
 from thompiler.load import load
 
 NP_DTYPES = {"f32": np.float32, "f16": np.float16, "f64": np.float64, "i32": np.int32, "i64": np.int64,
-             "u8": np.uint8}
+             "u8": np.uint8, "bf16": np.uint16}      # bf16 arrays hold the bit patterns (numpy has no such type)
+
+
+def to_bf16(x) -> np.ndarray:
+    """f32 values as bf16 bit patterns, rounded to nearest even (NaN stays NaN)."""
+    u = np.ascontiguousarray(x, dtype=np.float32).view(np.uint32)
+    r = ((u.astype(np.uint64) + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(np.asarray(x, dtype=np.float32)), np.uint16(0x7FC0), r)
+
+
+def from_bf16(bits: np.ndarray) -> np.ndarray:
+    """The f32 values of bf16 bit patterns."""
+    return (np.asarray(bits, dtype=np.uint16).astype(np.uint32) << 16).view(np.float32)
+
+
+def _as(values: np.ndarray, dtype: str) -> np.ndarray:
+    return to_bf16(values) if dtype == "bf16" else values.astype(NP_DTYPES[dtype])
 
 
 @dataclass
@@ -61,14 +77,14 @@ def seeded_input(shape, seed: int, dtype: str, init: dict | None = None) -> np.n
     ``normal`` mean/std, ``integers`` low..high inclusive)."""
     shape = list(shape) or [1]
     if init is None:
-        return np.random.default_rng(seed).standard_normal(shape).astype(NP_DTYPES[dtype])
+        return _as(np.random.default_rng(seed).standard_normal(shape), dtype)
     rng = np.random.default_rng(init.get("seed", seed))
     if init["dist"] == "uniform":
-        return rng.uniform(init.get("low", 0.0), init.get("high", 1.0), shape).astype(NP_DTYPES[dtype])
+        return _as(rng.uniform(init.get("low", 0.0), init.get("high", 1.0), shape), dtype)
     if init["dist"] == "integers":
-        return rng.integers(init.get("low", -2), init.get("high", 2) + 1, shape).astype(NP_DTYPES[dtype])
+        return _as(rng.integers(init.get("low", -2), init.get("high", 2) + 1, shape), dtype)
     if init["dist"] == "normal":
-        return (rng.standard_normal(shape) * init.get("std", 1.0) + init.get("mean", 0.0)).astype(NP_DTYPES[dtype])
+        return _as(rng.standard_normal(shape) * init.get("std", 1.0) + init.get("mean", 0.0), dtype)
     raise ValueError(f"input distribution {init['dist']!r}")
 
 
@@ -80,7 +96,7 @@ def make_inputs(pkg: Package) -> dict[str, np.ndarray]:
             if a.get("output") or a.get("intermediate") or a["name"] in out:
                 continue
             if "data" in a:
-                out[a["name"]] = np.asarray(a["data"], dtype=NP_DTYPES[a["dtype"]]).reshape(a["shape"])
+                out[a["name"]] = _as(np.asarray(a["data"]), a["dtype"]).reshape(a["shape"])
             else:
                 out[a["name"]] = seeded_input(a["shape"], a.get("seed", 0), a["dtype"], a.get("init"))
     return out
@@ -139,7 +155,10 @@ def compare(got: np.ndarray, want: np.ndarray, rtol: float, atol: float) -> tupl
 def check_package(pkg: Package, result: dict) -> list[tuple[str, bool, float]]:
     rows = []
     for name, want in (pkg.expected or {}).items():
-        ok, err = compare(result["outputs"][name], want, pkg.meta["rtol"], pkg.meta["atol"])
+        got = result["outputs"][name]
+        if any(a["name"] == name and a["dtype"] == "bf16" for k in pkg.meta["kernels"] for a in k["args"]):
+            got = from_bf16(got)
+        ok, err = compare(got, want, pkg.meta["rtol"], pkg.meta["atol"])
         rows.append((name, ok, err))
     return rows
 

@@ -23,7 +23,7 @@ import dataclasses
 import json
 from pathlib import Path
 
-from thompiler import ir
+from thompiler import ir, schedules
 
 F32T = ir.DataType("f32", "float32", 4)
 F16T = ir.DataType("f16", "float16", 2)
@@ -270,6 +270,141 @@ def matmul_package(outdir, M: int, N: int, K: int, b_layout: str = "col", out_dt
     bexpr = f"torch.randn({N}, {K}, dtype=torch.float16).T" if col else f"torch.randn({K}, {N}, dtype=torch.float16)"
     code = f"(torch.randn({M}, {K}, dtype=torch.float16) @ {bexpr})" + (".float()" if out_dtype == "f32" else "")
     return _write(outdir, f"synth_matmul_{M}x{N}x{K}_{b_layout}", code, entry, g, kmeta, 2e-2, 2e-3)
+
+
+def _layer_write(outdir, pid: str, code: str, entry: str, body, inputs: dict, outputs: dict, grid: int, T: int,
+                 rtol: float, atol: float) -> Path:
+    """A package of one kernel whose args are ``inputs`` then ``outputs`` (name -> (shape, dtype, init or
+    None)), seeded in order."""
+    names = list(outputs)
+    g = _graph({n: (shape, dt) for n, (shape, dt, _) in inputs.items()}, {}, names[0], outputs[names[0]][0], entry,
+               body, dtype=outputs[names[0]][1])
+    g["nodes"][names[0]]["outputs"] += [{"name": n, "shape": list(outputs[n][0]), "dtype": outputs[n][1]}
+                                        for n in names[1:]]
+    g["outputs"] = names
+    args = []
+    for i, (n, (shape, dt, init)) in enumerate(inputs.items()):
+        args.append({"name": n, "dtype": dt, "shape": list(shape), "seed": i})
+        if init:
+            args[-1]["init"] = dict(init, seed=i)
+    args += [{"name": n, "dtype": dt, "shape": list(shape), "output": True} for n, (shape, dt, _) in outputs.items()]
+    kmeta = {"node": names[0], "arg_order": [a["name"] for a in args], "grid": [grid, 1, 1], "block": [T, 1, 1],
+             "smem_bytes": 0, "zero_outputs": [], "args": args}
+    return _write(outdir, pid, code, entry, g, kmeta, rtol, atol)
+
+
+def _positive(**sizes) -> None:
+    for name, v in sizes.items():
+        if not isinstance(v, int) or isinstance(v, bool) or v < 1:
+            raise ValueError(f"{name} = {v!r}: a positive integer expected")
+
+
+def linear_package(outdir, M: int, N: int, K: int, dtype: str = "f16", out_dtype: str | None = None,
+                   bias: bool = False, activation: str | None = None, residual: bool = False,
+                   gated: bool = False) -> Path:
+    """linear[M, N] = act(x[M, K] @ w[N, K]^T + bias) + res, sums in f32 and one rounding to out_dtype.
+
+    x, w, bias[N] and res[M, N] are f16 or bf16 (``dtype``), the output the same or f32; the
+    activation is None, "relu", "silu" or "gelu_tanh".  gated: w[2N, K] and bias[2N] hold two
+    projections, and the result is act(first) * second (+ res).  M is any number of rows from one
+    on; N and K are multiples of 8 (16-byte rows).  The entry is ``k_linear`` over x, w, (bias,)
+    (res,) linear, buffers that do not overlap."""
+    _positive(M=M, N=N, K=K)
+    out_dtype = out_dtype or dtype
+    if dtype not in ("f16", "bf16") or out_dtype not in (dtype, "f32"):
+        raise ValueError(f"linear_package: dtype {dtype!r} -> {out_dtype!r} (f16 or bf16, into the same or f32)")
+    if N % 8 or K % 8:
+        raise ValueError(f"linear_package needs N and K multiples of 8, got N = {N}, K = {K}")
+    rows = 2 * N if gated else N
+    if max(M, rows, K) >= 2 ** 31 - 256:
+        raise ValueError("linear_package: an axis of 2^31 or more")
+    epi = schedules.linear_epilogue(M, N, dtype, bias, activation, residual, gated)
+    body = schedules.linear_body(M, N, K, dtype, gated, epi)
+    inputs = {"x": ((M, K), dtype, None), "w": ((rows, K), dtype, {"dist": "normal", "std": K ** -0.5})}
+    if bias:
+        inputs["bias"] = ((rows,), dtype, None)
+    if residual:
+        inputs["res"] = ((M, N), dtype, None)
+    z = "x @ w.T" + (" + bias" if bias else "")
+    if gated:
+        code = f"z, u = ({z}).chunk(2, -1); {activation or ''}(z) * u" + (" + res" if residual else "")
+    else:
+        code = f"{activation or ''}({z})" + (" + res" if residual else "")
+    # a multiple of 8 CTAs: the tuned kernels run in clusters of 2 to 8, and meta.json's launch is
+    # issued under the module's cluster shape (CTAs past the last tile return at once)
+    tiles = -(-M // 64) * -(-N // 64)
+    return _layer_write(outdir, f"synth_linear_{M}x{N}x{K}", code, "k_linear", body, inputs,
+                        {"linear": ((M, N), out_dtype, None)}, -(-tiles // 8) * 8, 128, 2e-2, 2e-3)
+
+
+def _heads_package(outdir, entry: str, Bn: int, S: int, heads: int, kv_heads: int, D: int, rotary: int | None,
+                   interleaved: bool, dtype: str, table: int, values: bool, heads_first: bool, inverse: bool,
+                   eps: float | None) -> Path:
+    R = D if rotary is None else rotary
+    _positive(B=Bn, S=S, heads=heads, D=D, rotary=R, table=table)
+    if not isinstance(kv_heads, int) or kv_heads < 0:
+        raise ValueError(f"kv_heads = {kv_heads!r}: a non-negative integer expected")
+    if dtype not in ("f16", "bf16", "f32"):
+        raise ValueError(f"{entry}: dtype {dtype!r} (f16, bf16 or f32)")
+    if R % 2 or R > D:
+        raise ValueError(f"{entry}: rotary = {R} of {D} elements (an even number of at most {D})")
+    if values and not kv_heads:
+        raise ValueError(f"{entry}: values without kv_heads")
+    if eps is not None and not eps >= 0:
+        raise ValueError(f"{entry}: eps = {eps!r}")
+    n = heads + kv_heads * (2 if values else 1)
+    if max(Bn, S, n, D, table) >= 2 ** 31:
+        raise ValueError(f"{entry}: an axis of 2^31 or more")
+    body = schedules.heads_body(Bn, S, heads, kv_heads, D, R, table, dtype, interleaved, values, heads_first,
+                                inverse, eps)
+    unit = {"dist": "uniform", "low": -1.0, "high": 1.0}
+    inputs = {"cos": ((table, R // 2), "f32", unit), "sin": ((table, R // 2), "f32", unit),
+              "pos": ((Bn, S), "i32", {"dist": "integers", "low": 0, "high": table - 1}),
+              "qkv": ((Bn, S, n, D), dtype, None)}
+    if eps is not None:
+        weight = {"dist": "uniform", "low": 0.5, "high": 1.5}
+        inputs["wq"] = ((D,), dtype, weight)
+        if kv_heads:
+            inputs["wk"] = ((D,), dtype, weight)
+    outputs = {}
+    for name, m in (("q", heads), ("k", kv_heads), ("v", kv_heads if values else 0)):
+        if m:
+            outputs[name] = ((Bn, m, S, D) if heads_first else (Bn, S, m, D), dtype, None)
+    threads = Bn * S * n * 32
+    if -(-threads // 128) >= 2 ** 31:
+        raise ValueError(f"{entry}: {Bn * S * n} heads are more than a launch holds")
+    tol = (1e-5, 1e-6) if dtype == "f32" else (2e-2, 2e-3)
+    return _layer_write(outdir, f"synth_{entry[2:]}_{Bn}x{S}x{n}x{D}", f"{entry[2:]}(qkv, pos, cos, sin)", entry, body,
+                        inputs, outputs, -(-threads // 128), 128, *tol)
+
+
+def rope_package(outdir, B: int, S: int, heads: int, kv_heads: int, D: int, rotary: int | None = None,
+                 interleaved: bool = False, dtype: str = "f16", table: int = 4096, values: bool = False,
+                 heads_first: bool = False, inverse: bool = False) -> Path:
+    """Rotary positions on the heads of packed rows qkv[B, S, heads + kv_heads (+ kv_heads with
+    ``values``), D] (f16, bf16 or f32), into q[B, S, heads, D], k and v -- or [B, heads, S, D], the
+    attention kernels' layout, with ``heads_first``.
+
+    Of each query and key head the leading ``rotary`` elements (all by default) rotate in pairs
+    (a, b) -> (a cos - b sin, b cos + a sin): (i, i + rotary/2), or neighbours when
+    ``interleaved``.  The angles come from row pos[b, s] (i32) of the tables cos and sin
+    [table, rotary/2] (f32; ``thompiler.rotary.tables`` makes them).  A position outside
+    [0, table) -- an empty slot's -1 -- leaves that token's rows of the outputs as they were.
+    ``inverse`` rotates by the negative angle: the gradient of the rotation.  The entry is
+    ``k_rope`` over cos, sin, pos, qkv, q, (k, (v))."""
+    return _heads_package(outdir, "k_rope", B, S, heads, kv_heads, D, rotary, interleaved, dtype, table, values,
+                          heads_first, inverse, None)
+
+
+def qk_norm_rope_package(outdir, B: int, S: int, heads: int, kv_heads: int, D: int, rotary: int | None = None,
+                         interleaved: bool = False, dtype: str = "f16", table: int = 4096, values: bool = False,
+                         heads_first: bool = False, eps: float = 1e-6) -> Path:
+    """``rope_package`` with each query and key head normalised first, in the same pass:
+    x / sqrt(mean(x^2) + eps) * w over the head's D elements, w = wq[D] or wk[D] (the rows' type).
+    Values are copied as they are.  The entry is ``k_qk_norm_rope`` over cos, sin, pos, qkv, wq,
+    (wk,) q, (k, (v))."""
+    return _heads_package(outdir, "k_qk_norm_rope", B, S, heads, kv_heads, D, rotary, interleaved, dtype, table,
+                          values, heads_first, False, eps)
 
 
 def attention_package(outdir, B: int, H: int, S: int, D: int, dtype: str = "f16", T: int = 128) -> Path:
