@@ -25,11 +25,12 @@ def recognise(kernel: KernelInfo):
     flat = tile is not None and all(isinstance(s, (ir.Load, ir.Assign, ir.Let, ir.Write))
                                     for s in tile.body)                  # pointwise
     simt_mm = ir.CpAsyncCopy in kinds and ir.MmaSyncPtx not in kinds    # f32 matmul on the FMA pipes
-    # storage types (a loaded bf16 is an f32 value, a loaded i32 an index), which only the generic handlers
-    # and the layer families know
-    if any(p.ty in (BF16, I32) for p in kernel.params):
-        return None
-    for name, maybe in (("strided", True), ("matmul_pair", mma), ("matmul", mma), ("matmul_f32", simt_mm),
+    heads = tile is not None and kernel.param("pos") is not None and kernel.param("qkv") is not None
+    layer = [("heads", heads)]
+    # storage types (a loaded bf16 is an f32 value, a loaded i32 an index) are known to the generic
+    # handlers and the layer families only
+    storage = any(p.ty in (BF16, I32) for p in kernel.params)
+    for name, maybe in layer if storage else (*layer, ("strided", True), ("matmul_pair", mma), ("matmul", mma), ("matmul_f32", simt_mm),
                         ("attention", top_loop), ("pointwise", flat)):
         if maybe:
             k = importlib.import_module(f"thompiler.families.{name}").recognise(kernel)
