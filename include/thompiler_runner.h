@@ -165,6 +165,12 @@ int thr_tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const
                   const uint64_t *args, int nargs, uint64_t stream, int *set);
 int thr_tmap_launched(uint64_t module, int set, uint64_t stream);
 
+/* thr_tmap_bind, thr_launch_ex and thr_tmap_launched in one call (a launch that fails reports no
+ * reader): what a caller on device pointers makes for every launch of a kernel with tensor maps. */
+int thr_launch_tmaps(uint64_t module, uint64_t function, const uint32_t grid[3], const uint32_t block[3],
+                     uint32_t smem_bytes, const thr_tmap_spec *tmaps, int ntmaps, const char *ptr_table,
+                     const uint64_t *args, int nargs, uint64_t stream, uint32_t flags);
+
 /* A 2-D..5-D tiled TMA descriptor (CUtensorMap, 128 bytes) for `base`.
  * dtype_code: 0 = f16, 1 = bf16, 2 = f32; swizzle: 0 none, 1 = 32B,
  * 2 = 64B, 3 = 128B.  dims / box innermost first; strides in bytes for

@@ -1,5 +1,5 @@
-"""The layer operators on the GPU, under their own launch and under meta.json's (the generic
-lowering of the same tree), against their float64 definitions.  Outputs lie inside larger buffers
+"""The layer operators on the GPU, under their own launch, under meta.json's and compiled without
+the tuned families (the generic lowering of the same tree), against their float64 definitions.  Outputs lie inside larger buffers
 whose other contents must not change; rows of empty slots keep what they held."""
 
 import numpy as np
@@ -42,7 +42,7 @@ def _np(t):
 
 
 def _kernel(d, launch):
-    return DeviceKernel(next(d.glob("*.ir.json")), honour_meta=launch == "meta")
+    return DeviceKernel(next(d.glob("*.ir.json")), honour_meta=launch == "meta", tuned=launch != "generic")
 
 
 def _linear_inputs(case, seed=0):
@@ -122,7 +122,7 @@ def _heads_check(spec, table, t, out, what):
         check(_np(view), w, allowed, f"{what} {name}")
 
 
-@pytest.mark.parametrize("launch", ["own", "meta"])
+@pytest.mark.parametrize("launch", ["own", "meta", "generic"])
 @pytest.mark.parametrize("case", HEADS, ids=str)
 def test_heads(tmp_path, case, launch):
     import torch

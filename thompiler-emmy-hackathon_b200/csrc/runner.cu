@@ -578,9 +578,15 @@ int thr_launch_ex(uint64_t function, const uint32_t grid[3], const uint32_t bloc
         CUresult r = g_drv.func_set(f, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)smem_bytes);
         if (r != CUDA_SUCCESS) return drv_fail(r, "raising the dynamic shared memory limit");
     }
-    std::vector<uint64_t> vals(args, args + nargs);
-    std::vector<void *> params(nargs);
-    for (int i = 0; i < nargs; ++i) params[i] = &vals[i];
+    // the driver reads each parameter through a pointer to it, during the call
+    void *few[16];
+    std::vector<void *> many;
+    void **params = few;
+    if (nargs > 16) {
+        many.resize(nargs);
+        params = many.data();
+    }
+    for (int i = 0; i < nargs; ++i) params[i] = const_cast<uint64_t *>(&args[i]);
     if ((flags & THR_LAUNCH_OVERLAP_PREVIOUS) && g_drv.launch_ex) {
         // programmatic stream serialisation: the launch may begin while the stream's previous
         // kernel is still running (once that kernel's CTAs signal griddepcontrol.launch_dependents);
@@ -601,11 +607,11 @@ int thr_launch_ex(uint64_t function, const uint32_t grid[3], const uint32_t bloc
         cfg.hStream = (CUstream)(uintptr_t)stream;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        CUresult r = g_drv.launch_ex(&cfg, f, nargs ? params.data() : nullptr, nullptr);
+        CUresult r = g_drv.launch_ex(&cfg, f, nargs ? params : nullptr, nullptr);
         return r == CUDA_SUCCESS ? THR_OK : fail(THR_ERR_RUN, "cuLaunchKernelEx: %s", cu_name(r));
     }
     CUresult r = g_drv.launch(f, grid[0], grid[1], grid[2], block[0], block[1], block[2], smem_bytes,
-                              (CUstream)(uintptr_t)stream, nargs ? params.data() : nullptr, nullptr);
+                              (CUstream)(uintptr_t)stream, nargs ? params : nullptr, nullptr);
     return r == CUDA_SUCCESS ? THR_OK : fail(THR_ERR_RUN, "cuLaunchKernel: %s", cu_name(r));
 }
 
@@ -768,6 +774,15 @@ int thr_tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const
 
 int thr_tmap_launched(uint64_t module, int set, uint64_t stream) {
     return tmap_launched(module, set, (cudaStream_t)(uintptr_t)stream);
+}
+
+int thr_launch_tmaps(uint64_t module, uint64_t function, const uint32_t grid[3], const uint32_t block[3],
+                     uint32_t smem_bytes, const thr_tmap_spec *tmaps, int ntmaps, const char *ptr_table,
+                     const uint64_t *args, int nargs, uint64_t stream, uint32_t flags) {
+    int set = -1;
+    int s = thr_tmap_bind(module, tmaps, ntmaps, ptr_table, args, nargs, stream, &set);
+    if (!s) s = thr_launch_ex(function, grid, block, smem_bytes, args, nargs, stream, flags);
+    return s ? s : thr_tmap_launched(module, set, stream);
 }
 
 int thr_tensor_map(void *out128, int dtype_code, int rank, uint64_t base, const uint64_t *dims,

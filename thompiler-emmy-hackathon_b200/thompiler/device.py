@@ -35,6 +35,7 @@ class DeviceKernel:
         self.plan = runner.plan_launch(self.module, self.kmeta, honour_meta=honour_meta)
         self.arg_order = list(self.kmeta["arg_order"])
         self.tmaps = runner.TensorMaps(self.module, self.plan, self.arg_order) if self.plan.tmaps else None
+        self._launch = runner.Launch(self.fn, self.plan, self.arg_order, self.tmaps)
 
     @property
     def family(self) -> str:
@@ -48,14 +49,7 @@ class DeviceKernel:
         """Launch on device pointers.  A tuned launch whose kernel waits for the previous grid
         before touching global data (``plan.pdl``) is issued as a programmatic dependent launch:
         its CTAs may start, and set up, while the stream's previous kernel finishes."""
-        args = [ptrs[n] for n in self.arg_order]
-        pdl = self.plan.pdl
-        if self.tmaps is None:
-            self.fn.launch(self.plan.grid, self.plan.block, self.plan.smem, args, stream, overlap=pdl)
-            return
-        k = self.tmaps.bind(ptrs, stream)
-        self.fn.launch(self.plan.grid, self.plan.block, self.plan.smem, args, stream, overlap=pdl)
-        self.tmaps.launched(k, stream)
+        self._launch(ptrs, stream)
 
     def error_word(self) -> int:
         """The module's error word (0: no bounded wait gave up, no guarded access was skipped)."""

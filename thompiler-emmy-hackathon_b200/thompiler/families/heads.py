@@ -63,13 +63,16 @@ class RotaryHeads(TunedKernel):
         self.rounds = self._pick_rounds()
         self.units = [-(-h // (self.per_round * self.rounds)) for *_, h in self.segments]
         self.warps_needed = self.T * sum(self.units)
-        self.threads = 256 if self.warps_needed >= 8 * SM_COUNT * 8 else 128
+        self.threads = 128
         self.grid = -(-self.warps_needed // (self.threads // 32))
 
     def _pick_rounds(self) -> int:
-        return next(r for r in (4, 2, 1) if r == 1 or (
-            self.items == 1
-            and self.T * sum(-(-h // (self.per_round * r)) for *_, h in self.segments) >= SM_COUNT * 32))
+        """Two rounds a unit while that leaves a warp for every scheduler, else one.  Measured at 32768 x 80
+        heads of 128 bf16 with norm: one round 292 us (the coefficients' loads and the launch of twice
+        the CTAs), two 225, four 239; at 3 x 1021 x 20 heads of 80: 8.7, 5.8, 6.2.  CTAs of 64, 128 and 256
+        threads: 224, 225, 246 us."""
+        units = self.T * sum(-(-h // (2 * self.per_round)) for *_, h in self.segments)
+        return 2 if self.items == 1 and units >= 4 * SM_COUNT else 1
 
     # ---- recognition ------------------------------------------------------------
 
@@ -346,8 +349,10 @@ class RotaryHeads(TunedKernel):
             ins(f"bra {self.exit}")
             em.place(turned)
 
-        # the tables' entries and the weights of this lane's items
-        cos, sin, weight = [], [], []
+        # the coefficients of this lane's items, packed two elements a register: with the weights folded in,
+        # y_a = n_a (w_a c) - n_b (w_b s) and y_b = n_b (w_b c) + n_a (w_a s), n = x rstd.  An item past the
+        # rotated part has c = 1 and stops at its first product
+        coef = []
         for i in range(self.items):
             q = inside
             for extra in (have[i], turns[i]):
@@ -355,21 +360,26 @@ class RotaryHeads(TunedKernel):
                     q2 = t("pred")
                     ins(f"and.pred {q2}, {q}, {extra}")
                     q = q2
-            for name, dst in (("cos", cos), ("sin", sin)):
+            tab = []
+            for name, other in (("cos", 1.0), ("sin", 0.0)):
                 a, w = t("b64"), t("b64")
                 ins(f"mad.wide.u32 {a}, {pos}, {R // 2 * 4}, {em.buffer_reg(name)}")
                 ins(f"cvt.u64.u32 {w}, {toff[i]}")
                 ins(f"add.u64 {a}, {a}, {w}")
                 regs = em.tmps("f32", V)
                 for x in regs:
-                    ins(f"mov.f32 {x}, {F32.imm(0.0)}")
+                    ins(f"mov.f32 {x}, {F32.imm(other)}")
                 step = min(4, V)
                 for c in range(0, V, step):
                     g = regs[c:c + step]
                     vec, body = (f".v{step}", f"{{{', '.join(g)}}}") if step > 1 else ("", g[0])
                     ins(f"@{q} ld.global.nc{vec}.f32 {body}, [{a}{f'+{4 * c}' if c else ''}]")
-                dst.append(regs)
-            if self.eps is not None:
+                tab.append(regs)
+            cos, sin = tab
+            if self.eps is None:
+                ca = cb = cos
+                sa = sb = sin
+            else:
                 pair = []
                 for off in (off0[i], off1[i]):
                     a, w = t("b64"), t("b64")
@@ -379,56 +389,99 @@ class RotaryHeads(TunedKernel):
                     for x in regs:
                         ins(f"mov.u32 {x}, 0")
                     self._vector("ld.global.nc", regs, a, f"@{have[i]} " if have[i] else "")
-                    pair.append(regs)
-                weight.append([self._unpack(x) for x in pair])
+                    pair.append(self._unpack(regs))
+                wa, wb = self._pairs_of(*pair)
+                ca, sa, cb, sb = ([self._f("mul.rn.f32", x, y) for x, y in zip(ws, tb)]
+                                  for ws, tb in ((wa, cos), (wa, sin), (wb, cos), (wb, sin)))
+            # the subtracted product's sine enters negated (the other one's for the inverse rotation)
+            if self.inverse:
+                sa = [self._f("neg.f32", x) for x in sa]
+            else:
+                sb = [self._f("neg.f32", x) for x in sb]
+            coef.append([self._twos(x) for x in (ca, sa, cb, sb)])
 
         for r in range(self.rounds):
-            vals = [[self._unpack(x) for x in raw[r][i]] for i in range(self.items)]
+            vals = [[self._twos(h) for h in self._pairs_of(*(self._unpack(x) for x in raw[r][i]))]
+                    for i in range(self.items)]
             if self.eps is not None:
-                acc = t("f32")
-                ins(f"mov.f32 {acc}, {F32.imm(0.0)}")
+                acc = t("b64")
+                ins(f"mov.b64 {acc}, 0")
                 for pair in vals:
                     for x in pair[0] + pair[1]:
-                        ins(f"fma.rn.f32 {acc}, {x}, {x}, {acc}")
+                        ins(f"fma.rn.f32x2 {acc}, {x}, {x}, {acc}")
+                lo, hi, rstd = t("f32"), t("f32"), t("f32")
+                ins(f"mov.b64 {{{lo}, {hi}}}, {acc}")
+                if V > 1:
+                    ins(f"add.rn.f32 {rstd}, {lo}, {hi}")
+                else:                                          # one element a register, doubled
+                    ins(f"mov.f32 {rstd}, {lo}")
                 step = self.lanes // 2
                 while step:
                     o = t("f32")
-                    ins(f"shfl.sync.bfly.b32 {o}, {acc}, {step}, 0x1f, 0xffffffff")
-                    ins(f"add.rn.f32 {acc}, {acc}, {o}")
+                    ins(f"shfl.sync.bfly.b32 {o}, {rstd}, {step}, 0x1f, 0xffffffff")
+                    ins(f"add.rn.f32 {rstd}, {rstd}, {o}")
                     step //= 2
-                rstd = t("f32")
-                ins(f"div.rn.f32 {rstd}, {acc}, {F32.imm(float(D))}")
+                ins(f"mul.rn.f32 {rstd}, {rstd}, {F32.imm(1.0 / D)}")
                 ins(f"add.rn.f32 {rstd}, {rstd}, {F32.imm(float(self.eps))}")
-                ins(f"sqrt.rn.f32 {rstd}, {rstd}")
-                ins(f"rcp.rn.f32 {rstd}, {rstd}")
-                for i, pair in enumerate(vals):
-                    for half, ws in zip(pair, weight[i]):
-                        for m, (x, wv) in enumerate(zip(half, ws)):
-                            y = t("f32")
-                            ins(f"mul.rn.f32 {y}, {x}, {rstd}")
-                            ins(f"mul.rn.f32 {y}, {y}, {wv}")
-                            half[m] = y
-            for i, (h0, h1) in enumerate(vals):
-                flat = h0 + h1
-                new = list(flat)
-                for m in range(V):
-                    ia, ib = (2 * m, 2 * m + 1) if self.interleaved else (m, V + m)
-                    a, b, c, s = flat[ia], flat[ib], cos[i][m], sin[i][m]
-                    ya, yb, bs, as_ = t("f32"), t("f32"), t("f32"), t("f32")
-                    ins(f"mul.rn.f32 {bs}, {b}, {s}")
-                    ins(f"mul.rn.f32 {as_}, {a}, {s}")
-                    if self.inverse:
-                        ins(f"fma.rn.f32 {ya}, {a}, {c}, {bs}")
-                        ins(f"neg.f32 {as_}, {as_}")
-                    else:
-                        ins(f"neg.f32 {bs}, {bs}")
-                        ins(f"fma.rn.f32 {ya}, {a}, {c}, {bs}")
-                    ins(f"fma.rn.f32 {yb}, {b}, {c}, {as_}")
+                ins(f"rsqrt.approx.f32 {rstd}, {rstd}")        # relative error at most 2^-22.9
+                rr = t("b64")
+                ins(f"mov.b64 {rr}, {{{rstd}, {rstd}}}")
+                for pair in vals:
+                    for half in pair:
+                        for m, x in enumerate(half):
+                            half[m] = t("b64")
+                            ins(f"mul.rn.f32x2 {half[m]}, {x}, {rr}")
+            for i, (na, nb_) in enumerate(vals):
+                out_a, out_b = [], []
+                for m, (a, b) in enumerate(zip(na, nb_)):
+                    ca, sa, cb, sb = (c[m] for c in coef[i])
+                    pa_, pb_, ya, yb = t("b64"), t("b64"), t("b64"), t("b64")
+                    ins(f"mul.rn.f32x2 {pa_}, {a}, {ca}")
+                    ins(f"mul.rn.f32x2 {pb_}, {b}, {cb}")
+                    ins(f"fma.rn.f32x2 {ya}, {b}, {sb}, {pa_}")
+                    ins(f"fma.rn.f32x2 {yb}, {a}, {sa}, {pb_}")
                     if turns[i]:
-                        ins(f"selp.f32 {ya}, {ya}, {a}, {turns[i]}")
-                        ins(f"selp.f32 {yb}, {yb}, {b}, {turns[i]}")
-                    new[ia], new[ib] = ya, yb
-                store(r, i, (self._pack(new[:V]), self._pack(new[V:])))
+                        ins(f"selp.b64 {ya}, {ya}, {pa_}, {turns[i]}")
+                        ins(f"selp.b64 {yb}, {yb}, {pb_}, {turns[i]}")
+                    out_a.append(ya)
+                    out_b.append(yb)
+                v0, v1 = self._vectors_of(self._ones(out_a), self._ones(out_b))
+                store(r, i, (self._pack(v0), self._pack(v1)))
+
+    def _f(self, op: str, *args: str) -> str:
+        r = self.em.tmp("f32")
+        self.em.ins(f"{op} {r}, {', '.join(args)}")
+        return r
+
+    def _twos(self, vals: list[str]) -> list[str]:
+        """f32 values two to a 64-bit register (an odd one doubled), for the f32x2 instructions."""
+        out = []
+        for m in range(0, len(vals), 2):
+            out.append(self.em.tmp("b64"))
+            self.em.ins(f"mov.b64 {out[-1]}, {{{vals[m]}, {vals[min(m + 1, len(vals) - 1)]}}}")
+        return out
+
+    def _ones(self, twos: list[str]) -> list[str]:
+        out = []
+        for x in twos:
+            lo, hi = self.em.tmp("f32"), self.em.tmp("f32")
+            self.em.ins(f"mov.b64 {{{lo}, {hi}}}, {x}")
+            out += [lo, hi]
+        return out[:self.V]
+
+    def _pairs_of(self, v0: list, v1: list) -> tuple[list, list]:
+        """The pairs' first and second elements of a lane's two vectors."""
+        if not self.interleaved:
+            return v0, v1
+        flat = v0 + v1
+        return flat[0::2], flat[1::2]
+
+    def _vectors_of(self, a: list, b: list) -> tuple[list, list]:
+        """The two vectors that hold the pairs' first and second elements ``a`` and ``b``."""
+        if not self.interleaved:
+            return a, b
+        flat = [x for ab in zip(a, b) for x in ab]
+        return flat[:self.V], flat[self.V:]
 
 
 def recognise(kernel: KernelInfo):

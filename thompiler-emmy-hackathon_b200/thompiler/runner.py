@@ -97,6 +97,8 @@ def library() -> ctypes.CDLL:
             "thr_tmap_bind": ([u64, ctypes.POINTER(ThrTmapSpec), i32, ctypes.c_char_p, ctypes.POINTER(u64), i32,
                                u64, ctypes.POINTER(i32)], i32),
             "thr_tmap_launched": ([u64, i32, u64], i32),
+            "thr_launch_tmaps": ([u64, u64, u32x3, u32x3, ctypes.c_uint32, ctypes.POINTER(ThrTmapSpec), i32,
+                                  ctypes.c_char_p, ctypes.POINTER(u64), i32, u64, ctypes.c_uint32], i32),
             "thr_peer_alloc": ([u64, ctypes.POINTER(u64), ctypes.c_char_p], i32),
             "thr_peer_open": ([ctypes.c_char_p, ctypes.POINTER(u64)], i32),
             "thr_peer_close": ([u64], i32),
@@ -295,6 +297,38 @@ class TensorMaps:
 
     def launched(self, set_: int, stream: int = 0) -> None:
         check(library().thr_tmap_launched(self.module.handle, int(set_), int(stream)), "tensor maps")
+
+
+class Launch:
+    """One kernel's launches on device pointers, with everything that stays the same from call to call
+    converted once: ``launch(ptrs, stream)`` is one C call (with its tensor maps' binding, when the
+    plan has any).  ``plan``'s grid, block and shared memory are read again whenever they are
+    replaced."""
+
+    def __init__(self, function: Function, plan: LaunchPlan, arg_order: list[str], tmaps: TensorMaps | None):
+        self.function, self.plan, self.order, self.tmaps = function, plan, tuple(arg_order), tmaps
+        self.n = len(self.order)
+        self._array = ctypes.c_uint64 * max(1, self.n)
+        lib = library()
+        self._plain, self._mapped = lib.thr_launch_ex, lib.thr_launch_tmaps
+        self._geometry = None
+
+    def __call__(self, ptrs: dict[str, int], stream: int = 0) -> None:
+        plan, f = self.plan, self.function
+        geometry = (plan.grid, plan.block, plan.smem)
+        if geometry != self._geometry:
+            self._dims = (_dims(plan.grid), _dims(plan.block), int(plan.smem), OVERLAP_PREVIOUS if plan.pdl else 0)
+            self._geometry = geometry
+        grid, block, smem, flags = self._dims
+        args = self._array(*[ptrs[n] for n in self.order])
+        if self.tmaps is None:
+            st = self._plain(f.handle, grid, block, smem, args, self.n, stream, flags)
+        else:
+            t = self.tmaps
+            st = self._mapped(t.module.handle, f.handle, grid, block, smem, t.specs, t.n, t.table, args, self.n,
+                              stream, flags)
+        if st:
+            check(st, f"launch of {f.name}")
 
 
 def read_error_word(module: Module, plan: LaunchPlan) -> int:
