@@ -66,7 +66,7 @@ def _linear_check(case, t, got, what):
     check(_np(got), want, allowed, what)
 
 
-@pytest.mark.parametrize("launch", ["own", "meta"])
+@pytest.mark.parametrize("launch", ["own", "meta", "generic"])
 @pytest.mark.parametrize("case", LINEAR, ids=str)
 def test_linear(tmp_path, case, launch):
     import torch

@@ -26,12 +26,14 @@ def recognise(kernel: KernelInfo):
                                     for s in tile.body)                  # pointwise
     simt_mm = ir.CpAsyncCopy in kinds and ir.MmaSyncPtx not in kinds    # f32 matmul on the FMA pipes
     heads = tile is not None and kernel.param("pos") is not None and kernel.param("qkv") is not None
-    layer = [("heads", heads)]
+    linear = mma and kernel.param("linear") is not None
+    layer = (("heads", heads), ("linear", linear))
     # storage types (a loaded bf16 is an f32 value, a loaded i32 an index) are known to the generic
     # handlers and the layer families only
     storage = any(p.ty in (BF16, I32) for p in kernel.params)
-    for name, maybe in layer if storage else (*layer, ("strided", True), ("matmul_pair", mma), ("matmul", mma), ("matmul_f32", simt_mm),
-                        ("attention", top_loop), ("pointwise", flat)):
+    others = (("strided", True), ("matmul_pair", mma), ("matmul", mma), ("matmul_f32", simt_mm),
+              ("attention", top_loop), ("pointwise", flat))
+    for name, maybe in layer if storage else layer + others:
         if maybe:
             k = importlib.import_module(f"thompiler.families.{name}").recognise(kernel)
             if k is not None:

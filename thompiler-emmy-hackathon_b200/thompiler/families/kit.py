@@ -5,7 +5,7 @@
   version (1 on sm_100), 61-63 layout (2 = 128-byte swizzle) -- the layout
   CUTLASS documents for sm100 UMMA descriptors;
 * the kind::f16 instruction descriptor (32-bit): D format (f32 = 1) at bit 4,
-  A / B formats at 7 / 10 (f16 = 0), A / B major-ness at 15 / 16 (1 =
+  A / B formats at 7 / 10 (f16 = 0, bf16 = 1), A / B major-ness at 15 / 16 (1 =
   MN-major), N >> 3 at bit 17, M >> 4 at bit 24;
 * bounded mbarrier waits: every wait gives up after ``WAIT_LIMIT`` rounds of
   ``mbarrier.try_wait``, records a code in the module's error word and jumps
@@ -90,9 +90,10 @@ def desc_hi(sbo: int, layout: int = SWIZZLE_128B) -> int:
     return ((sbo >> 4) & 0x3FFF) | (1 << 14) | (layout << 29)
 
 
-def idesc_f16(m: int, n: int, a_mn_major: bool = False, b_mn_major: bool = False) -> int:
-    """kind::f16 instruction descriptor: f16 A and B, f32 accumulator."""
-    return ((1 << 4) | ((1 if a_mn_major else 0) << 15) | ((1 if b_mn_major else 0) << 16)
+def idesc_f16(m: int, n: int, a_mn_major: bool = False, b_mn_major: bool = False, bf16: bool = False) -> int:
+    """kind::f16 instruction descriptor: f16 (or bf16) A and B, f32 accumulator."""
+    ab = (1 << 7) | (1 << 10) if bf16 else 0
+    return ((1 << 4) | ab | ((1 if a_mn_major else 0) << 15) | ((1 if b_mn_major else 0) << 16)
             | ((n >> 3) << 17) | ((m >> 4) << 24))
 
 

@@ -203,16 +203,16 @@ class TcMatmul(TunedKernel):
 
     def sidecar(self) -> dict:
         a, b = self.a, self.b
-        tm_a = {"global": TMAP_RING, "param": a.name, "dtype": "f16", "dims": [self.K, self.M],
+        tm_a = {"global": TMAP_RING, "param": a.name, "dtype": a.ty.name, "dims": [self.K, self.M],
                 "strides": [self.K * 2], "box": [BK, BM], "swizzle": 3}
         if self.b_kmajor:
-            tm_b = {"global": TMAP_RING, "param": b.name, "dtype": "f16", "dims": [self.K, self.N],
+            tm_b = {"global": TMAP_RING, "param": b.name, "dtype": b.ty.name, "dims": [self.K, b.shape[0]],
                     "strides": [self.K * 2], "box": [BK, self.BN], "swizzle": 3}
         else:
-            tm_b = {"global": TMAP_RING, "param": b.name, "dtype": "f16", "dims": [self.N, self.K],
+            tm_b = {"global": TMAP_RING, "param": b.name, "dtype": b.ty.name, "dims": [self.N, self.K],
                     "strides": [self.N * 2], "box": [64, BK], "swizzle": 3}
         esz = self.c.ty.nbytes
-        tm_c = {"global": TMAP_RING, "param": self.c.name, "dtype": "f32" if esz == 4 else "f16",
+        tm_c = {"global": TMAP_RING, "param": self.c.name, "dtype": self.c.ty.name,
                 "dims": [self.N, self.S * self.M], "strides": [self.N * esz], "box": [64 // esz, 32],
                 "swizzle": 2}
         side = {"grid": [self.ctas, 1, 1], "block": [THREADS, 1, 1], "smem_bytes": self.smem,

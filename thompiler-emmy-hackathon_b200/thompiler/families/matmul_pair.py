@@ -33,7 +33,7 @@ from thompiler.families.matmul import BK, BM, EPI_WARPS, SM_COUNT, STAGE_TILE, T
 from thompiler.families.base import TunedKernel
 from thompiler.families.tuning import TUNING
 from thompiler.load import KernelInfo
-from thompiler.lowering.types import F32
+from thompiler.lowering.types import BF16, F32
 
 PM = 2 * BM                  # rows of a pair tile
 PAIR_SLOTS = SM_COUNT // 2   # pairs resident at once
@@ -48,6 +48,7 @@ SMEM_LIMIT = 227 * 1024
 class TcMatmulPair(TcMatmul):
     family = "tcgen05-matmul-pair"
     tail_ranks = 2
+    epilogue = None              # a RegStore epilogue to apply (thompiler.families.linear)
 
     @classmethod
     def match(cls, kernel: KernelInfo):
@@ -99,10 +100,13 @@ class TcMatmulPair(TcMatmul):
         if 2 <= forced <= room // stage:
             self.stages = forced
         self.smem = self.stages * stage + self.staging + 1024 + 256
-        self.tiles = (M // PM) * (N // bn) * S
+        self.tiles_m, self.tiles_n, self.kblocks = M // PM, N // bn, self.Ks // BK
+        self.tile_cols = bn                                  # columns of C in a tile, and of B between tiles
+        self.rank_cols = self.HN                             # rows of B between the CTAs of a pair
+        self.tiles = self.tiles_m * self.tiles_n * S
         # the last, partial wave of pair tiles: its `rem` tiles are cut along K into `parts` units,
         # as in the single-CTA kernel (each CTA of a pair keeps its own partial and counter)
-        kblocks = self.Ks // BK
+        kblocks = self.kblocks
         rem0 = self.tiles % PAIR_SLOTS if self.tiles > PAIR_SLOTS else 0
         # the partial last wave: where its tiles halved fit one wave of pairs, each 256-wide tile
         # becomes two 256 x 128 units over the full K (no partials; measured faster than the K
@@ -138,6 +142,13 @@ class TcMatmulPair(TcMatmul):
         super().guard(generic)
         self.em.entry_attrs.append(".reqnctapercluster 2, 1, 1")
 
+    def tile_begin(self, row: str, rank: str, tm: str, tn: str, whole: str, part: str) -> None:
+        """Hook: an epilogue thread (its row of the CTA's 128) is about to wait for a tile's sums."""
+
+    def box(self, c0: int, cw: int, width: int, taddr: str) -> list[str]:
+        """Hook: columns c0 .. c0 + cw of this thread's row after ``epilogue``, packed for a store."""
+        raise NotImplementedError
+
     # ---- the tuned body -------------------------------------------------------------
 
     def emit_tuned(self) -> None:  # noqa: C901 - one kernel, written out in order
@@ -145,8 +156,8 @@ class TcMatmulPair(TcMatmul):
         t, ins, place, lab = em.tmp, em.ins, em.place, em.label
         BN, HN, ST = self.BN, self.HN, self.stages
         a_bytes, b_bytes = self.a_bytes, self.b_bytes
-        tiles_m, tiles_n = self.M // PM, self.N // BN
-        kblocks = self.Ks // BK
+        tiles_m, tiles_n, kblocks = self.tiles_m, self.tiles_n, self.kblocks
+        bf16 = self.a.ty is BF16
         mcommit = "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
         tma_ld = "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
         self.pdl_trigger()
@@ -275,14 +286,14 @@ class TcMatmulPair(TcMatmul):
         m0, n0, k0 = t("b32"), t("b32"), t("b32")
         ins(f"mul.lo.u32 {m0}, {tm_}, {PM}")
         ins(f"mad.lo.u32 {m0}, {rank}, {BM}, {m0}")
-        ins(f"mul.lo.u32 {n0}, {tn_}, {BN}")
+        ins(f"mul.lo.u32 {n0}, {tn_}, {self.tile_cols}")
         if self.hrem:
             # half unit h: columns 128 h .. of the tile, 64 per CTA; the box still spans 128 rows
             # (the second 64 are not read; past N they are the tensor map's zero fill)
             nh = t("b32")
             ins(f"mad.lo.u32 {nh}, {ppart}, {BN // 2}, {n0}")
             ins(f"mad.lo.u32 {nh}, {rank}, {HN // 2}, {nh}")
-        ins(f"mad.lo.u32 {n0}, {rank}, {HN}, {n0}")
+        ins(f"mad.lo.u32 {n0}, {rank}, {self.rank_cols}, {n0}")
         if self.hrem:
             ins(f"@!{pwhole} mov.u32 {n0}, {nh}")
         ins(f"mul.lo.u32 {k0}, {ts_}, {self.Ks}")
@@ -324,7 +335,7 @@ class TcMatmulPair(TcMatmul):
         elect_one(em, ism)
         hi = t("b32")
         ins(f"mov.u32 {hi}, {desc_hi(1024)}")
-        idesc = idesc_f16(PM, BN, b_mn_major=not self.b_kmajor)
+        idesc = idesc_f16(PM, BN, b_mn_major=not self.b_kmajor, bf16=bf16)
         zero = t("b32")
         ins(f"mov.u32 {zero}, 0")
         always, never = t("pred"), t("pred")
@@ -342,7 +353,7 @@ class TcMatmulPair(TcMatmul):
         idr = t("b32")
         ins(f"mov.u32 {idr}, {idesc}")
         if self.hrem:
-            ins(f"@!{mwhole} mov.u32 {idr}, {idesc_f16(PM, BN // 2, b_mn_major=not self.b_kmajor)}")
+            ins(f"@!{mwhole} mov.u32 {idr}, {idesc_f16(PM, BN // 2, b_mn_major=not self.b_kmajor, bf16=bf16)}")
         kfirst = t("b32")
         ins(f"mov.u32 {kfirst}, {kb2}")
         buf, ab = t("b32"), t("b32")
@@ -420,6 +431,7 @@ class TcMatmulPair(TcMatmul):
         place(etop)
         tile3, _, _, whole3, part3 = unit(eu)
         tm3, tn3, ts3 = decode(tile3)
+        self.tile_begin(row, rank, tm3, tn3, whole3, part3)
         buf3, ab3, lab3 = t("b32"), t("b32"), t("b32")
         ins(f"and.b32 {buf3}, {lt3}, 1")
         ins(f"mad.lo.u32 {ab3}, {buf3}, 8, {bars}")
@@ -438,7 +450,7 @@ class TcMatmulPair(TcMatmul):
         ins(f"mad.lo.u32 {row0}, {tm3}, {PM}, {row0}")
         ins(f"mad.lo.u32 {row0}, {rank}, {BM}, {row0}")
         ins(f"mad.lo.u32 {row0}, {quarter}, 32, {row0}")
-        ins(f"mul.lo.u32 {col0}, {tn3}, {BN}")
+        ins(f"mul.lo.u32 {col0}, {tn3}, {self.tile_cols}")
 
         def free_accumulator() -> None:
             """This warp has read the accumulator out: one arrival on the leader's barrier."""
@@ -446,7 +458,7 @@ class TcMatmulPair(TcMatmul):
             ins("bar.warp.sync -1")
             ins(f"@{lane0} mbarrier.arrive.release.cluster.shared::cluster.b64 _, [{lab3}+{acce_off}]")
 
-        def store_boxes(values, free_after_last: bool, width: int = BN) -> None:
+        def store_boxes(values, free_after_last: bool, width: int = self.tile_cols) -> None:
             """Columns c0 .. c0 + cw of this warp's 32 rows, for each c0 < width: ``values(c0)``
             gives the row's cw values as b32 registers (f32, or f16 pairs), staged (64-byte
             swizzle) and stored with TMA."""
@@ -469,7 +481,9 @@ class TcMatmulPair(TcMatmul):
                     f"[{sbuf}]")
                 ins(f"@{lane0} cp.async.bulk.commit_group")
 
-        def from_tmem(c0):
+        def from_tmem(c0, width=self.tile_cols):
+            if self.epilogue is not None:
+                return self.box(c0, cw, width, taddr)
             nv = 16 if esz == 4 else 32
             v = [t("b32") for _ in range(nv)]
             tc = t("b32")
@@ -479,7 +493,7 @@ class TcMatmulPair(TcMatmul):
             if esz == 2:
                 h = [t("b32") for _ in range(16)]
                 for i in range(16):
-                    ins(f"cvt.rn.f16x2.f32 {h[i]}, {v[2 * i + 1]}, {v[2 * i]}")
+                    ins(f"cvt.rn.{self.c.ty.ptx}x2.f32 {h[i]}, {v[2 * i + 1]}, {v[2 * i]}")
                 v = h
             return v
 
@@ -492,7 +506,7 @@ class TcMatmulPair(TcMatmul):
             ins(f"bra {enext}")
             place(tail)
             ins(f"mad.lo.u32 {col0}, {part3}, {BN // 2}, {col0}")
-            store_boxes(from_tmem, True, BN // 2)
+            store_boxes(lambda c0: from_tmem(c0, BN // 2), True, BN // 2)
         if self.rem:
             ins(f"bra {enext}")
             self._pair_tail(tail, enext, tile3, part3, rank, taddr, row, bars, ls, store_boxes, free_accumulator,

@@ -273,7 +273,7 @@ def matmul_package(outdir, M: int, N: int, K: int, b_layout: str = "col", out_dt
 
 
 def _layer_write(outdir, pid: str, code: str, entry: str, body, inputs: dict, outputs: dict, grid: int, T: int,
-                 rtol: float, atol: float) -> Path:
+                 rtol: float, atol: float, smem: int = 0) -> Path:
     """A package of one kernel whose args are ``inputs`` then ``outputs`` (name -> (shape, dtype, init or
     None)), seeded in order."""
     names = list(outputs)
@@ -289,7 +289,7 @@ def _layer_write(outdir, pid: str, code: str, entry: str, body, inputs: dict, ou
             args[-1]["init"] = dict(init, seed=i)
     args += [{"name": n, "dtype": dt, "shape": list(shape), "output": True} for n, (shape, dt, _) in outputs.items()]
     kmeta = {"node": names[0], "arg_order": [a["name"] for a in args], "grid": [grid, 1, 1], "block": [T, 1, 1],
-             "smem_bytes": 0, "zero_outputs": [], "args": args}
+             "smem_bytes": smem, "zero_outputs": [], "args": args}
     return _write(outdir, pid, code, entry, g, kmeta, rtol, atol)
 
 
@@ -334,7 +334,8 @@ def linear_package(outdir, M: int, N: int, K: int, dtype: str = "f16", out_dtype
     # issued under the module's cluster shape (CTAs past the last tile return at once)
     tiles = -(-M // 64) * -(-N // 64)
     return _layer_write(outdir, f"synth_linear_{M}x{N}x{K}", code, "k_linear", body, inputs,
-                        {"linear": ((M, N), out_dtype, None)}, -(-tiles // 8) * 8, 128, 2e-2, 2e-3)
+                        {"linear": ((M, N), out_dtype, None)}, -(-tiles // 8) * 8, 128, 2e-2, 2e-3,
+                        smem=(3 if gated else 2) * 64 * 64 * 2)
 
 
 def _heads_package(outdir, entry: str, Bn: int, S: int, heads: int, kv_heads: int, D: int, rotary: int | None,
