@@ -8,6 +8,7 @@ import pytest
 from layer_cases import HEADS, LINEAR, check, heads_expected, heads_package, heads_spec, linear_expected
 from thompiler import synth
 from thompiler.device import DeviceKernel
+from thompiler.families.tuning import TUNING
 
 pytestmark = pytest.mark.gpu
 
@@ -66,12 +67,17 @@ def _linear_check(case, t, got, what):
     check(_np(got), want, allowed, what)
 
 
-@pytest.mark.parametrize("launch", ["own", "meta", "generic"])
+@pytest.mark.parametrize("launch", ["own", "meta", "generic", "rows", "pair"])
 @pytest.mark.parametrize("case", LINEAR, ids=str)
-def test_linear(tmp_path, case, launch):
+def test_linear(tmp_path, monkeypatch, case, launch):
+    """``rows`` and ``pair`` force one of the two tuned kernels, also at sizes it is not chosen for."""
     import torch
     M, N = case[:2]
+    if launch in ("rows", "pair"):
+        monkeypatch.setattr(TUNING, "linear_kernel", launch)
     k = _kernel(synth.linear_package(tmp_path, *case), launch)
+    if launch in ("rows", "pair") and not k.family.endswith(launch):
+        pytest.skip(f"no {launch} plan for this size")
     t = _linear_inputs(case)
     whole, y = _out((M, N), case[4])
     ptrs = {n: v.data_ptr() for n, v in dict(t, linear=y).items()}

@@ -35,7 +35,7 @@ class DeviceKernel:
         self.plan = runner.plan_launch(self.module, self.kmeta, honour_meta=honour_meta)
         self.arg_order = list(self.kmeta["arg_order"])
         self.tmaps = runner.TensorMaps(self.module, self.plan, self.arg_order) if self.plan.tmaps else None
-        self._launch = runner.Launch(self.fn, self.plan, self.arg_order, self.tmaps)
+        self._launch = runner.Launch(self.fn, self.plan, self.kmeta, self.tmaps)
 
     @property
     def family(self) -> str:

@@ -21,7 +21,8 @@ from __future__ import annotations
 
 from thompiler import ir, schedules
 from thompiler.families.base import TunedKernel
-from thompiler.families.matmul import BK, BM, EPI_WARPS, STAGE_TILE
+from thompiler.families.kit import Kit, desc_hi, elect_one, idesc_f16
+from thompiler.families.matmul import BK, BM, EPI_WARPS, SM_COUNT, STAGE_TILE
 from thompiler.families.matmul_pair import PAIR_SLOTS, PAIR_WIDTHS, PM, SMEM_LIMIT, TcMatmulPair
 from thompiler.families.tuning import TUNING
 from thompiler.load import KernelInfo
@@ -217,6 +218,11 @@ class LinearPair(TcMatmulPair):
             out.append((time * bn / 256 / pref, bn, rem if half else 0))
         return out
 
+    def estimate(self) -> float:
+        """Microseconds, as ``RowsPlan.estimate``: a 256-wide tile's K block takes about 0.28."""
+        memory = self.p.w.nbytes / 5.5e6
+        return max(memory, min(self.plans(self.p))[0] * self.kblocks * 0.28) + 8
+
     def guard(self, generic: str) -> None:
         super().guard(generic)
         if self.replay:
@@ -314,10 +320,554 @@ class LinearPair(TcMatmulPair):
         return packed
 
 
+# ---- few rows ----------------------------------------------------------------------------
+
+ROW_SLAB = BM * BK * 2                       # one 128 x 64 slab of w
+EXCHANGE_LIMIT = 64 * 1024                   # shared memory for the partial sums of a cut K
+PRODUCERS = 128
+
+
+class LinearRows(TunedKernel):
+    """Few rows of x against all of w, bound by reading w once.  The roles are turned: 128 rows of w are
+    the tensor cores' M side and ``BT`` rows of x (16 .. 256, exactly the batch rounded up) the N
+    side, so a small batch wastes no tensor-core rows and w streams through in its own layout.
+
+    K is cut among the ``S`` CTAs of a cluster so that every SM has w to read; each CTA sends its
+    partial sums to the CTA that owns those rows of w through distributed shared memory, which adds
+    them in rank order (no atomics: the same bits every time), applies the epilogue and stores.
+
+    Four warps copy both operands with 16-byte cp.async into the 128-byte swizzle -- no tensor maps, so
+    nothing is kept for a buffer's address, and any number of weights share the kernel in captured
+    graphs -- and finish a stage with a proxy fence and an arrival on its mbarrier; a fifth warp issues
+    the MMAs.  Out-of-range rows and K are zero-filled by the copies.  Every wait is bounded."""
+
+    family = "tcgen05-linear-rows"
+
+    def __init__(self, p: Product, plan: "RowsPlan"):
+        super().__init__(p.kernel)
+        self.p, self.plan = p, plan
+        self.replay = Replay(self, p) if p.epilogue is not None else None
+
+    def sidecar(self) -> dict:
+        pl = self.plan
+        return {"grid": [pl.ctas, 1, 1], "block": [PRODUCERS + 32, 1, 1], "smem_bytes": pl.smem,
+                "error_word": "thc_error", "cluster": [pl.S, 1, 1], "tile": [BM, pl.BT, BK], "stages": pl.stages}
+
+    def guard(self, generic: str) -> None:
+        em = self.em
+        em.module(".global .align 4 .u32 thc_error")
+        em.module(".extern .shared .align 1024 .b8 smem_pool[]")
+        if self.plan.S > 1:
+            em.entry_attrs.append(f".reqnctapercluster {self.plan.S}, 1, 1")
+        q = em.tmp("pred")
+        em.ins(f"setp.ne.u32 {q}, {self.special('%ntid.x')}, {PRODUCERS + 32}")
+        em.ins(f"@{q} bra {generic}")
+        em.ins(f"setp.ne.u32 {q}, {self.special('%nctaid.x')}, {self.plan.ctas}")
+        em.ins(f"@{q} bra {generic}")
+
+    def emit_tuned(self) -> None:  # noqa: C901 - one kernel, written out in order
+        em, t, ins, place, lab = self.em, self.em.tmp, self.em.ins, self.em.place, self.em.label
+        p, pl = self.p, self.plan
+        S, BT, ST, G = pl.S, pl.BT, pl.stages, pl.G
+        stage_bytes = pl.stage_bytes
+        q = t("pred")
+        tid, warp, lane = self.special("%tid.x"), t("b32"), t("b32")
+        ins(f"shr.u32 {warp}, {tid}, 5")
+        ins(f"and.b32 {lane}, {tid}, 31")
+        base = t("b32")
+        ins(f"mov.u32 {base}, smem_pool")
+        ins(f"add.u32 {base}, {base}, 1023")
+        ins(f"and.b32 {base}, {base}, -1024")
+        # shared: stages (w slabs | x rows) | exchange | barriers (full, empty per stage; sums done) | TMEM slot
+        ex, bars = t("b32"), t("b32")
+        ins(f"add.u32 {ex}, {base}, {ST * stage_bytes}")
+        ins(f"add.u32 {bars}, {ex}, {pl.exchange}")
+        empty_off, done_off, slot_off = 8 * ST, 16 * ST, 16 * ST + 8
+        skip = lab("lr_noinit")
+        ins(f"setp.ne.u32 {q}, {tid}, 0")
+        ins(f"@{q} bra {skip}")
+        for s in range(ST):
+            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{8 * s}], {PRODUCERS}")
+            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{empty_off + 8 * s}], 1")
+        ins(f"mbarrier.init.shared::cta.b64 [{bars}+{done_off}], 1")
+        ins("fence.mbarrier_init.release.cluster")
+        ins("fence.proxy.async.shared::cta")
+        place(skip)
+        noalloc = lab("lr_noalloc")
+        ins(f"setp.ne.u32 {q}, {warp}, 4")
+        ins(f"@{q} bra {noalloc}")
+        slot = t("b32")
+        ins(f"add.u32 {slot}, {bars}, {slot_off}")
+        ins(f"tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [{slot}], {pl.tmem_cols}")
+        ins("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned")
+        place(noalloc)
+        ins("tcgen05.fence::before_thread_sync")
+        ins("bar.sync 0")
+        # the next kernel's CTAs may share the SM from here on, not before: one that took the tensor memory
+        # this CTA still had to allocate would keep it until this grid ends
+        self.pdl_trigger()
+        if S > 1:                     # met again before the first store into another CTA's shared memory
+            ins("barrier.cluster.arrive.release")
+        ins("tcgen05.fence::after_thread_sync")
+        self.pdl_wait()
+        tmem = t("b32")
+        ins(f"ld.shared.u32 {tmem}, [{bars}+{slot_off}]")
+        errp = t("b64")
+        ins(f"mov.u64 {errp}, thc_error")
+        end, fail = lab("lr_end"), lab("lr_fail")
+        kit = Kit(em, errp, fail)
+
+        # unit: the cluster's rank r holds K blocks [r kb / S, (r + 1) kb / S) of w tile tn, x tile tm
+        cta, rank, unit = self.special("%ctaid.x"), t("b32"), t("b32")
+        ins(f"and.b32 {rank}, {cta}, {S - 1}")
+        ins(f"shr.u32 {unit}, {cta}, {S.bit_length() - 1}")
+        tn, tm, n0, m0 = t("b32"), t("b32"), t("b32"), t("b32")
+        ins(f"rem.u32 {tm}, {unit}, {pl.tiles_m}")
+        ins(f"div.u32 {tn}, {unit}, {pl.tiles_m}")
+        ins(f"mul.lo.u32 {n0}, {tn}, {BM}")
+        ins(f"mul.lo.u32 {m0}, {tm}, {BT}")
+        kb, nk = t("b32"), t("b32")
+        ins(f"mul.lo.u32 {kb}, {rank}, {pl.kblocks}")
+        ins(f"div.u32 {kb}, {kb}, {S}")
+        ins(f"mad.lo.u32 {nk}, {rank}, {pl.kblocks}, {pl.kblocks}")
+        ins(f"div.u32 {nk}, {nk}, {S}")
+        ins(f"sub.u32 {nk}, {nk}, {kb}")                       # at least one: S <= kblocks
+        role_mma = lab("lr_mma")
+        ins(f"setp.eq.u32 {q}, {warp}, 4")
+        ins(f"@{q} bra {role_mma}")
+
+        # ---------------- producers (warps 0..3), then the epilogue ----------------
+        # thread -> 16-byte piece c of rows r0, r0 + 16, ..: a warp copies four whole 128-byte rows at a time
+        r0, c, soff, k8 = t("b32"), t("b32"), t("b32"), t("b32")
+        ins(f"shr.u32 {r0}, {tid}, 3")
+        ins(f"and.b32 {c}, {tid}, 7")
+        ins(f"xor.b32 {soff}, {r0}, {c}")
+        ins(f"and.b32 {soff}, {soff}, 7")
+        ins(f"shl.b32 {soff}, {soff}, 4")
+        ins(f"mad.lo.u32 {soff}, {r0}, 128, {soff}")
+        ins(f"add.u32 {soff}, {soff}, {base}")
+        ins(f"shl.b32 {k8}, {c}, 3")
+        ins(f"mad.lo.u32 {k8}, {kb}, {BK}, {k8}")              # this piece's first k
+        wp, xp = t("b64"), t("b64")
+
+        def row_pointer(dst: str, first: str, buf: str) -> None:
+            row, off = t("b32"), t("b64")
+            ins(f"add.u32 {row}, {first}, {r0}")
+            ins(f"mul.wide.u32 {off}, {row}, {p.K * 2}")
+            ins(f"add.u64 {dst}, {em.buffer_reg(buf)}, {off}")
+            ins(f"mul.wide.u32 {off}, {k8}, 2")
+            ins(f"add.u64 {dst}, {dst}, {off}")
+
+        row_pointer(wp, n0, p.w.name)
+        row_pointer(xp, m0, p.x.name)
+
+        def sizes(count: int, first: str, n: int, tile: int) -> list:
+            """Bytes to read of each of ``count`` rows (None: always 16): 0 past the axis' end."""
+            if n % tile == 0:
+                return [None] * count
+            out = []
+            for i in range(count):
+                row, z = t("b32"), t("b32")
+                ins(f"add.u32 {row}, {first}, {r0}")
+                ins(f"add.u32 {row}, {row}, {16 * i}")
+                ins(f"setp.lt.u32 {q}, {row}, {n}")
+                ins(f"selp.u32 {z}, 16, 0, {q}")
+                out.append(z)
+            return out
+
+        wsize, xsize = sizes(BM // 16, n0, p.N, BM), sizes(BT // 16, m0, p.M, BT)
+        kit_it, st, stage_addr = t("b32"), t("b32"), t("b32")
+        full_lag, lag_bar = t("b32"), t("b32")
+        ins(f"mov.u32 {kit_it}, 0")
+        ins(f"mov.u32 {st}, 0")
+        ins(f"mov.u32 {stage_addr}, {soff}")
+        ins(f"mov.u32 {lag_bar}, 0")
+        ph = t("b32")
+        ins(f"mov.u32 {ph}, 1")                                # parity of the empty barrier's previous phase
+        ptop, pdrain = lab("lr_load"), lab("lr_drain")
+        place(ptop)
+        eb = t("b32")
+        ins(f"mad.lo.u32 {eb}, {st}, 8, {bars}")
+        kit.wait(f"{eb}+{empty_off}", ph, 0)
+        ksize = None
+        if p.K % BK:
+            ksize = t("b32")
+            ins(f"setp.lt.u32 {q}, {k8}, {p.K}")
+            ins(f"selp.u32 {ksize}, 16, 0, {q}")
+
+        def copy(off: int, src: str, goff: int, size, hint: str = "") -> None:
+            if size is not None and ksize is not None:
+                z = t("b32")
+                ins(f"and.b32 {z}, {size}, {ksize}")
+            else:
+                z = size if size is not None else ksize
+            ins(f"cp.async.cg.shared.global{hint} [{stage_addr}+{off}], [{src}+{goff}], 16{f', {z}' if z else ''}")
+
+        for g in range(G):
+            src = wp
+            if g:
+                src = t("b64")
+                ins(f"add.u64 {src}, {wp}, {p.N * p.K * 2}")
+            for i in range(BM // 16):
+                copy(g * ROW_SLAB + i * 2048, src, i * 16 * p.K * 2, wsize[i], ".L2::256B")
+        for i in range(BT // 16):
+            copy(G * ROW_SLAB + i * 2048, xp, i * 16 * p.K * 2, xsize[i])
+        ins("cp.async.commit_group")
+        ins(f"add.u64 {wp}, {wp}, {BK * 2}")
+        ins(f"add.u64 {xp}, {xp}, {BK * 2}")
+        ins(f"add.u32 {k8}, {k8}, {BK}")
+        ins(f"add.u32 {kit_it}, {kit_it}, 1")
+        # the stage loaded ST - 1 iterations ago is complete: hand it to the tensor cores
+        nolag = lab("lr_nolag")
+        ins(f"setp.lt.u32 {q}, {kit_it}, {ST}")
+        ins(f"@{q} bra {nolag}")
+
+        def hand_over(pending: int) -> None:
+            ins(f"cp.async.wait_group {pending}")
+            ins("fence.proxy.async.shared::cta")
+            ins(f"mad.lo.u32 {full_lag}, {lag_bar}, 8, {bars}")
+            ins(f"mbarrier.arrive.shared::cta.b64 _, [{full_lag}]")
+            ins(f"add.u32 {lag_bar}, {lag_bar}, 1")
+            ins(f"setp.eq.u32 {q}, {lag_bar}, {ST}")
+            ins(f"selp.u32 {lag_bar}, 0, {lag_bar}, {q}")
+
+        hand_over(ST - 1)
+        place(nolag)
+        ins(f"add.u32 {st}, {st}, 1")
+        ins(f"add.u32 {stage_addr}, {stage_addr}, {stage_bytes}")
+        ins(f"setp.eq.u32 {q}, {st}, {ST}")
+        ins(f"selp.u32 {st}, 0, {st}, {q}")
+        ins(f"selp.b32 {stage_addr}, {soff}, {stage_addr}, {q}")
+        flip = t("b32")
+        ins(f"selp.u32 {flip}, 1, 0, {q}")
+        ins(f"xor.b32 {ph}, {ph}, {flip}")
+        ins(f"setp.lt.u32 {q}, {kit_it}, {nk}")
+        ins(f"@{q} bra {ptop}")
+        # the stages still in flight, oldest first: min(nk, ST - 1) of them
+        place(pdrain)
+        for left in range(ST - 2, -1, -1):
+            none = lab("lr_none")
+            ins(f"setp.le.u32 {q}, {nk}, {left}")
+            ins(f"@{q} bra {none}")
+            hand_over(left)
+            place(none)
+        self._epilogue(kit, tid, warp, lane, tmem, bars, done_off, ex, rank, n0, m0, end)
+        ins(f"bra {end}")
+
+        # ---------------- MMA issuer (warp 4) ----------------
+        place(role_mma)
+        one = t("pred")
+        elect_one(em, one)
+        hi, it2, st2, par, first = t("b32"), t("b32"), t("b32"), t("b32"), t("pred")
+        ins(f"mov.u32 {hi}, {desc_hi(1024)}")
+        ins(f"mov.u32 {it2}, 0")
+        ins(f"mov.u32 {st2}, 0")
+        ins(f"mov.u32 {par}, 0")
+        always = t("pred")
+        ins(f"setp.eq.u32 {always}, {hi}, {hi}")
+        idesc = idesc_f16(BM, BT, bf16=p.x.ty is BF16)
+        mtop = lab("lr_mma_k")
+        place(mtop)
+        fb, sa = t("b32"), t("b32")
+        ins(f"mad.lo.u32 {fb}, {st2}, 8, {bars}")
+        kit.wait(fb, par, 1)
+        ins("tcgen05.fence::after_thread_sync")
+        ins(f"mad.lo.u32 {sa}, {st2}, {stage_bytes}, {base}")
+        sx = t("b32")
+        ins(f"add.u32 {sx}, {sa}, {G * ROW_SLAB}")
+        ad0, bd0 = kit.desc(sa, 16, hi), kit.desc(sx, 16, hi)
+        ins(f"setp.ne.u32 {first}, {it2}, 0")                  # the first block overwrites the accumulators
+        for k in range(BK // 16):
+            bd = kit.desc_add(bd0, k * 32)
+            for g in range(G):
+                ad = kit.desc_add(ad0, g * ROW_SLAB + k * 32)
+                d = tmem
+                if g:
+                    d = t("b32")
+                    ins(f"add.u32 {d}, {tmem}, {BT}")
+                ins(f"@{one} tcgen05.mma.cta_group::1.kind::f16 [{d}], {ad}, {bd}, {idesc}, "
+                    f"{always if k else first}")
+        commit = "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64"
+        ins(f"@{one} {commit} [{fb}+{empty_off}]")
+        ins(f"add.u32 {it2}, {it2}, 1")
+        ins(f"add.u32 {st2}, {st2}, 1")
+        ins(f"setp.eq.u32 {q}, {st2}, {ST}")
+        ins(f"selp.u32 {st2}, 0, {st2}, {q}")
+        ins(f"selp.u32 {flip}, 1, 0, {q}")
+        ins(f"xor.b32 {par}, {par}, {flip}")
+        ins(f"setp.lt.u32 {q}, {it2}, {nk}")
+        ins(f"@{q} bra {mtop}")
+        ins(f"@{one} {commit} [{bars}+{done_off}]")
+        # a thread that gave up a wait meets the same cluster barriers as the others
+        place(fail)
+        if S > 1:
+            ins("barrier.cluster.wait.acquire")
+            ins("barrier.cluster.arrive.release")
+            ins("barrier.cluster.wait.acquire")
+
+        # ---------------- common exit ----------------
+        place(end)
+        ins("cp.async.wait_all")
+        ins("tcgen05.fence::before_thread_sync")
+        ins("barrier.sync 0")
+        nod = lab("lr_nodealloc")
+        ins(f"setp.ne.u32 {q}, {warp}, 4")
+        ins(f"@{q} bra {nod}")
+        ins("tcgen05.fence::after_thread_sync")
+        ins(f"tcgen05.dealloc.cta_group::1.sync.aligned.b32 {tmem}, {pl.tmem_cols}")
+        place(nod)
+
+    def _read_sums(self, tmem: str, c0: int, n: int) -> list[list[str]]:
+        """Columns c0 .. c0 + n of this thread's accumulator row(s)."""
+        em, out = self.em, []
+        for g in range(self.plan.G):
+            v, a = em.tmps("b32", n), em.tmp("b32")
+            em.ins(f"add.u32 {a}, {tmem}, {g * self.plan.BT + c0}")
+            em.ins(f"tcgen05.ld.sync.aligned.32x32b.x{n}.b32 {{{', '.join(v)}}}, [{a}]")
+            out.append(v)
+        em.ins("tcgen05.wait::ld.sync.aligned")
+        return out
+
+    def _epilogue(self, kit, tid, warp, lane, tmem, bars, done_off, ex, rank, n0, m0, end) -> None:
+        """The sums of row n (of w) by token, to C[m0 + token, n].
+
+        S = 1: a thread holds row ``tid``, its tokens in tensor-memory columns; a warp's loads and stores
+        of one token are 32 consecutive columns of C.  S > 1: each rank owns 128 / S rows; every CTA
+        stores its sums of those rows into the owner's exchange area [rank][accumulator][token][row], the
+        cluster meets, and the owner's threads (row, token mod S) add the ranks' sums in order."""
+        em, t, ins, place, lab = self.em, self.em.tmp, self.em.ins, self.em.place, self.em.label
+        p, pl = self.p, self.plan
+        S, BT, G = pl.S, pl.BT, pl.G
+        q = t("pred")
+        lane_off = t("b32")
+        ins(f"shl.b32 {lane_off}, {warp}, 21")                 # (32 * warp) << 16
+        acc = t("b32")
+        ins(f"add.u32 {acc}, {tmem}, {lane_off}")
+        left = t("b32")                                        # tokens of this tile
+        ins(f"sub.s32 {left}, {p.M}, {m0}")
+        ins(f"min.s32 {left}, {left}, {BT}")
+        zero = t("b32")
+        ins(f"mov.u32 {zero}, 0")
+        if S == 1:
+            n = t("b32")
+            ins(f"add.u32 {n}, {n0}, {tid}")
+            inside = None
+            if p.N % BM:
+                inside = t("pred")
+                ins(f"setp.lt.u32 {inside}, {n}, {p.N}")
+            self._columns(n, inside)
+            kit.wait(f"{bars}+{done_off}", zero, 2)
+            ins("tcgen05.fence::after_thread_sync")
+            for c0 in range(0, BT, 16):
+                if c0:
+                    ins(f"setp.le.s32 {q}, {left}, {c0}")
+                    ins(f"@{q} bra {end}")
+                ok, rows = [], []
+                for j in range(16):
+                    o, m = t("pred"), t("b32")
+                    ins(f"setp.gt.s32 {o}, {left}, {c0 + j}" if inside is None else
+                        f"setp.gt.and.s32 {o}, {left}, {c0 + j}, {inside}")
+                    ins(f"add.u32 {m}, {m0}, {c0 + j}")
+                    ok.append(o)
+                    rows.append(m)
+                fetched = [self._fetch(m, n, o) for m, o in zip(rows, ok)]
+                sums = self._read_sums(acc, c0, 16)
+                for j in range(16):
+                    self._finish([v[j] for v in sums], rows[j], n, ok[j], fetched[j])
+            return
+        RS = BM // S                                           # rows of w a rank owns
+        owner, mine, dst, dsm = t("b32"), t("b32"), t("b32"), t("b32")
+        ins(f"shr.u32 {owner}, {tid}, {RS.bit_length() - 1}")
+        ins(f"and.b32 {mine}, {tid}, {RS - 1}")
+        ins(f"mad.lo.u32 {dst}, {rank}, {G * BT * RS * 4}, {ex}")
+        ins(f"mad.lo.u32 {dst}, {mine}, 4, {dst}")
+        ins(f"mapa.shared::cluster.u32 {dsm}, {dst}, {owner}")
+        # this thread's part of the join: row ``mine`` of this rank's, tokens tid / RS + S j
+        n, tok0 = t("b32"), owner
+        ins(f"mad.lo.u32 {n}, {rank}, {RS}, {mine}")
+        ins(f"add.u32 {n}, {n}, {n0}")
+        inside = None
+        if p.N % BM:
+            inside = t("pred")
+            ins(f"setp.lt.u32 {inside}, {n}, {p.N}")
+        self._columns(n, inside)
+        kit.wait(f"{bars}+{done_off}", zero, 2)
+        ins("tcgen05.fence::after_thread_sync")
+        ins("barrier.cluster.wait.acquire")
+        sent = lab("lr_sent")
+        for c0 in range(0, BT, 16):
+            if c0:
+                ins(f"setp.le.s32 {q}, {left}, {c0}")
+                ins(f"@{q} bra {sent}")
+            sums = self._read_sums(acc, c0, 16)
+            for j in range(16):
+                o = t("pred")
+                ins(f"setp.gt.s32 {o}, {left}, {c0 + j}")
+                for g in range(G):
+                    ins(f"@{o} st.shared::cluster.b32 [{dsm}+{(g * BT + c0 + j) * RS * 4}], {sums[g][j]}")
+        place(sent)
+        ins("barrier.cluster.arrive.release")
+        ins("barrier.cluster.wait.acquire")
+        src = t("b32")
+        ins(f"mad.lo.u32 {src}, {mine}, 4, {ex}")
+        ins(f"mad.lo.u32 {src}, {tok0}, {RS * 4}, {src}")
+        chunk = 4
+        per = -(-BT // S)                                      # tokens a thread may have
+        for j0 in range(0, per, chunk):
+            if j0:
+                x = t("b32")
+                ins(f"add.u32 {x}, {tok0}, {j0 * S}")
+                ins(f"setp.le.s32 {q}, {left}, {x}")
+                ins(f"@{q} bra {end}")
+            todo = []
+            for j in range(j0, min(per, j0 + chunk)):
+                x, m, o = t("b32"), t("b32"), t("pred")
+                ins(f"add.u32 {x}, {tok0}, {j * S}")
+                ins(f"setp.gt.s32 {o}, {left}, {x}" if inside is None else
+                    f"setp.gt.and.s32 {o}, {left}, {x}, {inside}")
+                ins(f"add.u32 {m}, {m0}, {x}")
+                todo.append((j, m, o, self._fetch(m, n, o)))
+            for j, m, o, fetched in todo:
+                vals = []
+                for g in range(G):
+                    total = None
+                    for r in range(S):
+                        v = t("f32")
+                        ins(f"mov.f32 {v}, {F32.imm(0.0)}")
+                        ins(f"@{o} ld.shared.f32 {v}, [{src}+{((r * G + g) * BT + j * S) * RS * 4}]")
+                        if total is None:
+                            total = v
+                        else:
+                            ins(f"add.rn.f32 {total}, {total}, {v}")
+                    b = t("b32")
+                    ins(f"mov.b32 {b}, {total}")
+                    vals.append(b)
+                self._finish(vals, m, n, o, fetched)
+
+    def _load(self, name: str, index: str, pred: str | None) -> list[str]:
+        """One element of a source at a 64-bit element index, zero where ``pred`` is false."""
+        em, ty = self.em, self.p.kernel.param(name).ty
+        a, r = em.tmp("b64"), em.tmp("b32")
+        em.ins(f"mad.lo.s64 {a}, {index}, {ty.nbytes}, {em.buffer_reg(name)}")
+        at = f"@{pred} " if pred else ""
+        em.ins(f"mov.u32 {r}, 0")
+        if ty.nbytes == 4:
+            em.ins(f"{at}ld.global.nc.b32 {r}, [{a}]")
+        else:
+            h = em.tmp("b16")
+            em.ins(f"{at}ld.global.nc.b16 {h}, [{a}]")
+            em.ins(f"{at}cvt.u32.u16 {r}, {h}")
+        return [r]
+
+    def _columns(self, n: str, inside: str | None) -> None:
+        """The sources over columns, at this thread's column."""
+        em = self.em
+        self.cols = {}
+        for src in self.replay.sources if self.replay else ():
+            if src[1]:
+                i = em.tmp("b64")
+                em.ins(f"cvt.u64.u32 {i}, {n}")
+                if src[2]:
+                    em.ins(f"add.u64 {i}, {i}, {src[2]}")
+                self.cols[src] = self._load(src[0], i, inside)
+
+    def _fetch(self, m: str, n: str, ok: str) -> dict:
+        """The element sources at (m, n), and the columns' ones."""
+        em, out = self.em, dict(self.cols)
+        for src in self.replay.sources if self.replay else ():
+            if not src[1]:
+                i, c = em.tmp("b64"), em.tmp("b64")
+                em.ins(f"mul.wide.u32 {i}, {m}, {self.p.N}")
+                em.ins(f"cvt.u64.u32 {c}, {n}")
+                em.ins(f"add.u64 {i}, {i}, {c}")
+                out[src] = self._load(src[0], i, ok)
+        return out
+
+    def _finish(self, sums: list[str], m: str, n: str, ok: str, fetched: dict) -> None:
+        """Epilogue of one element and its store."""
+        em, t, ins, c = self.em, self.em.tmp, self.em.ins, self.p.c
+        vals = []
+        for b in sums:
+            f = t("f32")
+            ins(f"mov.b32 {f}, {b}")
+            vals.append(f)
+        y = vals[0]
+        if self.replay:
+            y = self.replay.element(vals[0], vals[1] if len(vals) > 1 else None, m, n, lambda src: (fetched[src], 0))
+        i, k = t("b64"), t("b64")
+        ins(f"mul.wide.u32 {i}, {m}, {self.p.N}")
+        ins(f"cvt.u64.u32 {k}, {n}")
+        ins(f"add.u64 {i}, {i}, {k}")
+        ins(f"mad.lo.s64 {i}, {i}, {c.ty.nbytes}, {em.buffer_reg(c.name)}")
+        if c.ty is F32:
+            ins(f"@{ok} st.global.f32 [{i}], {y}")
+        else:
+            h = t("b16")
+            ins(f"cvt.rn.{c.ty.ptx}.f32 {h}, {y}")
+            ins(f"@{ok} st.global.b16 [{i}], {h}")
+
+
+class RowsPlan:
+    """Tiles and launch of ``LinearRows``: ``BT`` tokens a tile, K in ``S`` parts."""
+
+    def __init__(self, p: Product, BT: int, S: int):
+        self.BT, self.S = BT, S
+        self.G = 2 if p.gated else 1
+        self.kblocks = -(-p.K // BK)
+        self.tiles_m, self.tiles_n = -(-p.M // BT), -(-p.N // BM)
+        self.ctas = self.tiles_m * self.tiles_n * S
+        self.stage_bytes = self.G * ROW_SLAB + BT * BK * 2
+        self.exchange = self.G * BT * BM * 4 if S > 1 else 0
+        self.tmem_cols = max(32, 1 << (self.G * BT - 1).bit_length())
+        # two CTAs an SM where the launch has more than one for each
+        half = self.ctas > SM_COUNT
+        room = (SMEM_LIMIT // 2 - 1024 if half else SMEM_LIMIT) - self.exchange - 1024 - 256 - p.static_smem
+        self.stages = min(12, -(-self.kblocks // S) + 1, room // self.stage_bytes)
+        self.smem = self.stages * self.stage_bytes + self.exchange + 1024 + 256
+        # CTAs of a cluster wait for one another while they hold tensor memory, so no two CTAs that share
+        # an SM may run out of it: each takes at least its columns' share of shared memory, and more than
+        # the CTA-pair kernels (all 512 columns, over 190 KB) leave
+        self.smem = max(self.smem, min(SMEM_LIMIT, self.tmem_cols * 456), 36 * 1024)
+
+    @property
+    def possible(self) -> bool:
+        return (self.stages >= 2 and self.S <= self.kblocks and self.exchange <= EXCHANGE_LIMIT
+                and self.G * self.BT <= 512 and self.ctas <= (SM_COUNT if self.smem > SMEM_LIMIT // 2 - 1024
+                                                              else 2 * SM_COUNT))
+
+    @classmethod
+    def best(cls, p: Product) -> "RowsPlan | None":
+        """The plan that the estimate takes for fastest, or None."""
+        out = []
+        for tiles_m in range(1, -(-p.M // 16) + 1):
+            BT = -(-(-(-p.M // tiles_m)) // 16) * 16
+            if BT > 256:
+                continue
+            if tiles_m > 8:
+                break
+            for S in (1, 2, 4, 8):
+                pl = cls(p, BT, S)
+                if pl.possible:
+                    out.append((pl.estimate(p), S, tiles_m, pl))
+        return min(out, key=lambda x: x[:3])[3] if out else None
+
+    def estimate(self, p: Product) -> float:
+        """Microseconds: w from memory once, against each SM's share of slabs through its copies and
+        tensor cores."""
+        memory = self.G * p.N * p.K * 2 / 5.5e6
+        per_sm = -(-self.ctas // SM_COUNT)
+        block = max(self.stage_bytes / 40, 2 * self.BT * self.G, 150) / 1900
+        return max(memory, per_sm * -(-self.kblocks // self.S) * block) + 3 + (1 if self.S > 1 else 0) + self.BT / 64
+
+
 def recognise(kernel: KernelInfo):
     p = Product.read(kernel)
     if p is None:
         return None
-    if p.M > 128:
-        return LinearPair(p)
-    return None
+    rows = RowsPlan.best(p)
+    pair = LinearPair(p)
+    if rows is None or TUNING.linear_kernel == "pair":
+        return pair
+    if TUNING.linear_kernel == "rows" or rows.estimate(p) < pair.estimate():
+        return LinearRows(p, rows)
+    return pair

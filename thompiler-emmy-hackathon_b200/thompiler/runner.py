@@ -303,10 +303,12 @@ class Launch:
     """One kernel's launches on device pointers, with everything that stays the same from call to call
     converted once: ``launch(ptrs, stream)`` is one C call (with its tensor maps' binding, when the
     plan has any).  ``plan``'s grid, block and shared memory are read again whenever they are
-    replaced."""
+    replaced; a buffer that meta.json wants aligned is refused when it is not."""
 
-    def __init__(self, function: Function, plan: LaunchPlan, arg_order: list[str], tmaps: TensorMaps | None):
-        self.function, self.plan, self.order, self.tmaps = function, plan, tuple(arg_order), tmaps
+    def __init__(self, function: Function, plan: LaunchPlan, kmeta: dict, tmaps: TensorMaps | None):
+        self.function, self.plan, self.order, self.tmaps = function, plan, tuple(kmeta["arg_order"]), tmaps
+        align = {a["name"]: a.get("align", 1) for a in kmeta["args"]}
+        self.aligned = [(i, align[n]) for i, n in enumerate(self.order) if align.get(n, 1) > 1]
         self.n = len(self.order)
         self._array = ctypes.c_uint64 * max(1, self.n)
         lib = library()
@@ -320,7 +322,12 @@ class Launch:
             self._dims = (_dims(plan.grid), _dims(plan.block), int(plan.smem), OVERLAP_PREVIOUS if plan.pdl else 0)
             self._geometry = geometry
         grid, block, smem, flags = self._dims
-        args = self._array(*[ptrs[n] for n in self.order])
+        vals = [ptrs[n] for n in self.order]
+        for i, align in self.aligned:
+            if vals[i] % align:
+                raise RunnerError("request", f"{f.name}: buffer {self.order[i]!r} at {vals[i]:#x} is not "
+                                             f"{align}-byte aligned")
+        args = self._array(*vals)
         if self.tmaps is None:
             st = self._plain(f.handle, grid, block, smem, args, self.n, stream, flags)
         else:

@@ -273,9 +273,9 @@ def matmul_package(outdir, M: int, N: int, K: int, b_layout: str = "col", out_dt
 
 
 def _layer_write(outdir, pid: str, code: str, entry: str, body, inputs: dict, outputs: dict, grid: int, T: int,
-                 rtol: float, atol: float, smem: int = 0) -> Path:
+                 rtol: float, atol: float, smem: int = 0, aligned: tuple = ()) -> Path:
     """A package of one kernel whose args are ``inputs`` then ``outputs`` (name -> (shape, dtype, init or
-    None)), seeded in order."""
+    None)), seeded in order; the buffers in ``aligned`` start on 16-byte boundaries."""
     names = list(outputs)
     g = _graph({n: (shape, dt) for n, (shape, dt, _) in inputs.items()}, {}, names[0], outputs[names[0]][0], entry,
                body, dtype=outputs[names[0]][1])
@@ -288,6 +288,9 @@ def _layer_write(outdir, pid: str, code: str, entry: str, body, inputs: dict, ou
         if init:
             args[-1]["init"] = dict(init, seed=i)
     args += [{"name": n, "dtype": dt, "shape": list(shape), "output": True} for n, (shape, dt, _) in outputs.items()]
+    for a in args:
+        if a["name"] in aligned:
+            a["align"] = 16
     kmeta = {"node": names[0], "arg_order": [a["name"] for a in args], "grid": [grid, 1, 1], "block": [T, 1, 1],
              "smem_bytes": smem, "zero_outputs": [], "args": args}
     return _write(outdir, pid, code, entry, g, kmeta, rtol, atol)
@@ -308,7 +311,7 @@ def linear_package(outdir, M: int, N: int, K: int, dtype: str = "f16", out_dtype
     activation is None, "relu", "silu" or "gelu_tanh".  gated: w[2N, K] and bias[2N] hold two
     projections, and the result is act(first) * second (+ res).  M is any number of rows from one
     on; N and K are multiples of 8 (16-byte rows).  The entry is ``k_linear`` over x, w, (bias,)
-    (res,) linear, buffers that do not overlap."""
+    (res,) linear, buffers that do not overlap; x, w and linear start on 16-byte boundaries."""
     _positive(M=M, N=N, K=K)
     out_dtype = out_dtype or dtype
     if dtype not in ("f16", "bf16") or out_dtype not in (dtype, "f32"):
@@ -335,7 +338,7 @@ def linear_package(outdir, M: int, N: int, K: int, dtype: str = "f16", out_dtype
     tiles = -(-M // 64) * -(-N // 64)
     return _layer_write(outdir, f"synth_linear_{M}x{N}x{K}", code, "k_linear", body, inputs,
                         {"linear": ((M, N), out_dtype, None)}, -(-tiles // 8) * 8, 128, 2e-2, 2e-3,
-                        smem=(3 if gated else 2) * 64 * 64 * 2)
+                        smem=(3 if gated else 2) * 64 * 64 * 2, aligned=("x", "w", "linear"))
 
 
 def _heads_package(outdir, entry: str, Bn: int, S: int, heads: int, kv_heads: int, D: int, rotary: int | None,
