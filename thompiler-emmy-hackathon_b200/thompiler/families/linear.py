@@ -259,54 +259,94 @@ class LinearPair(TcMatmulPair):
             if first:
                 ins(f"add.u64 {a}, {a}, {first * nb}")
             self.at[src] = a
-        cw = 64 // self.c.ty.nbytes
-        self.first = self._fetch(0, cw)
-        self.ahead = {}
+        self.ahead = self._fetch(0, 64 // self.c.ty.nbytes)
 
-    def _fetch(self, c0: int, cw: int) -> dict:
-        """Issue the loads of every source's elements c0 .. c0 + cw: {source: packed registers}."""
+    def _fetch(self, c0: int, cw: int, into: dict | None = None, when: str | None = None) -> dict:
+        """Issue the loads of every source's elements c0 .. c0 + cw from the current box on, where ``when``
+        holds: {source: packed registers} (``into``'s registers again, when given)."""
         em, t, ins = self.em, self.em.tmp, self.em.ins
         out = {}
         for src in self.replay.sources:
             name, cols_only, _ = src
             nb = self.p.kernel.param(name).ty.nbytes
             regs = []
-            for c in range(c0, c0 + cw, 16 // nb):
-                pred = None if cols_only else self.row_ok
+            for k, c in enumerate(range(c0, c0 + cw, 16 // nb)):
+                preds = [x for x in (when, None if cols_only else self.row_ok) if x]
                 if self.left is not None:
                     q = t("pred")
-                    ins(f"setp.gt.s32 {q}, {self.left}, {c}" if pred is None else
-                        f"setp.gt.and.s32 {q}, {self.left}, {c}, {pred}")
-                    pred = q
-                four = em.tmps("b32", 4)
-                if pred is not None:
-                    for r in four:
-                        ins(f"mov.u32 {r}, 0")
+                    ins(f"setp.gt.s32 {q}, {self.left}, {c}")
+                    preds.append(q)
+                pred = preds[0] if preds else None
+                for x in preds[1:]:
+                    both = t("pred")
+                    ins(f"and.pred {both}, {pred}, {x}")
+                    pred = both
+                four = into[src][4 * k:4 * k + 4] if into else em.tmps("b32", 4)
+                if pred is not None and not into:
+                    for x in four:
+                        ins(f"mov.u32 {x}, 0")
                 ins(f"{f'@{pred} ' if pred else ''}ld.global.nc.v4.b32 {{{', '.join(four)}}}, [{self.at[src]}+{c * nb}]")
                 regs += four
             out[src] = regs
         return out
 
-    def box(self, c0: int, cw: int, width: int, taddr: str) -> list[str]:
-        em, t, ins = self.em, self.em.tmp, self.em.ins
-        if c0 == 0:
-            self.ahead = {0: self.first}
-        mine = self.ahead.pop(c0)
-        sums = []
+    def store_tile(self, cw: int, width: int, taddr: str, col0: str, free, stage) -> None:
+        """The tile's boxes, two a turn of a loop: the code of a whole tile unrolled is tens of kilobytes that
+        a launch of few tiles would spend its time fetching.  Each box's sources were loaded while
+        the previous box was worked on."""
+        em, t, ins, place, lab = self.em, self.em.tmp, self.em.ins, self.em.place, self.em.label
+        turns = width // (2 * cw)
+        i, ta, cc, more, last = t("b32"), t("b32"), t("b32"), t("pred"), t("pred")
+        ins(f"mov.u32 {i}, 0")
+        ins(f"mov.u32 {ta}, {taddr}")
+        ins(f"mov.u32 {cc}, {col0}")
+        top = lab("lp_box")
+        place(top)
+        ins(f"setp.ne.u32 {more}, {i}, {turns - 1}")
+        ins(f"setp.eq.u32 {last}, {i}, {turns - 1}")
+        now = self.ahead
+        for b in (0, 1):
+            def values(b=b):
+                nonlocal now
+                sums = self._sums(ta, b * cw, cw)
+                if b == 0:
+                    following = self._fetch(cw, cw)
+                else:
+                    following = self._fetch(2 * cw, cw, into=self.ahead, when=more)
+                ins("tcgen05.wait::ld.sync.aligned")
+                if b:
+                    free(last)
+                v = self._apply(sums, now, b * cw, cw)
+                now = following
+                return v
+            stage(b, values, cc, b * cw)
+        ins(f"add.u32 {ta}, {ta}, {2 * cw}")
+        ins(f"add.u32 {cc}, {cc}, {2 * cw}")
+        ins(f"add.u32 {self.col}, {self.col}, {2 * cw}")
+        if self.left is not None:
+            ins(f"sub.s32 {self.left}, {self.left}, {2 * cw}")
+        for src, a in self.at.items():
+            ins(f"add.u64 {a}, {a}, {2 * cw * self.p.kernel.param(src[0]).ty.nbytes}")
+        ins(f"add.u32 {i}, {i}, 1")
+        ins(f"@{more} bra {top}")
+
+    def _sums(self, taddr: str, c0: int, cw: int) -> list[list[str]]:
+        em, out = self.em, []
         for base in (c0, c0 + self.HN) if self.p.gated else (c0,):
-            v = em.tmps("b32", cw)
-            a = t("b32")
-            ins(f"add.u32 {a}, {taddr}, {base}")
-            ins(f"tcgen05.ld.sync.aligned.32x32b.x{cw}.b32 {{{', '.join(v)}}}, [{a}]")
-            sums.append(v)
-        if c0 + cw < width:
-            self.ahead[c0 + cw] = self._fetch(c0 + cw, cw)
-        ins("tcgen05.wait::ld.sync.aligned")
+            v, a = em.tmps("b32", cw), em.tmp("b32")
+            em.ins(f"add.u32 {a}, {taddr}, {base}")
+            em.ins(f"tcgen05.ld.sync.aligned.32x32b.x{cw}.b32 {{{', '.join(v)}}}, [{a}]")
+            out.append(v)
+        return out
+
+    def _apply(self, sums: list[list[str]], mine: dict, c0: int, cw: int) -> list[str]:
+        """The epilogue of a box's elements, packed for the store."""
+        em, t, ins = self.em, self.em.tmp, self.em.ins
         out = []
         for j in range(cw):
             z = [t("f32") for _ in sums]
-            for r, v in zip(z, sums):
-                ins(f"mov.b32 {r}, {v[j]}")
+            for x, v in zip(z, sums):
+                ins(f"mov.b32 {x}, {v[j]}")
             col = t("b32")
             ins(f"add.u32 {col}, {self.col}, {c0 + j}")
             out.append(self.replay.element(z[0], z[1] if len(z) > 1 else None, self.row, col,
@@ -314,9 +354,9 @@ class LinearPair(TcMatmulPair):
         packed = []
         step = 4 // self.c.ty.nbytes
         for j in range(0, cw, step):
-            r = t("b32")
-            ins(f"mov.b32 {r}, {out[j]}" if step == 1 else f"cvt.rn.{self.c.ty.ptx}x2.f32 {r}, {out[j + 1]}, {out[j]}")
-            packed.append(r)
+            x = t("b32")
+            ins(f"mov.b32 {x}, {out[j]}" if step == 1 else f"cvt.rn.{self.c.ty.ptx}x2.f32 {x}, {out[j + 1]}, {out[j]}")
+            packed.append(x)
         return packed
 
 
@@ -324,7 +364,9 @@ class LinearPair(TcMatmulPair):
 
 ROW_SLAB = BM * BK * 2                       # one 128 x 64 slab of w
 EXCHANGE_LIMIT = 64 * 1024                   # shared memory for the partial sums of a cut K
-PRODUCERS = 128
+PRODUCERS = 256
+MMA_WARP = PRODUCERS // 32
+ROW_STEP = PRODUCERS // 8                    # rows that the producers copy a piece of at a time
 
 
 class LinearRows(TunedKernel):
@@ -336,10 +378,11 @@ class LinearRows(TunedKernel):
     partial sums to the CTA that owns those rows of w through distributed shared memory, which adds
     them in rank order (no atomics: the same bits every time), applies the epilogue and stores.
 
-    Four warps copy both operands with 16-byte cp.async into the 128-byte swizzle -- no tensor maps, so
+    Eight warps copy both operands with 16-byte cp.async into the 128-byte swizzle -- no tensor maps, so
     nothing is kept for a buffer's address, and any number of weights share the kernel in captured
-    graphs -- and finish a stage with a proxy fence and an arrival on its mbarrier; a fifth warp issues
-    the MMAs.  Out-of-range rows and K are zero-filled by the copies.  Every wait is bounded."""
+    graphs -- each thread's copies of a stage arriving on its mbarrier as they land; a ninth warp
+    allocates the tensor memory (after the first loads are on their way), waits, fences the proxies
+    and issues the MMAs.  Out-of-range rows and K are zero-filled by the copies.  Every wait is bounded."""
 
     family = "tcgen05-linear-rows"
 
@@ -378,40 +421,25 @@ class LinearRows(TunedKernel):
         ins(f"mov.u32 {base}, smem_pool")
         ins(f"add.u32 {base}, {base}, 1023")
         ins(f"and.b32 {base}, {base}, -1024")
-        # shared: stages (w slabs | x rows) | exchange | barriers (full, empty per stage; sums done) | TMEM slot
+        # shared: stages (w slabs | x rows) | exchange | barriers (full, empty per stage; sums done; tensor
+        # memory allocated) | its address
         ex, bars = t("b32"), t("b32")
         ins(f"add.u32 {ex}, {base}, {ST * stage_bytes}")
         ins(f"add.u32 {bars}, {ex}, {pl.exchange}")
-        empty_off, done_off, slot_off = 8 * ST, 16 * ST, 16 * ST + 8
-        skip = lab("lr_noinit")
-        ins(f"setp.ne.u32 {q}, {tid}, 0")
+        empty_off, done_off, alloc_off, slot_off = 8 * ST, 16 * ST, 16 * ST + 8, 16 * ST + 16
+        # one thread a barrier: the first ST (full) expect every producer, the others one arrival
+        skip, where, count = lab("lr_noinit"), t("b32"), t("b32")
+        ins(f"setp.ge.u32 {q}, {tid}, {2 * ST + 2}")
         ins(f"@{q} bra {skip}")
-        for s in range(ST):
-            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{8 * s}], {PRODUCERS}")
-            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{empty_off + 8 * s}], 1")
-        ins(f"mbarrier.init.shared::cta.b64 [{bars}+{done_off}], 1")
+        ins(f"mad.lo.u32 {where}, {tid}, 8, {bars}")
+        ins(f"setp.lt.u32 {q}, {tid}, {ST}")
+        ins(f"selp.u32 {count}, {PRODUCERS}, 1, {q}")
+        ins(f"mbarrier.init.shared::cta.b64 [{where}], {count}")
         ins("fence.mbarrier_init.release.cluster")
-        ins("fence.proxy.async.shared::cta")
         place(skip)
-        noalloc = lab("lr_noalloc")
-        ins(f"setp.ne.u32 {q}, {warp}, 4")
-        ins(f"@{q} bra {noalloc}")
-        slot = t("b32")
-        ins(f"add.u32 {slot}, {bars}, {slot_off}")
-        ins(f"tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [{slot}], {pl.tmem_cols}")
-        ins("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned")
-        place(noalloc)
-        ins("tcgen05.fence::before_thread_sync")
         ins("bar.sync 0")
-        # the next kernel's CTAs may share the SM from here on, not before: one that took the tensor memory
-        # this CTA still had to allocate would keep it until this grid ends
-        self.pdl_trigger()
         if S > 1:                     # met again before the first store into another CTA's shared memory
             ins("barrier.cluster.arrive.release")
-        ins("tcgen05.fence::after_thread_sync")
-        self.pdl_wait()
-        tmem = t("b32")
-        ins(f"ld.shared.u32 {tmem}, [{bars}+{slot_off}]")
         errp = t("b64")
         ins(f"mov.u64 {errp}, thc_error")
         end, fail = lab("lr_end"), lab("lr_fail")
@@ -433,11 +461,12 @@ class LinearRows(TunedKernel):
         ins(f"div.u32 {nk}, {nk}, {S}")
         ins(f"sub.u32 {nk}, {nk}, {kb}")                       # at least one: S <= kblocks
         role_mma = lab("lr_mma")
-        ins(f"setp.eq.u32 {q}, {warp}, 4")
+        ins(f"setp.eq.u32 {q}, {warp}, {MMA_WARP}")
         ins(f"@{q} bra {role_mma}")
 
-        # ---------------- producers (warps 0..3), then the epilogue ----------------
-        # thread -> 16-byte piece c of rows r0, r0 + 16, ..: a warp copies four whole 128-byte rows at a time
+        # ---------------- producers (warps 0..7), then the epilogue ----------------
+        # thread -> 16-byte piece c of rows r0, r0 + 32, ..: a warp copies four whole 128-byte rows at a time
+        self.pdl_wait()
         r0, c, soff, k8 = t("b32"), t("b32"), t("b32"), t("b32")
         ins(f"shr.u32 {r0}, {tid}, 3")
         ins(f"and.b32 {c}, {tid}, 7")
@@ -469,22 +498,23 @@ class LinearRows(TunedKernel):
             for i in range(count):
                 row, z = t("b32"), t("b32")
                 ins(f"add.u32 {row}, {first}, {r0}")
-                ins(f"add.u32 {row}, {row}, {16 * i}")
+                ins(f"add.u32 {row}, {row}, {ROW_STEP * i}")
                 ins(f"setp.lt.u32 {q}, {row}, {n}")
                 ins(f"selp.u32 {z}, 16, 0, {q}")
                 out.append(z)
             return out
 
-        wsize, xsize = sizes(BM // 16, n0, p.N, BM), sizes(BT // 16, m0, p.M, BT)
+        xrows = -(-BT // ROW_STEP)
+        wsize, xsize = sizes(BM // ROW_STEP, n0, p.N, BM), sizes(xrows, m0, p.M, BT)
+        half = t("pred")                                       # BT is a multiple of 16: the last step may be half a one
+        ins(f"setp.lt.u32 {half}, {r0}, {BT - (xrows - 1) * ROW_STEP}")
         kit_it, st, stage_addr = t("b32"), t("b32"), t("b32")
-        full_lag, lag_bar = t("b32"), t("b32")
         ins(f"mov.u32 {kit_it}, 0")
         ins(f"mov.u32 {st}, 0")
         ins(f"mov.u32 {stage_addr}, {soff}")
-        ins(f"mov.u32 {lag_bar}, 0")
         ph = t("b32")
         ins(f"mov.u32 {ph}, 1")                                # parity of the empty barrier's previous phase
-        ptop, pdrain = lab("lr_load"), lab("lr_drain")
+        ptop = lab("lr_load")
         place(ptop)
         eb = t("b32")
         ins(f"mad.lo.u32 {eb}, {st}, 8, {bars}")
@@ -495,44 +525,30 @@ class LinearRows(TunedKernel):
             ins(f"setp.lt.u32 {q}, {k8}, {p.K}")
             ins(f"selp.u32 {ksize}, 16, 0, {q}")
 
-        def copy(off: int, src: str, goff: int, size, hint: str = "") -> None:
+        def copy(off: int, src: str, goff: int, size, hint: str = "", when: str = "") -> None:
             if size is not None and ksize is not None:
                 z = t("b32")
                 ins(f"and.b32 {z}, {size}, {ksize}")
             else:
                 z = size if size is not None else ksize
-            ins(f"cp.async.cg.shared.global{hint} [{stage_addr}+{off}], [{src}+{goff}], 16{f', {z}' if z else ''}")
+            ins(f"{when}cp.async.cg.shared.global{hint} [{stage_addr}+{off}], [{src}+{goff}], 16{f', {z}' if z else ''}")
 
         for g in range(G):
             src = wp
             if g:
                 src = t("b64")
                 ins(f"add.u64 {src}, {wp}, {p.N * p.K * 2}")
-            for i in range(BM // 16):
-                copy(g * ROW_SLAB + i * 2048, src, i * 16 * p.K * 2, wsize[i], ".L2::256B")
-        for i in range(BT // 16):
-            copy(G * ROW_SLAB + i * 2048, xp, i * 16 * p.K * 2, xsize[i])
-        ins("cp.async.commit_group")
+            for i in range(BM // ROW_STEP):
+                copy(g * ROW_SLAB + i * ROW_STEP * 128, src, i * ROW_STEP * p.K * 2, wsize[i], ".L2::256B")
+        for i in range(xrows):
+            copy(G * ROW_SLAB + i * ROW_STEP * 128, xp, i * ROW_STEP * p.K * 2, xsize[i],
+                 when=f"@{half} " if i == xrows - 1 and BT % ROW_STEP else "")
+        # this thread's arrival on the stage's barrier, once its copies have landed
+        ins(f"cp.async.mbarrier.arrive.noinc.shared::cta.b64 [{eb}]")
         ins(f"add.u64 {wp}, {wp}, {BK * 2}")
         ins(f"add.u64 {xp}, {xp}, {BK * 2}")
         ins(f"add.u32 {k8}, {k8}, {BK}")
         ins(f"add.u32 {kit_it}, {kit_it}, 1")
-        # the stage loaded ST - 1 iterations ago is complete: hand it to the tensor cores
-        nolag = lab("lr_nolag")
-        ins(f"setp.lt.u32 {q}, {kit_it}, {ST}")
-        ins(f"@{q} bra {nolag}")
-
-        def hand_over(pending: int) -> None:
-            ins(f"cp.async.wait_group {pending}")
-            ins("fence.proxy.async.shared::cta")
-            ins(f"mad.lo.u32 {full_lag}, {lag_bar}, 8, {bars}")
-            ins(f"mbarrier.arrive.shared::cta.b64 _, [{full_lag}]")
-            ins(f"add.u32 {lag_bar}, {lag_bar}, 1")
-            ins(f"setp.eq.u32 {q}, {lag_bar}, {ST}")
-            ins(f"selp.u32 {lag_bar}, 0, {lag_bar}, {q}")
-
-        hand_over(ST - 1)
-        place(nolag)
         ins(f"add.u32 {st}, {st}, 1")
         ins(f"add.u32 {stage_addr}, {stage_addr}, {stage_bytes}")
         ins(f"setp.eq.u32 {q}, {st}, {ST}")
@@ -543,19 +559,23 @@ class LinearRows(TunedKernel):
         ins(f"xor.b32 {ph}, {ph}, {flip}")
         ins(f"setp.lt.u32 {q}, {kit_it}, {nk}")
         ins(f"@{q} bra {ptop}")
-        # the stages still in flight, oldest first: min(nk, ST - 1) of them
-        place(pdrain)
-        for left in range(ST - 2, -1, -1):
-            none = lab("lr_none")
-            ins(f"setp.le.u32 {q}, {nk}, {left}")
-            ins(f"@{q} bra {none}")
-            hand_over(left)
-            place(none)
-        self._epilogue(kit, tid, warp, lane, tmem, bars, done_off, ex, rank, n0, m0, end)
+        self._epilogue(kit, tid, warp, bars, done_off, alloc_off, slot_off, ex, rank, n0, m0, end)
         ins(f"bra {end}")
 
-        # ---------------- MMA issuer (warp 4) ----------------
+        # ---------------- MMA issuer (warp 8) ----------------
         place(role_mma)
+        slot, tmem = t("b32"), t("b32")
+        ins(f"add.u32 {slot}, {bars}, {slot_off}")
+        ins(f"tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [{slot}], {pl.tmem_cols}")
+        ins("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned")
+        # the next kernel's CTAs may share the SM from here on, not before: one that took the tensor memory
+        # this CTA still had to allocate would keep it until this grid ends
+        self.pdl_trigger()
+        ins("bar.warp.sync -1")
+        ins(f"ld.shared.u32 {tmem}, [{slot}]")
+        first_lane = t("pred")
+        ins(f"setp.eq.u32 {first_lane}, {lane}, 0")
+        ins(f"@{first_lane} mbarrier.arrive.shared::cta.b64 _, [{bars}+{alloc_off}]")
         one = t("pred")
         elect_one(em, one)
         hi, it2, st2, par, first = t("b32"), t("b32"), t("b32"), t("b32"), t("pred")
@@ -571,6 +591,8 @@ class LinearRows(TunedKernel):
         fb, sa = t("b32"), t("b32")
         ins(f"mad.lo.u32 {fb}, {st2}, 8, {bars}")
         kit.wait(fb, par, 1)
+        # the copies wrote through the generic proxy, the tensor cores read through the async one
+        ins("fence.proxy.async.shared::cta")
         ins("tcgen05.fence::after_thread_sync")
         ins(f"mad.lo.u32 {sa}, {st2}, {stage_bytes}, {base}")
         sx = t("b32")
@@ -611,143 +633,196 @@ class LinearRows(TunedKernel):
         ins("tcgen05.fence::before_thread_sync")
         ins("barrier.sync 0")
         nod = lab("lr_nodealloc")
-        ins(f"setp.ne.u32 {q}, {warp}, 4")
+        ins(f"setp.ne.u32 {q}, {warp}, {MMA_WARP}")
         ins(f"@{q} bra {nod}")
         ins("tcgen05.fence::after_thread_sync")
         ins(f"tcgen05.dealloc.cta_group::1.sync.aligned.b32 {tmem}, {pl.tmem_cols}")
         place(nod)
 
-    def _read_sums(self, tmem: str, c0: int, n: int) -> list[list[str]]:
-        """Columns c0 .. c0 + n of this thread's accumulator row(s)."""
+    def _read_sums(self, tmem: str, n: int) -> list[list[str]]:
+        """The ``n`` columns at ``tmem`` of this thread's accumulator row(s)."""
         em, out = self.em, []
         for g in range(self.plan.G):
             v, a = em.tmps("b32", n), em.tmp("b32")
-            em.ins(f"add.u32 {a}, {tmem}, {g * self.plan.BT + c0}")
+            em.ins(f"add.u32 {a}, {tmem}, {g * self.plan.BT}")
             em.ins(f"tcgen05.ld.sync.aligned.32x32b.x{n}.b32 {{{', '.join(v)}}}, [{a}]")
             out.append(v)
         em.ins("tcgen05.wait::ld.sync.aligned")
         return out
 
-    def _epilogue(self, kit, tid, warp, lane, tmem, bars, done_off, ex, rank, n0, m0, end) -> None:
+    def _epilogue(self, kit, tid, warp, bars, done_off, alloc_off, slot_off, ex, rank, n0, m0, end) -> None:
         """The sums of row n (of w) by token, to C[m0 + token, n].
 
-        S = 1: a thread holds row ``tid``, its tokens in tensor-memory columns; a warp's loads and stores
-        of one token are 32 consecutive columns of C.  S > 1: each rank owns 128 / S rows; every CTA
-        stores its sums of those rows into the owner's exchange area [rank][accumulator][token][row], the
-        cluster meets, and the owner's threads (row, token mod S) add the ranks' sums in order."""
+        Warps w and w + 4 hold the same 32 rows of w and take alternate groups of eight tokens.  S = 1: a
+        warp's loads and stores of one token are 32 consecutive columns of C.  S > 1: each rank owns
+        128 / S rows; every CTA stores its sums of those rows into the owner's exchange area
+        [rank][accumulator][token][row], a warp's 32 rows of a token in one store; the cluster meets, and
+        the owner's threads (a row, four tokens) add the ranks' sums in order."""
         em, t, ins, place, lab = self.em, self.em.tmp, self.em.ins, self.em.place, self.em.label
         p, pl = self.p, self.plan
         S, BT, G = pl.S, pl.BT, pl.G
         q = t("pred")
-        lane_off = t("b32")
-        ins(f"shl.b32 {lane_off}, {warp}, 21")                 # (32 * warp) << 16
-        acc = t("b32")
-        ins(f"add.u32 {acc}, {tmem}, {lane_off}")
+        row, side, c = t("b32"), t("b32"), t("b32")            # of w's 128; which of the two warps; first token
+        ins(f"and.b32 {row}, {tid}, {BM - 1}")
+        ins(f"shr.u32 {side}, {warp}, 2")
+        ins(f"shl.b32 {c}, {side}, 3")
         left = t("b32")                                        # tokens of this tile
         ins(f"sub.s32 {left}, {p.M}, {m0}")
         ins(f"min.s32 {left}, {left}, {BT}")
-        zero = t("b32")
+        zero, acc = t("b32"), t("b32")
         ins(f"mov.u32 {zero}, 0")
+
+        def sums_ready() -> None:
+            """Every MMA is done: ``acc`` addresses this thread's row at token c."""
+            kit.wait(f"{bars}+{alloc_off}", zero, 2)
+            kit.wait(f"{bars}+{done_off}", zero, 2)
+            ins("tcgen05.fence::after_thread_sync")
+            ins(f"ld.shared.u32 {acc}, [{bars}+{slot_off}]")
+            ins(f"add.u32 {acc}, {acc}, {c}")
+            lanes = t("b32")
+            ins(f"and.b32 {lanes}, {warp}, 3")
+            ins(f"shl.b32 {lanes}, {lanes}, 21")               # (32 * (warp mod 4)) << 16
+            ins(f"add.u32 {acc}, {acc}, {lanes}")
+
         if S == 1:
-            n = t("b32")
-            ins(f"add.u32 {n}, {n0}, {tid}")
+            n, m = t("b32"), t("b32")
+            ins(f"add.u32 {n}, {n0}, {row}")
             inside = None
             if p.N % BM:
                 inside = t("pred")
                 ins(f"setp.lt.u32 {inside}, {n}, {p.N}")
             self._columns(n, inside)
-            kit.wait(f"{bars}+{done_off}", zero, 2)
-            ins("tcgen05.fence::after_thread_sync")
-            for c0 in range(0, BT, 16):
-                if c0:
-                    ins(f"setp.le.s32 {q}, {left}, {c0}")
-                    ins(f"@{q} bra {end}")
-                ok, rows = [], []
-                for j in range(16):
-                    o, m = t("pred"), t("b32")
-                    ins(f"setp.gt.s32 {o}, {left}, {c0 + j}" if inside is None else
-                        f"setp.gt.and.s32 {o}, {left}, {c0 + j}, {inside}")
-                    ins(f"add.u32 {m}, {m0}, {c0 + j}")
-                    ok.append(o)
-                    rows.append(m)
-                fetched = [self._fetch(m, n, o) for m, o in zip(rows, ok)]
-                sums = self._read_sums(acc, c0, 16)
-                for j in range(16):
-                    self._finish([v[j] for v in sums], rows[j], n, ok[j], fetched[j])
+            ins(f"add.u32 {m}, {m0}, {c}")
+            ahead = self._tokens(c, m, n, left, inside, 8)
+            sums_ready()
+            ins(f"setp.ge.s32 {q}, {c}, {left}")
+            ins(f"@{q} bra {end}")
+            top = lab("lr_out")
+            place(top)
+            sums = self._read_sums(acc, 8)
+            mine = self._taken(ahead)
+            ins(f"add.u32 {c}, {c}, 16")
+            ins(f"add.u32 {m}, {m}, 16")
+            ins(f"add.u32 {acc}, {acc}, 16")
+            self._tokens(c, m, n, left, inside, 8, into=ahead)
+            for j, (mj, o, fetched) in enumerate(mine):
+                self._finish([v[j] for v in sums], mj, n, o, fetched)
+            ins(f"setp.lt.s32 {q}, {c}, {left}")
+            ins(f"@{q} bra {top}")
             return
         RS = BM // S                                           # rows of w a rank owns
-        owner, mine, dst, dsm = t("b32"), t("b32"), t("b32"), t("b32")
-        ins(f"shr.u32 {owner}, {tid}, {RS.bit_length() - 1}")
-        ins(f"and.b32 {mine}, {tid}, {RS - 1}")
-        ins(f"mad.lo.u32 {dst}, {rank}, {G * BT * RS * 4}, {ex}")
-        ins(f"mad.lo.u32 {dst}, {mine}, 4, {dst}")
+        slab = BT * RS * 4                                     # bytes of one rank's sums of one accumulator
+        owner, dst, dsm = t("b32"), t("b32"), t("b32")
+        ins(f"shr.u32 {owner}, {row}, {RS.bit_length() - 1}")
+        ins(f"and.b32 {row}, {row}, {RS - 1}")
+        ins(f"mad.lo.u32 {dst}, {rank}, {G * slab}, {ex}")
+        ins(f"mad.lo.u32 {dst}, {row}, 4, {dst}")
+        ins(f"mad.lo.u32 {dst}, {c}, {RS * 4}, {dst}")
         ins(f"mapa.shared::cluster.u32 {dsm}, {dst}, {owner}")
-        # this thread's part of the join: row ``mine`` of this rank's, tokens tid / RS + S j
-        n, tok0 = t("b32"), owner
-        ins(f"mad.lo.u32 {n}, {rank}, {RS}, {mine}")
+        # this thread's part of the join: one of this rank's rows, tokens x .. x + 3
+        n, x, m, src = t("b32"), t("b32"), t("b32"), t("b32")
+        ins(f"and.b32 {n}, {tid}, {RS - 1}")
+        ins(f"mad.lo.u32 {src}, {n}, 4, {ex}")
+        ins(f"mad.lo.u32 {n}, {rank}, {RS}, {n}")
         ins(f"add.u32 {n}, {n}, {n0}")
+        ins(f"shr.u32 {x}, {tid}, {RS.bit_length() - 1}")
+        ins(f"shl.b32 {x}, {x}, 2")
+        ins(f"mad.lo.u32 {src}, {x}, {RS * 4}, {src}")
+        ins(f"add.u32 {m}, {m0}, {x}")
+        stride = 4 * (PRODUCERS // RS)                         # tokens of a turn
         inside = None
         if p.N % BM:
             inside = t("pred")
             ins(f"setp.lt.u32 {inside}, {n}, {p.N}")
         self._columns(n, inside)
-        kit.wait(f"{bars}+{done_off}", zero, 2)
-        ins("tcgen05.fence::after_thread_sync")
+        ahead = self._tokens(x, m, n, left, inside, 4)
+        sums_ready()
         ins("barrier.cluster.wait.acquire")
-        sent = lab("lr_sent")
-        for c0 in range(0, BT, 16):
-            if c0:
-                ins(f"setp.le.s32 {q}, {left}, {c0}")
-                ins(f"@{q} bra {sent}")
-            sums = self._read_sums(acc, c0, 16)
-            for j in range(16):
-                o = t("pred")
-                ins(f"setp.gt.s32 {o}, {left}, {c0 + j}")
-                for g in range(G):
-                    ins(f"@{o} st.shared::cluster.b32 [{dsm}+{(g * BT + c0 + j) * RS * 4}], {sums[g][j]}")
+        send, sent, ok, room = lab("lr_send"), lab("lr_sent"), t("pred"), t("b32")
+        ins(f"setp.ge.s32 {q}, {c}, {left}")
+        ins(f"@{q} bra {sent}")
+        place(send)
+        sums = self._read_sums(acc, 8)
+        ins(f"sub.s32 {room}, {left}, {c}")
+        for h in range(8):
+            if h:
+                ins(f"setp.gt.s32 {ok}, {room}, {h}")
+            for g in range(G):
+                ins(f"{f'@{ok} ' if h else ''}st.shared::cluster.b32 [{dsm}+{g * slab + h * RS * 4}], {sums[g][h]}")
+        ins(f"add.u32 {c}, {c}, 16")
+        ins(f"add.u32 {acc}, {acc}, 16")
+        ins(f"add.u32 {dsm}, {dsm}, {16 * RS * 4}")
+        ins(f"setp.lt.s32 {q}, {c}, {left}")
+        ins(f"@{q} bra {send}")
         place(sent)
         ins("barrier.cluster.arrive.release")
         ins("barrier.cluster.wait.acquire")
-        src = t("b32")
-        ins(f"mad.lo.u32 {src}, {mine}, 4, {ex}")
-        ins(f"mad.lo.u32 {src}, {tok0}, {RS * 4}, {src}")
-        chunk = 4
-        per = -(-BT // S)                                      # tokens a thread may have
-        for j0 in range(0, per, chunk):
-            if j0:
-                x = t("b32")
-                ins(f"add.u32 {x}, {tok0}, {j0 * S}")
-                ins(f"setp.le.s32 {q}, {left}, {x}")
-                ins(f"@{q} bra {end}")
-            todo = []
-            for j in range(j0, min(per, j0 + chunk)):
-                x, m, o = t("b32"), t("b32"), t("pred")
-                ins(f"add.u32 {x}, {tok0}, {j * S}")
-                ins(f"setp.gt.s32 {o}, {left}, {x}" if inside is None else
-                    f"setp.gt.and.s32 {o}, {left}, {x}, {inside}")
-                ins(f"add.u32 {m}, {m0}, {x}")
-                todo.append((j, m, o, self._fetch(m, n, o)))
-            for j, m, o, fetched in todo:
-                vals = []
-                for g in range(G):
-                    total = None
-                    for r in range(S):
-                        v = t("f32")
-                        ins(f"mov.f32 {v}, {F32.imm(0.0)}")
-                        ins(f"@{o} ld.shared.f32 {v}, [{src}+{((r * G + g) * BT + j * S) * RS * 4}]")
-                        if total is None:
-                            total = v
-                        else:
-                            ins(f"add.rn.f32 {total}, {total}, {v}")
-                    b = t("b32")
-                    ins(f"mov.b32 {b}, {total}")
-                    vals.append(b)
-                self._finish(vals, m, n, o, fetched)
+        ins(f"setp.ge.s32 {q}, {x}, {left}")
+        ins(f"@{q} bra {end}")
+        top = lab("lr_out")
+        place(top)
+        todo = self._taken(ahead)
+        ins(f"add.u32 {x}, {x}, {stride}")
+        ins(f"add.u32 {m}, {m}, {stride}")
+        self._tokens(x, m, n, left, inside, 4, into=ahead)
+        totals = []
+        for g in range(G):
+            total = None
+            for k in range(S):
+                v = em.tmps("f32", 4)
+                for h, (a, (_, ok, _)) in enumerate(zip(v, todo)):
+                    ins(f"mov.f32 {a}, {F32.imm(0.0)}")
+                    ins(f"@{ok} ld.shared.f32 {a}, [{src}+{(k * G + g) * slab + h * RS * 4}]")
+                if total is None:
+                    total = v
+                else:
+                    for a, b in zip(total, v):
+                        ins(f"add.rn.f32 {a}, {a}, {b}")
+            totals.append(total)
+        for j, (mj, ok, fetched) in enumerate(todo):
+            bits = []
+            for total in totals:
+                bits.append(t("b32"))
+                ins(f"mov.b32 {bits[-1]}, {total[j]}")
+            self._finish(bits, mj, n, ok, fetched)
+        ins(f"add.u32 {src}, {src}, {stride * RS * 4}")
+        ins(f"setp.lt.s32 {q}, {x}, {left}")
+        ins(f"@{q} bra {top}")
 
-    def _load(self, name: str, index: str, pred: str | None) -> list[str]:
+    def _tokens(self, x: str, m: str, n: str, left: str, inside: str | None, count: int,
+                into: list | None = None) -> list:
+        """Tokens x, x + 1, .. of the tile (rows m, m + 1, .. of C): [(row, stored?, sources)], with the
+        sources' loads issued -- into the registers of an earlier call, when given."""
+        em, t, ins, out = self.em, self.em.tmp, self.em.ins, []
+        room = t("b32")
+        ins(f"sub.s32 {room}, {left}, {x}")
+        for j in range(count):
+            mj, o, fetched = into[j] if into else (t("b32"), t("pred"), None)
+            ins(f"setp.gt.s32 {o}, {room}, {j}" if inside is None else
+                f"setp.gt.and.s32 {o}, {room}, {j}, {inside}")
+            ins(f"add.u32 {mj}, {m}, {j}")
+            out.append((mj, o, self._fetch(mj, n, o, fetched)))
+        return out
+
+    def _taken(self, ahead: list) -> list:
+        """The tokens of ``ahead`` in registers of their own (the next ones are loaded over them)."""
+        em, out = self.em, []
+        for mj, o, fetched in ahead:
+            m, p, got = em.tmp("b32"), em.tmp("pred"), dict(fetched)
+            em.ins(f"mov.b32 {m}, {mj}")
+            em.ins(f"mov.pred {p}, {o}")
+            for src, regs in fetched.items():
+                if not src[1]:
+                    v = em.tmp("b32")
+                    em.ins(f"mov.b32 {v}, {regs[0]}")
+                    got[src] = [v]
+            out.append((m, p, got))
+        return out
+
+    def _load(self, name: str, index: str, pred: str | None, into: str | None = None) -> list[str]:
         """One element of a source at a 64-bit element index, zero where ``pred`` is false."""
         em, ty = self.em, self.p.kernel.param(name).ty
-        a, r = em.tmp("b64"), em.tmp("b32")
+        a, r = em.tmp("b64"), into or em.tmp("b32")
         em.ins(f"mad.lo.s64 {a}, {index}, {ty.nbytes}, {em.buffer_reg(name)}")
         at = f"@{pred} " if pred else ""
         em.ins(f"mov.u32 {r}, 0")
@@ -771,7 +846,7 @@ class LinearRows(TunedKernel):
                     em.ins(f"add.u64 {i}, {i}, {src[2]}")
                 self.cols[src] = self._load(src[0], i, inside)
 
-    def _fetch(self, m: str, n: str, ok: str) -> dict:
+    def _fetch(self, m: str, n: str, ok: str, into: dict | None = None) -> dict:
         """The element sources at (m, n), and the columns' ones."""
         em, out = self.em, dict(self.cols)
         for src in self.replay.sources if self.replay else ():
@@ -780,7 +855,7 @@ class LinearRows(TunedKernel):
                 em.ins(f"mul.wide.u32 {i}, {m}, {self.p.N}")
                 em.ins(f"cvt.u64.u32 {c}, {n}")
                 em.ins(f"add.u64 {i}, {i}, {c}")
-                out[src] = self._load(src[0], i, ok)
+                out[src] = self._load(src[0], i, ok, into[src][0] if into else None)
         return out
 
     def _finish(self, sums: list[str], m: str, n: str, ok: str, fetched: dict) -> None:

@@ -145,8 +145,10 @@ class TcMatmulPair(TcMatmul):
     def tile_begin(self, row: str, rank: str, tm: str, tn: str, whole: str, part: str) -> None:
         """Hook: an epilogue thread (its row of the CTA's 128) is about to wait for a tile's sums."""
 
-    def box(self, c0: int, cw: int, width: int, taddr: str) -> list[str]:
-        """Hook: columns c0 .. c0 + cw of this thread's row after ``epilogue``, packed for a store."""
+    def store_tile(self, cw: int, width: int, taddr: str, col0: str, free, stage) -> None:
+        """Hook: ``epilogue`` on ``width`` columns of the accumulator at ``taddr``, stored from column ``col0``
+        on in boxes of ``cw``: ``stage(buffer, values, column, offset)`` writes one, ``free(last)`` releases
+        the accumulator where ``last`` holds."""
         raise NotImplementedError
 
     # ---- the tuned body -------------------------------------------------------------
@@ -481,9 +483,36 @@ class TcMatmulPair(TcMatmul):
                     f"[{sbuf}]")
                 ins(f"@{lane0} cp.async.bulk.commit_group")
 
-        def from_tmem(c0, width=self.tile_cols):
+        def stage_store(b: int, values, cc: str, off: int) -> None:
+            """Box ``b`` (0 or 1, the staging buffer) of a turn of ``store_tile``'s loop."""
+            ins(f"@{lane0} cp.async.bulk.wait_group.read 1")
+            ins("bar.warp.sync -1")
+            v = values()
+            for i in range(4):
+                a_ = t("b32")
+                ins(f"add.u32 {a_}, {stage_buf[b]}, {soff[i]}")
+                ins(f"st.shared.v4.b32 [{a_}], {{{', '.join(v[4 * i:4 * i + 4])}}}")
+            ins("fence.proxy.async.shared::cta")
+            ins("bar.warp.sync -1")
+            c_ = t("b32")
+            ins(f"add.u32 {c_}, {cc}, {off}")
+            ins(f"@{lane0} cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [{tmc}, {{{c_}, {row0}}}], "
+                f"[{stage_buf[b]}]")
+            ins(f"@{lane0} cp.async.bulk.commit_group")
+
+        def free_if(last: str) -> None:
+            keep = lab("mp_keep")
+            ins(f"@!{last} bra {keep}")
+            free_accumulator()
+            place(keep)
+
+        def store(width: int) -> None:
             if self.epilogue is not None:
-                return self.box(c0, cw, width, taddr)
+                self.store_tile(cw, width, taddr, col0, free_if, stage_store)
+            else:
+                store_boxes(from_tmem, True, width)
+
+        def from_tmem(c0):
             nv = 16 if esz == 4 else 32
             v = [t("b32") for _ in range(nv)]
             tc = t("b32")
@@ -500,13 +529,13 @@ class TcMatmulPair(TcMatmul):
         tail = lab("mp_epi_tail")
         if self.rem or self.hrem:
             ins(f"@!{whole3} bra {tail}")
-        store_boxes(from_tmem, True)
+        store(self.tile_cols)
         if self.hrem:
             # a half unit: 128 columns of the tile, starting at 128 h
             ins(f"bra {enext}")
             place(tail)
             ins(f"mad.lo.u32 {col0}, {part3}, {BN // 2}, {col0}")
-            store_boxes(lambda c0: from_tmem(c0, BN // 2), True, BN // 2)
+            store(BN // 2)
         if self.rem:
             ins(f"bra {enext}")
             self._pair_tail(tail, enext, tile3, part3, rank, taddr, row, bars, ls, store_boxes, free_accumulator,
