@@ -67,16 +67,16 @@ def _linear_check(case, t, got, what):
     check(_np(got), want, allowed, what)
 
 
-@pytest.mark.parametrize("launch", ["own", "meta", "generic", "rows", "pair"])
+@pytest.mark.parametrize("launch", ["own", "meta", "generic", "stream", "rows", "pair"])
 @pytest.mark.parametrize("case", LINEAR, ids=str)
 def test_linear(tmp_path, monkeypatch, case, launch):
-    """``rows`` and ``pair`` force one of the two tuned kernels, also at sizes it is not chosen for."""
+    """``stream``, ``rows`` and ``pair`` force one of the tuned kernels, also at sizes it is not chosen for."""
     import torch
     M, N = case[:2]
-    if launch in ("rows", "pair"):
+    if launch in ("stream", "rows", "pair"):
         monkeypatch.setattr(TUNING, "linear_kernel", launch)
     k = _kernel(synth.linear_package(tmp_path, *case), launch)
-    if launch in ("rows", "pair") and not k.family.endswith(launch):
+    if launch in ("stream", "rows", "pair") and not k.family.endswith(launch):
         pytest.skip(f"no {launch} plan for this size")
     t = _linear_inputs(case)
     whole, y = _out((M, N), case[4])
@@ -144,3 +144,344 @@ def test_heads(tmp_path, case, launch):
     torch.cuda.synchronize()
     _heads_check(spec, table, t, out, f"{k.family} {launch}")
     k.close()
+
+
+# ---- as they are used --------------------------------------------------------------------------
+
+def _family(k, *names):
+    assert any(n in k.family for n in names), k.family
+
+
+@pytest.mark.parametrize("dtype", ["f16"])
+def test_a_layer(tmp_path, dtype):
+    """The dense path of a layer on one stream, eagerly and as a captured graph with fresh inputs: projection
+    with bias, norm and rotation into the attention kernel's layout, attention, projection onto the
+    residual stream, gated projection, projection onto the residual stream.  Each output is compared
+    with its float64 definition on what the kernel before it wrote, so a kernel that starts too
+    early shows."""
+    import torch
+    from thompiler import rotary
+    B, S, H, D = 1, 256, 4, 64
+    C, F, T = H * D, 512, B * S
+
+    def linear(name, *a, **kw):
+        return DeviceKernel(synth.linear_package(tmp_path / name, *a, dtype=dtype, **kw) / "k_linear.ir.json")
+    k_qkv = linear("qkv", T, 3 * C, C, bias=True)
+    k_rot = DeviceKernel(synth.qk_norm_rope_package(tmp_path / "rot", B, S, H, H, D, dtype=dtype, table=S + 100,
+                                                    values=True, heads_first=True) / "k_qk_norm_rope.ir.json")
+    k_att = DeviceKernel(synth.attention_package(tmp_path / "att", B, H, S, D) / "k_attention.ir.json")
+    k_out = linear("out", T, C, C, residual=True)
+    k_up = linear("up", T, F, C, activation="silu", gated=True)
+    k_down = linear("down", T, C, F, residual=True)
+    _family(k_rot, "rotary-heads")
+    for k in (k_qkv, k_out, k_up, k_down):
+        _family(k, "linear")
+    g = torch.Generator(device="cuda").manual_seed(11)
+
+    def new(*shape):
+        return torch.empty(*shape, device="cuda", dtype=torch.float16)
+    par = {n: (torch.randn(*s, device="cuda", generator=g) * sc).half() for n, s, sc in (
+        ("wqkv", (3 * C, C), C ** -0.5), ("bqkv", (3 * C,), 0.5), ("wq", (D,), 1.0), ("wk", (D,), 1.0),
+        ("wout", (C, C), C ** -0.5), ("wup", (2 * F, C), C ** -0.5), ("wdown", (C, F), F ** -0.5))}
+    cos, sin = (torch.from_numpy(t).cuda() for t in rotary.tables(S + 100, D))
+    pos = (torch.arange(S, device="cuda", dtype=torch.int32) + 100).repeat(B, 1)
+    scale = torch.tensor([D ** 0.5], device="cuda")
+    x, qkv, q, kk, v, o = new(T, C), new(T, 3 * C), *(new(B, H, S, D) for _ in range(4))
+    o2, h, up, y = new(T, C), new(T, C), new(T, F), new(T, C)
+
+    def p(**t):
+        return {n: a.data_ptr() for n, a in t.items()}
+
+    def run():
+        s = _stream()
+        k_qkv(p(x=x, w=par["wqkv"], bias=par["bqkv"], linear=qkv), s)
+        k_rot(p(cos=cos, sin=sin, pos=pos, qkv=qkv, wq=par["wq"], wk=par["wk"], q=q, k=kk, v=v), s)
+        k_att(p(div_c1=scale, q=q, k=kk, v=v, attn=o), s)
+        o2.copy_(o.permute(0, 2, 1, 3).reshape(T, C))
+        k_out(p(x=o2, w=par["wout"], res=x, linear=h), s)
+        k_up(p(x=h, w=par["wup"], linear=up), s)
+        k_down(p(x=up, w=par["wdown"], res=h, linear=y), s)
+
+    def verify(what):
+        import numpy as np
+        n = {k: _np(t) for k, t in dict(par, x=x, qkv=qkv, q=q, k=kk, v=v, o=o, o2=o2, h=h, up=up, y=y).items()}
+        for name, a, w, b, r, N, act, gated in (
+                ("qkv", "x", "wqkv", "bqkv", None, 3 * C, None, False), ("h", "o2", "wout", None, "x", C, None, False),
+                ("up", "h", "wup", None, None, F, "silu", True), ("y", "up", "wdown", None, "h", C, None, False)):
+            want, allowed = linear_expected(n[a], n[w], n[b] if b else None, n[r] if r else None, N, act, gated, dtype)
+            check(n[name], want, allowed, f"{what} {name}")
+        spec = dict(B=B, S=S, heads=H, kv=H, D=D, R=D, dtype=dtype, interleaved=False, values=True, heads_first=True,
+                    inverse=False, norm=True)
+        src = {"cos": cos.cpu().numpy(), "sin": sin.cpu().numpy(), "pos": pos.cpu().numpy(),
+               "qkv": n["qkv"].reshape(B, S, 3 * H, D), "wq": n["wq"], "wk": n["wk"]}
+        for name, (want, allowed) in heads_expected(src, spec, S + 100, {t: 0.0 for t in "qkv"}).items():
+            check(n[name], want, allowed, f"{what} {name}")
+        s_ = n["q"].astype(np.float64) @ n["k"].astype(np.float64).transpose(0, 1, 3, 2) / D ** 0.5
+        e_ = np.exp(s_ - s_.max(-1, keepdims=True))
+        want = (e_ / e_.sum(-1, keepdims=True)) @ n["v"].astype(np.float64)
+        assert np.allclose(n["o"], want, rtol=2e-2, atol=2e-3), what
+        for k in (k_qkv, k_att, k_out, k_up, k_down):
+            assert k.error_word() == 0
+
+    def refill():
+        x.copy_(torch.randn(T, C, device="cuda", generator=g))
+        for t in (qkv, q, kk, v, o, o2, h, up, y):
+            t.fill_(float("nan"))
+
+    for i in range(3):
+        refill()
+        run()
+        torch.cuda.synchronize()
+        verify(f"eager {i}")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for i in range(3):
+        refill()
+        graph.replay()
+        torch.cuda.synchronize()
+        verify(f"replay {i}")
+    del graph
+    for k in (k_qkv, k_rot, k_att, k_out, k_up, k_down):
+        k.close()
+
+
+@pytest.mark.parametrize("kernel", ["stream", "rows"])
+def test_few_row_kernels_share_a_graph_with_many_weights(tmp_path, monkeypatch, kernel):
+    """One compiled kernel for all layers of a model: twenty weights captured into one graph with no call
+    on them before the capture (nothing is kept for a buffer), replayed with new activations."""
+    import torch
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    M, N = 5, 512
+    case = (M, N, N, "bf16", "bf16", False, "silu", True, False)
+    k = _kernel(synth.linear_package(tmp_path, *case), "own")
+    _family(k, kernel)
+    t = _linear_inputs(case)
+    ws = [torch.randn(N, N, device="cuda").mul_(N ** -0.5).to(torch.bfloat16) for _ in range(20)]
+    ys = [torch.empty(M, N, device="cuda", dtype=torch.bfloat16) for _ in ws]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        src = t["x"]
+        for w, y in zip(ws, ys):                          # each layer's result is the next one's input
+            k({"x": src.data_ptr(), "w": w.data_ptr(), "res": t["res"].data_ptr(), "linear": y.data_ptr()}, _stream())
+            src = y
+    for seed in (1, 2):
+        t["x"].copy_(_linear_inputs(case, seed)["x"])
+        for y in ys:
+            y.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        src = t["x"]
+        for i, (w, y) in enumerate(zip(ws, ys)):
+            _linear_check(case, {"x": src, "w": w, "res": t["res"]}, y, f"layer {i}")
+            src = y
+    assert k.error_word() == 0
+    del graph
+    k.close()
+
+
+@pytest.mark.parametrize("kernel", ["stream", "rows", "pair"])
+def test_two_streams_at_once(tmp_path, monkeypatch, kernel):
+    """Calls of one kernel in flight on two streams, on buffers of their own."""
+    import torch
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    case = (24, 2048, 1024, "f16", "f16", True, "gelu_tanh", True, False)
+    k = _kernel(synth.linear_package(tmp_path, *case), "own")
+    _family(k, kernel)
+    sets = [_linear_inputs(case, s) for s in (1, 2)]
+    outs = [torch.full((24, 2048), float("nan"), device="cuda", dtype=torch.float16) for _ in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for t, y, s in zip(sets, outs, streams):
+            k({n: v.data_ptr() for n, v in dict(t, linear=y).items()}, s.cuda_stream)
+    torch.cuda.synchronize()
+    assert k.error_word() == 0
+    for t, y in zip(sets, outs):
+        _linear_check(case, t, y, kernel)
+    k.close()
+
+
+@pytest.mark.parametrize("kernel", ["stream", "rows", "pair", "generic"])
+def test_not_finite(tmp_path, monkeypatch, kernel):
+    """NaN and infinities stay in the rows and columns they belong to: a NaN row of x, an infinite row of w,
+    an infinite residual; the padding of K, M and N adds none."""
+    import torch
+    if kernel != "generic":
+        monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    case = (20, 200, 136, "bf16", "bf16", True, "silu", True, False)
+    k = _kernel(synth.linear_package(tmp_path, *case), "generic" if kernel == "generic" else "own")
+    t = _linear_inputs(case)
+    t["x"][3, 7] = float("nan")
+    t["w"][199, 135] = float("inf")
+    t["x"][:, 135] = t["x"][:, 135].abs() + 0.5           # inf * x stays +inf: silu(+inf) = +inf
+    t["res"][5, 11] = float("-inf")
+    y = torch.zeros(20, 200, device="cuda", dtype=torch.bfloat16)
+    k({n: v.data_ptr() for n, v in dict(t, linear=y).items()}, _stream())
+    torch.cuda.synchronize()
+    got = _np(y)
+    assert np.isnan(got[3]).all() and np.isposinf(np.delete(got[:, 199], 3)).all() and np.isneginf(got[5, 11])
+    rest = np.ones_like(got, dtype=bool)
+    rest[3], rest[:, 199], rest[5, 11] = False, False, False
+    assert np.isfinite(got[rest]).all()
+    clean = dict(t)
+    clean["x"], clean["w"], clean["res"] = t["x"].clone(), t["w"].clone(), t["res"].clone()
+    clean["x"][3, 7], clean["w"][199, 135], clean["res"][5, 11] = 0, 0, 0
+    x = {n: _np(v) for n, v in clean.items()}
+    want, allowed = linear_expected(x["x"], x["w"], x["bias"], x["res"], 200, "silu", False, "bf16")
+    check(np.where(rest, got, want), want, allowed, kernel)
+    k.close()
+
+
+def test_heads_not_finite(tmp_path):
+    """Of a head that rotates half of its elements, a NaN in the rest stays where it is; with the norm it
+    takes the head and no other."""
+    import torch
+    spec = heads_spec((1, 6, 3, 1, 64, 32, "bf16", True, True, False, False, False))
+    for norm in (False, True):
+        spec["norm"] = norm
+        k = _kernel(heads_package(synth, tmp_path / str(norm), spec, 100), "own")
+        t = _heads_inputs(spec, 100)
+        t["qkv"][0, 2, 1, 40] = float("nan")              # a query head's unrotated part
+        t["qkv"][0, 3, 0, 5] = float("inf")               # a rotated pair
+        t["qkv"][0, 4, 4, 9] = float("nan")               # a value
+        out = _heads_outputs(spec)
+        k(dict({n: v.data_ptr() for n, v in t.items()}, **{n: v.data_ptr() for n, (_, v) in out.items()}), _stream())
+        torch.cuda.synchronize()
+        q, kk, v = (_np(out[n][1]) for n in ("q", "k", "v"))
+        bad = np.argwhere(~np.isfinite(q))
+        heads = {(int(s), int(h)) for _, s, h, _ in bad}
+        assert heads == {(2, 1), (3, 0)}
+        if not norm:
+            assert {int(d) for _, s, _, d in bad if s == 2} == {40}
+            assert {int(d) for _, s, _, d in bad if s == 3} == {4, 5}
+        assert np.isfinite(kk).all() and np.argwhere(~np.isfinite(v)).tolist() == [[0, 4, 0, 9]]
+        k.close()
+
+
+def test_misaligned_buffers(tmp_path):
+    """A buffer that does not start on the boundary its vectors need is refused before the launch, by name; one
+    that starts on a later such boundary is served."""
+    import torch
+    from thompiler.runner import RunnerError
+    for M in (4, 100, 700):
+        case = (M, 64, 64, "f16", "f16", True, None, True, False)
+        k = _kernel(synth.linear_package(tmp_path / str(M), *case), "own")
+        t = _linear_inputs(case)
+        y = torch.zeros(M * 64 + 16, device="cuda", dtype=torch.float16)
+        ptrs = {n: v.data_ptr() for n, v in dict(t, linear=y).items()}
+        for name in ptrs:
+            with pytest.raises(RunnerError, match=f"buffer '{name}' .* not 16-byte aligned"):
+                k(dict(ptrs, **{name: ptrs[name] + 8}), _stream())
+        for name in ptrs:
+            u, at = dict(t), y[:M * 64]
+            if name in u:
+                u[name] = torch.empty(t[name].numel() + 8, device="cuda", dtype=torch.float16)[8:].view(t[name].shape)
+                u[name].copy_(t[name])
+            else:
+                at = y[8:8 + M * 64]
+            y.fill_(float("nan"))
+            k({n: v.data_ptr() for n, v in dict(u, linear=at).items()}, _stream())
+            torch.cuda.synchronize()
+            assert k.error_word() == 0
+            _linear_check(case, t, at.view(M, 64), f"{k.family} {name}")
+        k.close()
+    for D, R, step in ((64, 64, 8), (80, 40, 4), (10, 6, 1)):
+        spec = heads_spec((1, 33, 4, 2, D, R, "f16", False, True, True, False, True))
+        k = _kernel(heads_package(synth, tmp_path / f"h{D}", spec, 100), "own")
+        t = _heads_inputs(spec, 100)
+        for name in ("qkv", "wq", "wk", "q", "k", "v"):
+            out, u = _heads_outputs(spec), dict(t)
+            ptrs = {n: v.data_ptr() for n, v in t.items()}
+            ptrs.update({n: v.data_ptr() for n, (_, v) in out.items()})
+            if step > 1:
+                with pytest.raises(RunnerError, match=f"buffer '{name}' .* not {2 * step}-byte aligned"):
+                    k(dict(ptrs, **{name: ptrs[name] + step}), _stream())
+            whole, src = None, out[name][1] if name in out else t[name]
+            whole = torch.full((src.numel() + 2 * PAD,), SENTINEL, device="cuda", dtype=torch.float16)
+            view = whole[PAD + step:PAD + step + src.numel()].view(src.shape)
+            view.copy_(src)
+            k(dict(ptrs, **{name: view.data_ptr()}), _stream())
+            torch.cuda.synchronize()
+            assert k.error_word() == 0
+            if name in out:
+                out[name][1].copy_(view)
+            _heads_check(spec, 100, t, out, f"{name} at {step}")
+        k.close()
+
+
+def test_offsets_past_32_bits(tmp_path):
+    """Rows and products of more than 2^31 elements: the last ones are right."""
+    import torch
+    spec = heads_spec((1, 400000, 32, 16, 96, 96, "bf16", False, True, False, False, False))
+    assert 400000 * 64 * 96 > 2 ** 31
+    k = _kernel(heads_package(synth, tmp_path / "h", spec, 16), "own")
+    _family(k, "rotary-heads")
+    S, tail = 400000, 3
+    qkv = torch.zeros(1, S, 64, 96, device="cuda", dtype=torch.bfloat16)
+    qkv[:, -tail:] = torch.randn(1, tail, 64, 96, device="cuda").to(torch.bfloat16)
+    small = dict(spec, S=tail)
+    t = _heads_inputs(small, 16)
+    t["qkv"] = qkv[:, -tail:].contiguous()
+    pos = torch.zeros(1, S, device="cuda", dtype=torch.int32)
+    pos[:, -tail:] = t["pos"]
+    out = {n: torch.full((1, S, h, 96), SENTINEL, device="cuda", dtype=torch.bfloat16)
+           for n, h in (("q", 32), ("k", 16), ("v", 16))}
+    ptrs = {n: v.data_ptr() for n, v in dict(t, qkv=qkv, pos=pos, **out).items()}
+    k(ptrs, _stream())
+    torch.cuda.synchronize()
+    x = {n: v.cpu().numpy() if n == "pos" else _np(v) for n, v in t.items()}
+    for name, (want, allowed) in heads_expected(x, small, 16, {n: SENTINEL for n in out}).items():
+        check(_np(out[name][:, -tail:]), want, allowed, name)
+    k.close()
+    del qkv, out, pos
+    torch.cuda.empty_cache()
+    M, N, K = 33000, 65536, 64
+    case = (M, N, K, "f16", "f16", False, None, True, False)
+    k = _kernel(synth.linear_package(tmp_path / "l", *case), "own")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, w = (torch.randn(n, K, device="cuda", generator=g).half() for n in (M, N))
+    y = torch.full((M, N), float("nan"), device="cuda", dtype=torch.float16)
+    res = torch.zeros(M, N, device="cuda", dtype=torch.float16)
+    res[-2:] = torch.randn(2, N, device="cuda", generator=g).half()
+    k({"x": x.data_ptr(), "w": w.data_ptr(), "res": res.data_ptr(), "linear": y.data_ptr()}, _stream())
+    torch.cuda.synchronize()
+    assert k.error_word() == 0
+    for rows in (slice(0, 2), slice(M - 2, M)):
+        want, allowed = linear_expected(_np(x[rows]), _np(w), None, _np(res[rows]), N, None, False, "f16")
+        check(_np(y[rows]), want, allowed, "linear")
+    k.close()
+
+
+def test_rotation_inverse_undoes_and_is_the_gradient(tmp_path):
+    """inverse(rope(x)) = x; and for a linear map, <g, rope(x)> = <inverse(g), x>: the inverse rotation is
+    the gradient, checked against differences of the forward kernel too."""
+    import torch
+    spec = heads_spec((2, 17, 4, 0, 64, 48, "f32", True, False, False, False, False))
+    fwd = _kernel(heads_package(synth, tmp_path / "f", spec, 64), "own")
+    bwd = _kernel(heads_package(synth, tmp_path / "b", dict(spec, inverse=True), 64), "own")
+    t = _heads_inputs(spec, 64)
+
+    def call(k, x):
+        y = torch.zeros_like(x)
+        k({"cos": t["cos"].data_ptr(), "sin": t["sin"].data_ptr(), "pos": t["pos"].data_ptr(), "qkv": x.data_ptr(),
+           "q": y.data_ptr()}, _stream())
+        torch.cuda.synchronize()
+        return y
+    x = t["qkv"]
+    y = call(fwd, x)
+    # each pair: two products and a sum twice over, of values below 2^3: 2^-24 * 8 * 8
+    assert (call(bwd, y) - x).abs().max().item() <= 2.0 ** -18
+    g = torch.randn_like(x)
+    dx = call(bwd, g).double()
+    lhs, rhs = (g.double() * y.double()).sum().item(), (dx * x.double()).sum().item()
+    assert abs(lhs - rhs) <= 2.0 ** -20 * (g.double().abs() * y.double().abs()).sum().item()
+    for i in (0, 777, 2049, x.numel() - 1):               # differences: the map is linear, so a step of 1 is exact
+        e = x.clone()
+        e.view(-1)[i] += 1.0
+        step = (e.view(-1)[i] - x.view(-1)[i]).item()
+        diff = ((call(fwd, e).double() - y.double()) * g.double()).sum().item() / step
+        # the rotated pair of the changed element differs by roundings of values below 2^3
+        assert abs(diff - dx.view(-1)[i].item()) <= 2.0 ** -18 * (1 + g.abs().max().item())
+    fwd.close()
+    bwd.close()

@@ -88,6 +88,19 @@ class TunedKernel:
         return em.render(prologue.header(), self.k.name, prologue.params(self.k))
 
     # helpers ----------------------------------------------------------------
+    def refuse(self, bad: str, code: int) -> None:
+        """Place ``bad``: record ``code`` in the module's error word and leave.  For a launch in the tuned
+        geometry that the tuned body cannot serve: the generic lowering needs meta.json's."""
+        em = self.em
+        em.module(".global .align 4 .u32 thc_error")
+        skip, a = em.label("served"), em.tmp("b64")
+        em.ins(f"bra {skip}")
+        em.place(bad)
+        em.ins(f"mov.u64 {a}, thc_error")
+        em.ins(f"atom.global.or.b32 {em.tmp('b32')}, [{a}], {1 << code}")
+        em.ins("ret")
+        em.place(skip)
+
     def special(self, reg: str) -> str:
         r = self.em.tmp("b32")
         self.em.ins(f"mov.u32 {r}, {reg}")

@@ -46,10 +46,7 @@ class RotaryHeads(TunedKernel):
         self.heads_first, self.inverse, self.eps = heads_first, inverse, eps
         self.T = B * S
         self.n = heads + kv * (2 if values else 1)
-        V = 16 // ty.nbytes
-        while (R // 2) % V or ((D - R) // 2) % V:
-            V //= 2
-        self.V = V
+        self.V = V = schedules.heads_vector(D, R, ty.nbytes)
         self.J = D // 2 // V                                  # lanes' items in a head
         self.lanes = min(32, _pow2_at_least(self.J))
         self.items = -(-self.J // 32)                         # items a lane holds
@@ -120,7 +117,8 @@ class RotaryHeads(TunedKernel):
     # ---- launch ------------------------------------------------------------------
 
     def sidecar(self) -> dict:
-        return {"grid": [self.grid, 1, 1], "block": [self.threads, 1, 1], "smem_bytes": 0}
+        return {"grid": [self.grid, 1, 1], "block": [self.threads, 1, 1], "smem_bytes": 0,
+                "error_word": "thc_error"}
 
     def guard(self, generic: str) -> None:
         em = self.em
@@ -129,14 +127,25 @@ class RotaryHeads(TunedKernel):
         em.ins(f"@{p} bra {generic}")
         em.ins(f"setp.lt.u32 {p}, {self.special('%nctaid.x')}, {self.grid}")
         em.ins(f"@{p} bra {generic}")
-        # every vector access aligned: V elements of the rows, up to four table entries
+        # every vector access aligned: V elements of the rows, up to four table entries.  (The runner refuses
+        # such calls; a launch that covers the generic lowering's heads is served by it)
+        bad = em.label("misaligned")
         for prm in self.k.params:
             align = 4 if prm.name == "pos" else min(16, self.V * prm.ty.nbytes)
             if align > prm.ty.nbytes:
                 a = em.tmp("b64")
                 em.ins(f"and.b64 {a}, {em.buffer_reg(prm.name)}, {align - 1}")
                 em.ins(f"setp.ne.u64 {p}, {a}, 0")
-                em.ins(f"@{p} bra {generic}")
+                em.ins(f"@{p} bra {bad}")
+        covered = em.label("covered")
+        em.ins(f"bra {covered}")
+        em.place(bad)
+        em.ins(f"setp.ge.u32 {p}, {self.special('%nctaid.x')}, {-(-self.T * self.n * 32 // self.threads)}")
+        em.ins(f"@{p} bra {generic}")
+        short = em.label("short")
+        em.ins(f"bra {short}")
+        em.place(covered)
+        self.refuse(short, 4)
 
     # ---- emission ------------------------------------------------------------------
 

@@ -116,15 +116,15 @@ class Replay:
                     return False
         return True
 
-    def check_alignment(self, generic: str) -> None:
-        """Branch to ``generic`` unless every source takes 16-byte accesses."""
+    def check_alignment(self, bad: str) -> None:
+        """Branch to ``bad`` unless every source takes 16-byte accesses (the runner refuses such calls)."""
         em = self.f.em
         q = em.tmp("pred")
         for name in sorted({s[0] for s in self.sources}):
             a = em.tmp("b64")
             em.ins(f"and.b64 {a}, {em.buffer_reg(name)}, 15")
             em.ins(f"setp.ne.u64 {q}, {a}, 0")
-            em.ins(f"@{q} bra {generic}")
+            em.ins(f"@{q} bra {bad}")
 
     def unpacked(self, regs: list[str], i: int, ty: Ty) -> str:
         """Element ``i`` of packed ``regs`` as its load would leave it: an f32 value, or f16's b16."""
@@ -219,14 +219,16 @@ class LinearPair(TcMatmulPair):
         return out
 
     def estimate(self) -> float:
-        """Microseconds, as ``RowsPlan.estimate``: a 256-wide tile's K block takes about 0.28."""
-        memory = self.p.w.nbytes / 5.5e6
-        return max(memory, min(self.plans(self.p))[0] * self.kblocks * 0.28) + 8
+        """Microseconds (``choose`` says how the constants came about)."""
+        waves = min(self.plans(self.p))[0]
+        return 1.4 + ((self.p.w.nbytes / 4.6e6) ** 4 + (waves * self.kblocks * 0.31) ** 4) ** 0.25 + 4.1 * waves
 
     def guard(self, generic: str) -> None:
         super().guard(generic)
         if self.replay:
-            self.replay.check_alignment(generic)
+            bad = self.em.label("misaligned")
+            self.replay.check_alignment(bad)
+            self.refuse(bad, 4)
 
     # ---- the epilogue, a box of columns at a time -----------------------------------------
 
@@ -369,7 +371,108 @@ MMA_WARP = PRODUCERS // 32
 ROW_STEP = PRODUCERS // 8                    # rows that the producers copy a piece of at a time
 
 
-class LinearRows(TunedKernel):
+class ByElement(TunedKernel):
+    """What the kernels for few rows share: a thread finishes single elements of C."""
+
+    def __init__(self, p: Product):
+        super().__init__(p.kernel)
+        self.p = p
+        self.replay = Replay(self, p) if p.epilogue is not None else None
+
+    def _tokens(self, x: str, m: str, n: str, left: str, inside: str | None, count: int,
+                into: list | None = None) -> list:
+        """Tokens x, x + 1, .. of the tile (rows m, m + 1, .. of C): [(row, stored?, sources)], with the
+        sources' loads issued -- into the registers of an earlier call, when given."""
+        em, t, ins, out = self.em, self.em.tmp, self.em.ins, []
+        room = t("b32")
+        ins(f"sub.s32 {room}, {left}, {x}")
+        for j in range(count):
+            mj, o, fetched = into[j] if into else (t("b32"), t("pred"), None)
+            ins(f"setp.gt.s32 {o}, {room}, {j}" if inside is None else
+                f"setp.gt.and.s32 {o}, {room}, {j}, {inside}")
+            ins(f"add.u32 {mj}, {m}, {j}")
+            out.append((mj, o, self._fetch(mj, n, o, fetched)))
+        return out
+
+    def _taken(self, ahead: list) -> list:
+        """The tokens of ``ahead`` in registers of their own (the next ones are loaded over them)."""
+        em, out = self.em, []
+        for mj, o, fetched in ahead:
+            m, p, got = em.tmp("b32"), em.tmp("pred"), dict(fetched)
+            em.ins(f"mov.b32 {m}, {mj}")
+            em.ins(f"mov.pred {p}, {o}")
+            for src, regs in fetched.items():
+                if not src[1]:
+                    v = em.tmp("b32")
+                    em.ins(f"mov.b32 {v}, {regs[0]}")
+                    got[src] = [v]
+            out.append((m, p, got))
+        return out
+
+    def _load(self, name: str, index: str, pred: str | None, into: str | None = None) -> list[str]:
+        """One element of a source at a 64-bit element index, zero where ``pred`` is false."""
+        em, ty = self.em, self.p.kernel.param(name).ty
+        a, r = em.tmp("b64"), into or em.tmp("b32")
+        em.ins(f"mad.lo.s64 {a}, {index}, {ty.nbytes}, {em.buffer_reg(name)}")
+        at = f"@{pred} " if pred else ""
+        em.ins(f"mov.u32 {r}, 0")
+        if ty.nbytes == 4:
+            em.ins(f"{at}ld.global.nc.b32 {r}, [{a}]")
+        else:
+            h = em.tmp("b16")
+            em.ins(f"{at}ld.global.nc.b16 {h}, [{a}]")
+            em.ins(f"{at}cvt.u32.u16 {r}, {h}")
+        return [r]
+
+    def _columns(self, n: str, inside: str | None) -> None:
+        """The sources over columns, at this thread's column."""
+        em = self.em
+        self.cols = {}
+        for src in self.replay.sources if self.replay else ():
+            if src[1]:
+                i = em.tmp("b64")
+                em.ins(f"cvt.u64.u32 {i}, {n}")
+                if src[2]:
+                    em.ins(f"add.u64 {i}, {i}, {src[2]}")
+                self.cols[src] = self._load(src[0], i, inside)
+
+    def _fetch(self, m: str, n: str, ok: str, into: dict | None = None) -> dict:
+        """The element sources at (m, n), and the columns' ones."""
+        em, out = self.em, dict(self.cols)
+        for src in self.replay.sources if self.replay else ():
+            if not src[1]:
+                i, c = em.tmp("b64"), em.tmp("b64")
+                em.ins(f"mul.wide.u32 {i}, {m}, {self.p.N}")
+                em.ins(f"cvt.u64.u32 {c}, {n}")
+                em.ins(f"add.u64 {i}, {i}, {c}")
+                out[src] = self._load(src[0], i, ok, into[src][0] if into else None)
+        return out
+
+    def _finish(self, sums: list[str], m: str, n: str, ok: str, fetched: dict) -> None:
+        """Epilogue of one element and its store."""
+        em, t, ins, c = self.em, self.em.tmp, self.em.ins, self.p.c
+        vals = []
+        for b in sums:
+            f = t("f32")
+            ins(f"mov.b32 {f}, {b}")
+            vals.append(f)
+        y = vals[0]
+        if self.replay:
+            y = self.replay.element(vals[0], vals[1] if len(vals) > 1 else None, m, n, lambda src: (fetched[src], 0))
+        i, k = t("b64"), t("b64")
+        ins(f"mul.wide.u32 {i}, {m}, {self.p.N}")
+        ins(f"cvt.u64.u32 {k}, {n}")
+        ins(f"add.u64 {i}, {i}, {k}")
+        ins(f"mad.lo.s64 {i}, {i}, {c.ty.nbytes}, {em.buffer_reg(c.name)}")
+        if c.ty is F32:
+            ins(f"@{ok} st.global.f32 [{i}], {y}")
+        else:
+            h = t("b16")
+            ins(f"cvt.rn.{c.ty.ptx}.f32 {h}, {y}")
+            ins(f"@{ok} st.global.b16 [{i}], {h}")
+
+
+class LinearRows(ByElement):
     """Few rows of x against all of w, bound by reading w once.  The roles are turned: 128 rows of w are
     the tensor cores' M side and ``BT`` rows of x (16 .. 256, exactly the batch rounded up) the N
     side, so a small batch wastes no tensor-core rows and w streams through in its own layout.
@@ -387,9 +490,8 @@ class LinearRows(TunedKernel):
     family = "tcgen05-linear-rows"
 
     def __init__(self, p: Product, plan: "RowsPlan"):
-        super().__init__(p.kernel)
-        self.p, self.plan = p, plan
-        self.replay = Replay(self, p) if p.epilogue is not None else None
+        super().__init__(p)
+        self.plan = plan
 
     def sidecar(self) -> dict:
         pl = self.plan
@@ -405,8 +507,10 @@ class LinearRows(TunedKernel):
         q = em.tmp("pred")
         em.ins(f"setp.ne.u32 {q}, {self.special('%ntid.x')}, {PRODUCERS + 32}")
         em.ins(f"@{q} bra {generic}")
+        bad = em.label("other_grid")
         em.ins(f"setp.ne.u32 {q}, {self.special('%nctaid.x')}, {self.plan.ctas}")
-        em.ins(f"@{q} bra {generic}")
+        em.ins(f"@{q} bra {bad}")
+        self.refuse(bad, 4)
 
     def emit_tuned(self) -> None:  # noqa: C901 - one kernel, written out in order
         em, t, ins, place, lab = self.em, self.em.tmp, self.em.ins, self.em.place, self.em.label
@@ -789,98 +893,6 @@ class LinearRows(TunedKernel):
         ins(f"setp.lt.s32 {q}, {x}, {left}")
         ins(f"@{q} bra {top}")
 
-    def _tokens(self, x: str, m: str, n: str, left: str, inside: str | None, count: int,
-                into: list | None = None) -> list:
-        """Tokens x, x + 1, .. of the tile (rows m, m + 1, .. of C): [(row, stored?, sources)], with the
-        sources' loads issued -- into the registers of an earlier call, when given."""
-        em, t, ins, out = self.em, self.em.tmp, self.em.ins, []
-        room = t("b32")
-        ins(f"sub.s32 {room}, {left}, {x}")
-        for j in range(count):
-            mj, o, fetched = into[j] if into else (t("b32"), t("pred"), None)
-            ins(f"setp.gt.s32 {o}, {room}, {j}" if inside is None else
-                f"setp.gt.and.s32 {o}, {room}, {j}, {inside}")
-            ins(f"add.u32 {mj}, {m}, {j}")
-            out.append((mj, o, self._fetch(mj, n, o, fetched)))
-        return out
-
-    def _taken(self, ahead: list) -> list:
-        """The tokens of ``ahead`` in registers of their own (the next ones are loaded over them)."""
-        em, out = self.em, []
-        for mj, o, fetched in ahead:
-            m, p, got = em.tmp("b32"), em.tmp("pred"), dict(fetched)
-            em.ins(f"mov.b32 {m}, {mj}")
-            em.ins(f"mov.pred {p}, {o}")
-            for src, regs in fetched.items():
-                if not src[1]:
-                    v = em.tmp("b32")
-                    em.ins(f"mov.b32 {v}, {regs[0]}")
-                    got[src] = [v]
-            out.append((m, p, got))
-        return out
-
-    def _load(self, name: str, index: str, pred: str | None, into: str | None = None) -> list[str]:
-        """One element of a source at a 64-bit element index, zero where ``pred`` is false."""
-        em, ty = self.em, self.p.kernel.param(name).ty
-        a, r = em.tmp("b64"), into or em.tmp("b32")
-        em.ins(f"mad.lo.s64 {a}, {index}, {ty.nbytes}, {em.buffer_reg(name)}")
-        at = f"@{pred} " if pred else ""
-        em.ins(f"mov.u32 {r}, 0")
-        if ty.nbytes == 4:
-            em.ins(f"{at}ld.global.nc.b32 {r}, [{a}]")
-        else:
-            h = em.tmp("b16")
-            em.ins(f"{at}ld.global.nc.b16 {h}, [{a}]")
-            em.ins(f"{at}cvt.u32.u16 {r}, {h}")
-        return [r]
-
-    def _columns(self, n: str, inside: str | None) -> None:
-        """The sources over columns, at this thread's column."""
-        em = self.em
-        self.cols = {}
-        for src in self.replay.sources if self.replay else ():
-            if src[1]:
-                i = em.tmp("b64")
-                em.ins(f"cvt.u64.u32 {i}, {n}")
-                if src[2]:
-                    em.ins(f"add.u64 {i}, {i}, {src[2]}")
-                self.cols[src] = self._load(src[0], i, inside)
-
-    def _fetch(self, m: str, n: str, ok: str, into: dict | None = None) -> dict:
-        """The element sources at (m, n), and the columns' ones."""
-        em, out = self.em, dict(self.cols)
-        for src in self.replay.sources if self.replay else ():
-            if not src[1]:
-                i, c = em.tmp("b64"), em.tmp("b64")
-                em.ins(f"mul.wide.u32 {i}, {m}, {self.p.N}")
-                em.ins(f"cvt.u64.u32 {c}, {n}")
-                em.ins(f"add.u64 {i}, {i}, {c}")
-                out[src] = self._load(src[0], i, ok, into[src][0] if into else None)
-        return out
-
-    def _finish(self, sums: list[str], m: str, n: str, ok: str, fetched: dict) -> None:
-        """Epilogue of one element and its store."""
-        em, t, ins, c = self.em, self.em.tmp, self.em.ins, self.p.c
-        vals = []
-        for b in sums:
-            f = t("f32")
-            ins(f"mov.b32 {f}, {b}")
-            vals.append(f)
-        y = vals[0]
-        if self.replay:
-            y = self.replay.element(vals[0], vals[1] if len(vals) > 1 else None, m, n, lambda src: (fetched[src], 0))
-        i, k = t("b64"), t("b64")
-        ins(f"mul.wide.u32 {i}, {m}, {self.p.N}")
-        ins(f"cvt.u64.u32 {k}, {n}")
-        ins(f"add.u64 {i}, {i}, {k}")
-        ins(f"mad.lo.s64 {i}, {i}, {c.ty.nbytes}, {em.buffer_reg(c.name)}")
-        if c.ty is F32:
-            ins(f"@{ok} st.global.f32 [{i}], {y}")
-        else:
-            h = t("b16")
-            ins(f"cvt.rn.{c.ty.ptx}.f32 {h}, {y}")
-            ins(f"@{ok} st.global.b16 [{i}], {h}")
-
 
 class RowsPlan:
     """Tiles and launch of ``LinearRows``: ``BT`` tokens a tile, K in ``S`` parts."""
@@ -894,8 +906,9 @@ class RowsPlan:
         self.stage_bytes = self.G * ROW_SLAB + BT * BK * 2
         self.exchange = self.G * BT * BM * 4 if S > 1 else 0
         self.tmem_cols = max(32, 1 << (self.G * BT - 1).bit_length())
-        # two CTAs an SM where the launch has more than one for each
-        half = self.ctas > SM_COUNT
+        # two CTAs an SM where the launch has more than one for each, or clusters so large that the SMs of a
+        # processing cluster do not divide into them
+        half = self.ctas > SM_COUNT or S == 8
         room = (SMEM_LIMIT // 2 - 1024 if half else SMEM_LIMIT) - self.exchange - 1024 - 256 - p.static_smem
         self.stages = min(12, -(-self.kblocks // S) + 1, room // self.stage_bytes)
         self.smem = self.stages * self.stage_bytes + self.exchange + 1024 + 256
@@ -927,22 +940,253 @@ class RowsPlan:
         return min(out, key=lambda x: x[:3])[3] if out else None
 
     def estimate(self, p: Product) -> float:
-        """Microseconds: w from memory once, against each SM's share of slabs through its copies and
-        tensor cores."""
-        memory = self.G * p.N * p.K * 2 / 5.5e6
+        """Microseconds.  Reading w once from memory, and an SM's slabs through its copies (81 bytes a cycle)
+        or tensor cores (140 cycles a K block at least), overlap by halves (the power mean); then the
+        join of a cut K and the epilogue, by the tokens a CTA holds."""
         per_sm = -(-self.ctas // SM_COUNT)
-        block = max(self.stage_bytes / 40, 2 * self.BT * self.G, 150) / 1900
-        return max(memory, per_sm * -(-self.kblocks // self.S) * block) + 3 + (1 if self.S > 1 else 0) + self.BT / 64
+        block = max(self.stage_bytes / 81, 0.35 * self.BT * self.G, 140) / 1900
+        memory, sm = p.w.nbytes / 8.9e6, per_sm * -(-self.kblocks // self.S) * block
+        tokens = self.BT * self.G / 100
+        join = 0.3 + 1.5 * tokens if self.S > 1 else 0
+        return 2.2 + (memory ** 1.34 + sm ** 1.34) ** (1 / 1.34) + join + 2.0 * tokens * per_sm / self.S
+
+
+class LinearStream(ByElement):
+    """A handful of rows of x (up to 32) against all of w, bound by reading w once.
+
+    A CTA owns 16 rows of w (16 of each half when gated) and all of K; its eight warps take K in turns
+    of ``U`` 32-wide chunks.  A lane loads 16 bytes of row g and of row g + 8 (g = lane / 4) at
+    k = 8 (lane mod 4): taken as they lie, those registers are the A operand of two m16n8k16 MMAs whose
+    k runs in another order -- the same for w and x, so the sums are the same products -- and the x
+    of eight tokens, loaded by the same pattern, is their B operand.  So w goes from memory to the tensor
+    cores through registers alone, with no barrier between, and a chunk's registers are loaded again
+    as soon as its MMAs have read them.  The eight warps' sums meet in shared memory, added in
+    warp order; a thread finishes one element at a time.
+
+    (mma.sync, because nothing is bound by its rate here: at 1 x 4096 x 4096 the tensor memory's
+    allocation, the operand barriers and the cluster's join of ``LinearRows`` cost a fifth of the time.)"""
+
+    family = "linear-stream"
+
+    def __init__(self, p: Product, plan: "StreamPlan"):
+        super().__init__(p)
+        self.plan = plan
+
+    def sidecar(self) -> dict:
+        return {"grid": [self.plan.ctas, 1, 1], "block": [256, 1, 1], "smem_bytes": self.plan.smem,
+                "error_word": "thc_error"}
+
+    def guard(self, generic: str) -> None:
+        em = self.em
+        em.module(".extern .shared .align 1024 .b8 smem_pool[]")
+        q = em.tmp("pred")
+        em.ins(f"setp.ne.u32 {q}, {self.special('%ntid.x')}, 256")
+        em.ins(f"@{q} bra {generic}")
+        bad = em.label("other_grid")
+        em.ins(f"setp.ne.u32 {q}, {self.special('%nctaid.x')}, {self.plan.ctas}")
+        em.ins(f"@{q} bra {bad}")
+        self.refuse(bad, 4)
+
+    def emit_tuned(self) -> None:
+        em, t, ins, place, lab = self.em, self.em.tmp, self.em.ins, self.em.place, self.em.label
+        p, pl = self.p, self.plan
+        U, NT, G = pl.U, pl.NT, pl.G
+        q = t("pred")
+        self.pdl_trigger()
+        tid, warp, lane, g, k8 = self.special("%tid.x"), t("b32"), t("b32"), t("b32"), t("b32")
+        ins(f"shr.u32 {warp}, {tid}, 5")
+        ins(f"and.b32 {lane}, {tid}, 31")
+        ins(f"shr.u32 {g}, {lane}, 2")
+        ins(f"and.b32 {k8}, {lane}, 3")
+        n0 = t("b32")
+        ins(f"shl.b32 {n0}, {self.special('%ctaid.x')}, 4")
+        k = t("b32")                                           # this lane's first k of the turn
+        ins(f"shl.b32 {k}, {k8}, 3")
+        ins(f"mad.lo.u32 {k}, {warp}, {32 * U}, {k}")
+        high = None                                            # the tile's second eight rows (N is a multiple of 8)
+        if p.N % 16:
+            high = t("pred")
+            n8 = t("b32")
+            ins(f"add.u32 {n8}, {n0}, 8")
+            ins(f"setp.lt.u32 {high}, {n8}, {p.N}")
+
+        def pointer(row: str, buf: str) -> str:
+            a, o = t("b64"), t("b64")
+            ins(f"mul.wide.u32 {a}, {row}, {p.K * 2}")
+            ins(f"mul.wide.u32 {o}, {k}, 2")
+            ins(f"add.u64 {a}, {a}, {o}")
+            ins(f"add.u64 {a}, {a}, {em.buffer_reg(buf)}")
+            return a
+
+        row = t("b32")
+        ins(f"add.u32 {row}, {n0}, {g}")
+        wp = [pointer(row, p.w.name)]
+        if G == 2:
+            second = t("b64")
+            ins(f"add.u64 {second}, {wp[0]}, {p.N * p.K * 2}")
+            wp.append(second)
+        xp, tokens = [], []
+        for i in range(NT):
+            tok = t("b32")
+            ins(f"add.u32 {tok}, {g}, {8 * i}")
+            xp.append(pointer(tok, p.x.name))
+            ok = None
+            if 8 * (i + 1) > p.M:
+                ok = t("pred")
+                ins(f"setp.lt.u32 {ok}, {tok}, {p.M}")
+            tokens.append(ok)
+        # the elements this thread will finish: column n, tokens tok0, tok0 + 16, ..
+        n, tok0 = t("b32"), t("b32")
+        ins(f"and.b32 {n}, {tid}, 15")
+        ins(f"shr.u32 {tok0}, {tid}, 4")
+        mine = t("b32")
+        ins(f"mov.u32 {mine}, {n}")
+        ins(f"add.u32 {n}, {n}, {n0}")
+        inside = None
+        if p.N % 16:
+            inside = t("pred")
+            ins(f"setp.lt.u32 {inside}, {n}, {p.N}")
+        self.pdl_wait()
+
+        w_regs = [[[em.tmps("b32", 4) for _ in range(2)] for _ in range(G)] for _ in range(U)]
+        x_regs = [[em.tmps("b32", 4) for _ in range(NT)] for _ in range(U)]
+        ragged = p.K % (32 * U * 8) != 0                        # some turn of some warp passes K
+
+        def load(u: int, first: bool) -> None:
+            """Chunk ``u`` of the turn that starts at k (its registers hold nothing that is still needed)."""
+            fits = None
+            if ragged or not first:
+                fits, kk = t("pred"), t("b32")
+                ins(f"add.u32 {kk}, {k}, {32 * u}")
+                ins(f"setp.lt.u32 {fits}, {kk}, {p.K}")
+
+            def both(other):
+                if fits is None or other is None:
+                    return fits or other
+                out = t("pred")
+                ins(f"and.pred {out}, {fits}, {other}")
+                return out
+
+            def one(regs, addr, off, pred, how) -> None:
+                if pred is not None:
+                    for x in regs:
+                        ins(f"mov.u32 {x}, 0")
+                ins(f"{f'@{pred} ' if pred else ''}{how}.v4.b32 {{{', '.join(regs)}}}, [{addr}+{off}]")
+
+            for i in range(G):
+                for h in (0, 1):
+                    one(w_regs[u][i][h], wp[i], 64 * u + h * 8 * p.K * 2, both(high if h else None),
+                        "ld.global.nc.L1::no_allocate.L2::256B")
+            for i in range(NT):
+                one(x_regs[u][i], xp[i], 64 * u, both(tokens[i]), "ld.global.nc")
+
+        for u in range(U):
+            load(u, True)
+        self._columns(n, inside)
+        ahead = []
+        for e in range(-(-p.M // 16)):
+            tok, ok = t("b32"), t("pred")
+            ins(f"add.u32 {tok}, {tok0}, {16 * e}")
+            ins(f"setp.lt.u32 {ok}, {tok}, {p.M}" if inside is None else
+                f"setp.lt.and.u32 {ok}, {tok}, {p.M}, {inside}")
+            ahead.append((tok, ok, self._fetch(tok, n, ok)))
+        acc = [[em.tmps("f32", 4) for _ in range(NT)] for _ in range(G)]
+        for tile in acc:
+            for regs in tile:
+                for x in regs:
+                    ins(f"mov.f32 {x}, {F32.imm(0.0)}")
+        top = lab("ls_turn")
+        place(top)
+        ab = p.x.ty.name
+        turn = 32 * U * 8
+        ins(f"add.u32 {k}, {k}, {turn}")
+        for a in wp + xp:
+            ins(f"add.u64 {a}, {a}, {turn * 2}")
+        for u in range(U):
+            for half in (0, 2):
+                for i in range(G):
+                    lo, hi = w_regs[u][i]
+                    a = f"{{{lo[half]}, {hi[half]}, {lo[half + 1]}, {hi[half + 1]}}}"
+                    for j in range(NT):
+                        x = x_regs[u][j]
+                        c = f"{{{', '.join(acc[i][j])}}}"
+                        ins(f"mma.sync.aligned.m16n8k16.row.col.f32.{ab}.{ab}.f32 {c}, {a}, "
+                            f"{{{x[half]}, {x[half + 1]}}}, {c}")
+            load(u, False)
+        first_k = t("b32")
+        ins(f"and.b32 {first_k}, {k}, -32")                     # the turn's first k, the same in all lanes
+        ins(f"setp.lt.u32 {q}, {first_k}, {p.K}")
+        ins(f"@{q} bra {top}")
+
+        # sums to shared memory: [warp][accumulator][token][16 rows, pitch 20: no two lanes share a bank]
+        base, at = t("b32"), t("b32")
+        ins(f"mov.u32 {base}, smem_pool")
+        ins(f"mad.lo.u32 {at}, {warp}, {G * NT * 8 * 80}, {base}")
+        ins(f"mad.lo.u32 {at}, {k8}, {2 * 80}, {at}")
+        ins(f"mad.lo.u32 {at}, {g}, 4, {at}")
+        for i in range(G):
+            for j in range(NT):
+                for e, x in enumerate(acc[i][j]):
+                    ins(f"st.shared.f32 [{at}+{((i * NT + j) * 8 + e % 2) * 80 + (32 if e > 1 else 0)}], {x}")
+        ins("bar.sync 0")
+        src = t("b32")
+        ins(f"mad.lo.u32 {src}, {tok0}, 80, {base}")
+        ins(f"mad.lo.u32 {src}, {mine}, 4, {src}")
+        for e, (tok, ok, fetched) in enumerate(ahead):
+            sums = []
+            for i in range(G):
+                total = None
+                for wv in range(8):
+                    v = t("f32")
+                    ins(f"mov.f32 {v}, {F32.imm(0.0)}")
+                    ins(f"@{ok} ld.shared.f32 {v}, [{src}+{((wv * G + i) * NT * 8 + 16 * e) * 80}]")
+                    if total is None:
+                        total = v
+                    else:
+                        ins(f"add.rn.f32 {total}, {total}, {v}")
+                bits = t("b32")
+                ins(f"mov.b32 {bits}, {total}")
+                sums.append(bits)
+            self._finish(sums, tok, n, ok, fetched)
+
+
+class StreamPlan:
+    def __init__(self, p: Product):
+        self.G = 2 if p.gated else 1
+        self.NT = -(-p.M // 8)
+        self.U = 8 if self.NT == 1 and self.G == 1 else 4
+        self.ctas = -(-p.N // 16)
+        self.smem = 8 * self.G * self.NT * 8 * 80
+
+    @classmethod
+    def of(cls, p: Product) -> "StreamPlan | None":
+        return cls(p) if p.M <= 32 else None
+
+    def estimate(self, p: Product) -> float:
+        turns = -(-self.ctas // (2 * SM_COUNT)) * p.K * self.G * 0.55e-3
+        return 1.5 + max(p.w.nbytes / 10.5e6, turns) + p.w.nbytes * self.NT * 0.068e-6
+
+
+def choose(p: Product) -> TunedKernel:
+    """The kernel and plan whose estimated time is least.
+
+    The estimates' forms follow what bounds each kernel; their constants are a least-squares fit (of log
+    time) to 1,178 timings on a B200 of every plan at M = 1 .. 2048, (N, K) from 512 x 512 to 8192 x 4096,
+    plain and gated, back to back in graphs.  Over those 154 sizes the choice costs 1.7 % against the best
+    plan on average and 32 % at worst.  Some of both sides, in us (rows / stream / pair): 1 x 512 x 512
+    2.6 / 1.7 / 5.2; 1 x 4096 x 4096 7.2 / 6.5 / 21; 16 x 4096 x 4096 7.6 / 8.4 / 17; 128 x 4096 x 4096
+    12.5 / - / 18.6; 512 x 4096 x 4096 21.8 / - / 20.3; 2048 x 4096 x 4096 - / - / 51."""
+    pair = LinearPair(p)
+    plans = [(pair.estimate(), "pair", lambda: pair)]
+    rows, stream = RowsPlan.best(p), StreamPlan.of(p)
+    if rows is not None:
+        plans.append((rows.estimate(p), "rows", lambda: LinearRows(p, rows)))
+    if stream is not None:
+        plans.append((stream.estimate(p), "stream", lambda: LinearStream(p, stream)))
+    forced = [x for x in plans if x[1] == TUNING.linear_kernel]
+    return min(forced or plans, key=lambda x: x[0])[2]()
 
 
 def recognise(kernel: KernelInfo):
     p = Product.read(kernel)
-    if p is None:
-        return None
-    rows = RowsPlan.best(p)
-    pair = LinearPair(p)
-    if rows is None or TUNING.linear_kernel == "pair":
-        return pair
-    if TUNING.linear_kernel == "rows" or rows.estimate(p) < pair.estimate():
-        return LinearRows(p, rows)
-    return pair
+    return None if p is None else choose(p)

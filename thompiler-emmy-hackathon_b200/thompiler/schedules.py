@@ -177,6 +177,15 @@ def linear_body(M: int, N: int, K: int, ab: str, gated: bool, epilogue, x: str =
 
 # ---- rotary heads ---------------------------------------------------------------------------
 
+def heads_vector(D: int, R: int, nbytes: int) -> int:
+    """Elements of a head (of D, R of them rotating) that the tuned kernel moves at a time: 16 bytes, or
+    the largest power of two that divides the rotating half and the rest's."""
+    V = 16 // nbytes
+    while (R // 2) % V or ((D - R) // 2) % V:
+        V //= 2
+    return V
+
+
 def heads_body(Bn: int, S: int, heads: int, kv: int, D: int, R: int, P: int, dtype: str, interleaved: bool,
                values: bool, heads_first: bool, inverse: bool, eps: float | None):
     """The heads of qkv[B, S, heads + kv (+ kv), D] into q, k (and v): one head of one token per warp.

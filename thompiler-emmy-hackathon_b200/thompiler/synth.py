@@ -273,9 +273,9 @@ def matmul_package(outdir, M: int, N: int, K: int, b_layout: str = "col", out_dt
 
 
 def _layer_write(outdir, pid: str, code: str, entry: str, body, inputs: dict, outputs: dict, grid: int, T: int,
-                 rtol: float, atol: float, smem: int = 0, aligned: tuple = ()) -> Path:
+                 rtol: float, atol: float, smem: int = 0, aligned: dict | None = None) -> Path:
     """A package of one kernel whose args are ``inputs`` then ``outputs`` (name -> (shape, dtype, init or
-    None)), seeded in order; the buffers in ``aligned`` start on 16-byte boundaries."""
+    None)), seeded in order; ``aligned``: the boundary, in bytes, that a buffer must start on."""
     names = list(outputs)
     g = _graph({n: (shape, dt) for n, (shape, dt, _) in inputs.items()}, {}, names[0], outputs[names[0]][0], entry,
                body, dtype=outputs[names[0]][1])
@@ -289,8 +289,8 @@ def _layer_write(outdir, pid: str, code: str, entry: str, body, inputs: dict, ou
             args[-1]["init"] = dict(init, seed=i)
     args += [{"name": n, "dtype": dt, "shape": list(shape), "output": True} for n, (shape, dt, _) in outputs.items()]
     for a in args:
-        if a["name"] in aligned:
-            a["align"] = 16
+        if a["name"] in (aligned or {}):
+            a["align"] = aligned[a["name"]]
     kmeta = {"node": names[0], "arg_order": [a["name"] for a in args], "grid": [grid, 1, 1], "block": [T, 1, 1],
              "smem_bytes": smem, "zero_outputs": [], "args": args}
     return _write(outdir, pid, code, entry, g, kmeta, rtol, atol)
@@ -311,7 +311,7 @@ def linear_package(outdir, M: int, N: int, K: int, dtype: str = "f16", out_dtype
     activation is None, "relu", "silu" or "gelu_tanh".  gated: w[2N, K] and bias[2N] hold two
     projections, and the result is act(first) * second (+ res).  M is any number of rows from one
     on; N and K are multiples of 8 (16-byte rows).  The entry is ``k_linear`` over x, w, (bias,)
-    (res,) linear, buffers that do not overlap; x, w and linear start on 16-byte boundaries."""
+    (res,) linear, buffers that do not overlap and start on 16-byte boundaries."""
     _positive(M=M, N=N, K=K)
     out_dtype = out_dtype or dtype
     if dtype not in ("f16", "bf16") or out_dtype not in (dtype, "f32"):
@@ -338,7 +338,8 @@ def linear_package(outdir, M: int, N: int, K: int, dtype: str = "f16", out_dtype
     tiles = -(-M // 64) * -(-N // 64)
     return _layer_write(outdir, f"synth_linear_{M}x{N}x{K}", code, "k_linear", body, inputs,
                         {"linear": ((M, N), out_dtype, None)}, -(-tiles // 8) * 8, 128, 2e-2, 2e-3,
-                        smem=(3 if gated else 2) * 64 * 64 * 2, aligned=("x", "w", "linear"))
+                        smem=(3 if gated else 2) * 64 * 64 * 2,
+                        aligned=dict.fromkeys((*inputs, "linear"), 16))
 
 
 def _heads_package(outdir, entry: str, Bn: int, S: int, heads: int, kv_heads: int, D: int, rotary: int | None,
@@ -378,8 +379,10 @@ def _heads_package(outdir, entry: str, Bn: int, S: int, heads: int, kv_heads: in
     if -(-threads // 128) >= 2 ** 31:
         raise ValueError(f"{entry}: {Bn * S * n} heads are more than a launch holds")
     tol = (1e-5, 1e-6) if dtype == "f32" else (2e-2, 2e-3)
+    V, nb = schedules.heads_vector(D, R, schedules.TYPES[dtype].nbytes) if D % 2 == 0 else 1, schedules.TYPES[dtype].nbytes
+    aligned = {n: min(16, V * (4 if n in ("cos", "sin") else nb)) for n in (*inputs, *outputs) if n != "pos"}
     return _layer_write(outdir, f"synth_{entry[2:]}_{Bn}x{S}x{n}x{D}", f"{entry[2:]}(qkv, pos, cos, sin)", entry, body,
-                        inputs, outputs, -(-threads // 128), 128, *tol)
+                        inputs, outputs, -(-threads // 128), 128, *tol, aligned=aligned)
 
 
 def rope_package(outdir, B: int, S: int, heads: int, kv_heads: int, D: int, rotary: int | None = None,
@@ -395,7 +398,8 @@ def rope_package(outdir, B: int, S: int, heads: int, kv_heads: int, D: int, rota
     [table, rotary/2] (f32; ``thompiler.rotary.tables`` makes them).  A position outside
     [0, table) -- an empty slot's -1 -- leaves that token's rows of the outputs as they were.
     ``inverse`` rotates by the negative angle: the gradient of the rotation.  The entry is
-    ``k_rope`` over cos, sin, pos, qkv, q, (k, (v))."""
+    ``k_rope`` over cos, sin, pos, qkv, q, (k, (v)); each buffer starts on a multiple of the vectors that
+    the kernel moves (16 bytes, less where the sizes leave less: ``align`` in meta.json)."""
     return _heads_package(outdir, "k_rope", B, S, heads, kv_heads, D, rotary, interleaved, dtype, table, values,
                           heads_first, inverse, None)
 
