@@ -165,11 +165,26 @@ int thr_tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const
                   const uint64_t *args, int nargs, uint64_t stream, int *set);
 int thr_tmap_launched(uint64_t module, int set, uint64_t stream);
 
-/* thr_tmap_bind, thr_launch_ex and thr_tmap_launched in one call (a launch that fails reports no
- * reader): what a caller on device pointers makes for every launch of a kernel with tensor maps. */
-int thr_launch_tmaps(uint64_t module, uint64_t function, const uint32_t grid[3], const uint32_t block[3],
-                     uint32_t smem_bytes, const thr_tmap_spec *tmaps, int ntmaps, const char *ptr_table,
-                     const uint64_t *args, int nargs, uint64_t stream, uint32_t flags);
+/* Everything of a launch on device pointers that stays the same from call to call: filled in once,
+ * read by each thr_launch_prepared. */
+typedef struct {
+    uint64_t module;                /* of `function` (for tensor maps; 0 without maps) */
+    uint64_t function;
+    uint32_t grid[3];
+    uint32_t block[3];
+    uint32_t smem_bytes;
+    uint32_t flags;                 /* as thr_launch_ex */
+    int32_t nargs;
+    int32_t ntmaps;
+    const uint32_t *align;          /* per argument: the power of two its address must be a multiple of, 0 for any
+                                       (NULL: any for all) */
+    const thr_tmap_spec *tmaps;
+    const char *ptr_table;
+} thr_launch_desc;
+
+/* One launch of `desc` on args[nargs]: addresses checked against `align` (THR_ERR_REQUEST before
+ * anything is issued), tensor maps bound, launched and their reader reported in one call. */
+int thr_launch_prepared(const thr_launch_desc *desc, const uint64_t *args, uint64_t stream);
 
 /* A 2-D..5-D tiled TMA descriptor (CUtensorMap, 128 bytes) for `base`.
  * dtype_code: 0 = f16, 1 = bf16, 2 = f32; swizzle: 0 none, 1 = 32B,

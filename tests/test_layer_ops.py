@@ -110,6 +110,30 @@ def test_heads_assemble(tmp_path, case, tuned):
     _ptxas(compile_kernel(load.load(str(_ir(d))), tuned=tuned), tmp_path)
 
 
+def test_misaligned_buffer_is_refused_by_name(tmp_path):
+    """The check precedes everything of the launch, so it answers without a GPU."""
+    from types import SimpleNamespace
+
+    from thompiler import runner
+    if not runner.LIB_PATH.exists():
+        pytest.skip("runner library not built")
+    for d in (synth.linear_package(tmp_path / "l", 4, 64, 64, bias=True, residual=True),
+              synth.qk_norm_rope_package(tmp_path / "h", 1, 4, 4, 2, 128, values=True),
+              synth.rope_package(tmp_path / "r", 1, 4, 4, 2, 80, rotary=40)):
+        import json
+        kmeta = json.loads((d / "meta.json").read_text())["kernels"][0]
+        k = runner.Launch(SimpleNamespace(handle=1, name=kmeta["entry"], module=SimpleNamespace(handle=0)),
+                          SimpleNamespace(grid=(1, 1, 1), block=(128, 1, 1), smem=0, pdl=True), kmeta, None)
+        want = {a["name"]: a["align"] for a in kmeta["args"] if "align" in a}
+        assert set(want) == set(kmeta["arg_order"]) - {"pos"}
+        good = {n: 4096 * (i + 1) for i, n in enumerate(kmeta["arg_order"])}
+        for name, align in want.items():
+            with pytest.raises(runner.RunnerError, match=f"buffer '{name}' .* not {align}-byte aligned") as e:
+                k(dict(good, **{name: good[name] + align // 2}))
+            assert e.value.stage == "request"
+    assert min(want.values()) == 8                        # the last one moves four f16 elements at a time
+
+
 # ---- storage types -----------------------------------------------------------------------
 
 def test_bf16_bits_round_to_nearest_even():

@@ -470,6 +470,32 @@ int wait_event(cudaEvent_t ev, double timeout_s) {
 
 }  // namespace
 
+namespace {
+
+// Functions whose dynamic shared memory limit was raised, and to what: the attribute is set once, not
+// before every launch.  Forgotten whenever a module is loaded or unloaded (a later function may have the
+// handle of an earlier one, after a cudaDeviceReset too).
+std::map<uint64_t, uint32_t> g_smem_limit;
+std::mutex g_smem_mu;
+
+void forget_smem_limits() {
+    std::lock_guard<std::mutex> lk(g_smem_mu);
+    g_smem_limit.clear();
+}
+
+int raise_smem_limit(uint64_t function, uint32_t bytes) {
+    std::lock_guard<std::mutex> lk(g_smem_mu);
+    uint32_t &have = g_smem_limit[function];
+    if (have >= bytes) return THR_OK;
+    CUresult r = g_drv.func_set((CUfunction)(uintptr_t)function, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES,
+                                (int)bytes);
+    if (r != CUDA_SUCCESS) return drv_fail(r, "raising the dynamic shared memory limit");
+    have = bytes;
+    return THR_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 int thr_version(void) { return 2; }
@@ -516,6 +542,7 @@ int thr_module_load(const char *ptx, uint64_t *module, char *log, size_t log_len
     }
     if (r != CUDA_SUCCESS)
         return fail(THR_ERR_PTXAS, "PTX JIT failed (%s): %s", cu_name(r), error.data());
+    forget_smem_limits();
     *module = (uint64_t)(uintptr_t)m;
     return THR_OK;
 }
@@ -524,6 +551,7 @@ int thr_module_unload(uint64_t module) {
     int s = ensure_driver();
     if (s) return s;
     drop_ring(module);
+    forget_smem_limits();
     CUresult r = g_drv.unload((CUmodule)(uintptr_t)module);
     return r == CUDA_SUCCESS ? THR_OK : drv_fail(r, "cuModuleUnload");
 }
@@ -574,10 +602,7 @@ int thr_launch_ex(uint64_t function, const uint32_t grid[3], const uint32_t bloc
     if (!grid || !block || nargs < 0 || (nargs > 0 && !args) || (flags & ~THR_LAUNCH_OVERLAP_PREVIOUS))
         return fail(THR_ERR_REQUEST, "thr_launch: bad arguments");
     CUfunction f = (CUfunction)(uintptr_t)function;
-    if (smem_bytes > 48 * 1024) {
-        CUresult r = g_drv.func_set(f, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)smem_bytes);
-        if (r != CUDA_SUCCESS) return drv_fail(r, "raising the dynamic shared memory limit");
-    }
+    if (smem_bytes > 48 * 1024 && (s = raise_smem_limit(function, smem_bytes))) return s;
     // the driver reads each parameter through a pointer to it, during the call
     void *few[16];
     std::vector<void *> many;
@@ -776,13 +801,20 @@ int thr_tmap_launched(uint64_t module, int set, uint64_t stream) {
     return tmap_launched(module, set, (cudaStream_t)(uintptr_t)stream);
 }
 
-int thr_launch_tmaps(uint64_t module, uint64_t function, const uint32_t grid[3], const uint32_t block[3],
-                     uint32_t smem_bytes, const thr_tmap_spec *tmaps, int ntmaps, const char *ptr_table,
-                     const uint64_t *args, int nargs, uint64_t stream, uint32_t flags) {
-    int set = -1;
-    int s = thr_tmap_bind(module, tmaps, ntmaps, ptr_table, args, nargs, stream, &set);
-    if (!s) s = thr_launch_ex(function, grid, block, smem_bytes, args, nargs, stream, flags);
-    return s ? s : thr_tmap_launched(module, set, stream);
+int thr_launch_prepared(const thr_launch_desc *d, const uint64_t *args, uint64_t stream) {
+    if (!d || (d->nargs > 0 && !args)) return fail(THR_ERR_REQUEST, "thr_launch_prepared: bad arguments");
+    if (d->align)
+        for (int i = 0; i < d->nargs; ++i)
+            if (d->align[i] > 1 && (args[i] & (d->align[i] - 1)))
+                return fail(THR_ERR_REQUEST, "argument %d at 0x%llx is not %u-byte aligned", i,
+                            (unsigned long long)args[i], d->align[i]);
+    int set = -1, s = THR_OK;
+    if (d->ntmaps > 0 &&
+        (s = thr_tmap_bind(d->module, d->tmaps, d->ntmaps, d->ptr_table, args, d->nargs, stream, &set)))
+        return s;
+    s = thr_launch_ex(d->function, d->grid, d->block, d->smem_bytes, args, d->nargs, stream, d->flags);
+    if (!s && d->ntmaps > 0) s = thr_tmap_launched(d->module, set, stream);
+    return s;
 }
 
 int thr_tensor_map(void *out128, int dtype_code, int rank, uint64_t base, const uint64_t *dims,

@@ -19,7 +19,9 @@ There is no fallback: without the built library every call raises.
 from __future__ import annotations
 
 import ctypes
+import operator
 import re
+import struct
 from dataclasses import dataclass, field
 from pathlib import Path
 
@@ -55,6 +57,13 @@ class ThrRunDesc(ctypes.Structure):
                 ("block", ctypes.c_uint32 * 3), ("smem_bytes", ctypes.c_uint32), ("nargs", ctypes.c_int32),
                 ("args", ctypes.POINTER(ThrArg)), ("tmaps", ctypes.POINTER(ThrTmapSpec)), ("ntmaps", ctypes.c_int32),
                 ("ptr_table", ctypes.c_char_p)]
+
+
+class ThrLaunchDesc(ctypes.Structure):
+    _fields_ = [("module", ctypes.c_uint64), ("function", ctypes.c_uint64), ("grid", ctypes.c_uint32 * 3),
+                ("block", ctypes.c_uint32 * 3), ("smem_bytes", ctypes.c_uint32), ("flags", ctypes.c_uint32),
+                ("nargs", ctypes.c_int32), ("ntmaps", ctypes.c_int32), ("align", ctypes.POINTER(ctypes.c_uint32)),
+                ("tmaps", ctypes.POINTER(ThrTmapSpec)), ("ptr_table", ctypes.c_char_p)]
 
 
 _lib = None
@@ -97,8 +106,7 @@ def library() -> ctypes.CDLL:
             "thr_tmap_bind": ([u64, ctypes.POINTER(ThrTmapSpec), i32, ctypes.c_char_p, ctypes.POINTER(u64), i32,
                                u64, ctypes.POINTER(i32)], i32),
             "thr_tmap_launched": ([u64, i32, u64], i32),
-            "thr_launch_tmaps": ([u64, u64, u32x3, u32x3, ctypes.c_uint32, ctypes.POINTER(ThrTmapSpec), i32,
-                                  ctypes.c_char_p, ctypes.POINTER(u64), i32, u64, ctypes.c_uint32], i32),
+            "thr_launch_prepared": ([p, ctypes.c_char_p, u64], i32),
             "thr_peer_alloc": ([u64, ctypes.POINTER(u64), ctypes.c_char_p], i32),
             "thr_peer_open": ([ctypes.c_char_p, ctypes.POINTER(u64)], i32),
             "thr_peer_close": ([u64], i32),
@@ -300,42 +308,43 @@ class TensorMaps:
 
 
 class Launch:
-    """One kernel's launches on device pointers, with everything that stays the same from call to call
-    converted once: ``launch(ptrs, stream)`` is one C call (with its tensor maps' binding, when the
-    plan has any).  ``plan``'s grid, block and shared memory are read again whenever they are
-    replaced; a buffer that meta.json wants aligned is refused when it is not."""
+    """One kernel's launches on device pointers.  What stays the same from call to call is a C record made
+    once, so ``launch(ptrs, stream)`` packs the pointers and makes one C call (with its tensor maps'
+    binding, when the plan has any).  ``plan``'s grid, block and shared memory are read again whenever
+    they are replaced; a buffer that meta.json wants aligned is refused when it is not."""
 
     def __init__(self, function: Function, plan: LaunchPlan, kmeta: dict, tmaps: TensorMaps | None):
         self.function, self.plan, self.order, self.tmaps = function, plan, tuple(kmeta["arg_order"]), tmaps
-        align = {a["name"]: a.get("align", 1) for a in kmeta["args"]}
-        self.aligned = [(i, align[n]) for i, n in enumerate(self.order) if align.get(n, 1) > 1]
-        self.n = len(self.order)
-        self._array = ctypes.c_uint64 * max(1, self.n)
-        lib = library()
-        self._plain, self._mapped = lib.thr_launch_ex, lib.thr_launch_tmaps
-        self._geometry = None
+        n = len(self.order)
+        self._get = operator.itemgetter(*self.order) if n > 1 else lambda ptrs: tuple(ptrs[x] for x in self.order)
+        self._pack = struct.Struct(f"@{max(1, n)}Q").pack if n else lambda: bytes(8)
+        align = {a["name"]: a.get("align", 0) for a in kmeta["args"]}
+        self._align = (ctypes.c_uint32 * max(1, n))(*[align.get(x, 0) for x in self.order])
+        self._call = library().thr_launch_prepared
+        self._geometry, self._descs = None, []
+
+    def _prepare(self) -> None:
+        plan, t = self.plan, self.tmaps
+        d = ThrLaunchDesc(self.function.module.handle if t else 0, self.function.handle, _dims(plan.grid),
+                          _dims(plan.block), int(plan.smem), OVERLAP_PREVIOUS if plan.pdl else 0, len(self.order))
+        d.align = self._align
+        if t is not None:
+            d.tmaps, d.ntmaps, d.ptr_table = t.specs, t.n, t.table
+        self._descs.append(d)                 # kept: a call in another thread may still be reading the last one
+        self._at = ctypes.addressof(d)
+        self._geometry = (plan.grid, plan.block, plan.smem)
 
     def __call__(self, ptrs: dict[str, int], stream: int = 0) -> None:
-        plan, f = self.plan, self.function
-        geometry = (plan.grid, plan.block, plan.smem)
-        if geometry != self._geometry:
-            self._dims = (_dims(plan.grid), _dims(plan.block), int(plan.smem), OVERLAP_PREVIOUS if plan.pdl else 0)
-            self._geometry = geometry
-        grid, block, smem, flags = self._dims
-        vals = [ptrs[n] for n in self.order]
-        for i, align in self.aligned:
-            if vals[i] % align:
-                raise RunnerError("request", f"{f.name}: buffer {self.order[i]!r} at {vals[i]:#x} is not "
-                                             f"{align}-byte aligned")
-        args = self._array(*vals)
-        if self.tmaps is None:
-            st = self._plain(f.handle, grid, block, smem, args, self.n, stream, flags)
-        else:
-            t = self.tmaps
-            st = self._mapped(t.module.handle, f.handle, grid, block, smem, t.specs, t.n, t.table, args, self.n,
-                              stream, flags)
+        plan = self.plan
+        if (plan.grid, plan.block, plan.smem) != self._geometry:
+            self._prepare()
+        st = self._call(self._at, self._pack(*self._get(ptrs)), stream)
         if st:
-            check(st, f"launch of {f.name}")
+            why = last_error()
+            m = re.match(r"argument (\d+) at", why)
+            if m:
+                why = f"buffer {self.order[int(m[1])]!r}" + why[m.end() - 3:]
+            raise RunnerError(STAGES.get(st, "cuda"), f"launch of {self.function.name}: {why}")
 
 
 def read_error_word(module: Module, plan: LaunchPlan) -> int:
