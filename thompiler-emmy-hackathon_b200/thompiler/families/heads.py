@@ -297,6 +297,9 @@ class RotaryHeads(TunedKernel):
 
         # from here on the warp reads and writes global data
         self.pdl_wait()
+        pos, pa, inside = t("b32"), t("b64"), t("pred")               # the position; does the unit store at all?
+        ins(f"mad.wide.u32 {pa}, {token}, 4, {em.buffer_reg('pos')}")
+        ins(f"ld.global.nc.u32 {pos}, [{pa}]")
         raw, live = [], []
         for r in range(self.rounds):
             ok = t("pred")
@@ -331,10 +334,6 @@ class RotaryHeads(TunedKernel):
             raw.append(raws)
             live.append(lives)
 
-        # the position, and whether the unit stores at all
-        pos, pa, inside = t("b32"), t("b64"), t("pred")
-        ins(f"mad.wide.u32 {pa}, {token}, 4, {em.buffer_reg('pos')}")
-        ins(f"ld.global.nc.u32 {pos}, [{pa}]")
         ins(f"setp.lt.u32 {inside}, {pos}, {self.P}")                  # unsigned: negative positions lie past the table
 
         def store(r: int, i: int, packed) -> None:
@@ -358,10 +357,9 @@ class RotaryHeads(TunedKernel):
             ins(f"bra {self.exit}")
             em.place(turned)
 
-        # the coefficients of this lane's items, packed two elements a register: with the weights folded in,
-        # y_a = n_a (w_a c) - n_b (w_b s) and y_b = n_b (w_b c) + n_a (w_a s), n = x rstd.  An item past the
-        # rotated part has c = 1 and stops at its first product
-        coef = []
+        # the tables' entries and the weights of this lane's items, on their way while the norms are taken.  An
+        # item past the rotated part has c = 1, s = 0
+        tables, weights = [], []
         for i in range(self.items):
             q = inside
             for extra in (have[i], turns[i]):
@@ -384,22 +382,29 @@ class RotaryHeads(TunedKernel):
                     vec, body = (f".v{step}", f"{{{', '.join(g)}}}") if step > 1 else ("", g[0])
                     ins(f"@{q} ld.global.nc{vec}.f32 {body}, [{a}{f'+{4 * c}' if c else ''}]")
                 tab.append(regs)
-            cos, sin = tab
-            if self.eps is None:
-                ca = cb = cos
-                sa = sb = sin
-            else:
-                pair = []
-                for off in (off0[i], off1[i]):
-                    a, w = t("b64"), t("b64")
-                    ins(f"cvt.u64.u32 {w}, {off}")
-                    ins(f"add.u64 {a}, {wbase}, {w}")
-                    regs = em.tmps("b32", self._raw())
-                    for x in regs:
-                        ins(f"mov.u32 {x}, 0")
-                    self._vector("ld.global.nc", regs, a, f"@{have[i]} " if have[i] else "")
-                    pair.append(self._unpack(regs))
-                wa, wb = self._pairs_of(*pair)
+            tables.append(tab)
+            pair = []
+            for off in (off0[i], off1[i]) if self.eps is not None else ():
+                a, w = t("b64"), t("b64")
+                ins(f"cvt.u64.u32 {w}, {off}")
+                ins(f"add.u64 {a}, {wbase}, {w}")
+                regs = em.tmps("b32", self._raw())
+                for x in regs:
+                    ins(f"mov.u32 {x}, 0")
+                self._vector("ld.global.nc", regs, a, f"@{have[i]} " if have[i] else "")
+                pair.append(regs)
+            weights.append(pair)
+
+        rstd = [self._rstd(raw[r]) for r in range(self.rounds)] if self.eps is not None else []
+
+        # the coefficients, packed two elements a register: with the weights folded in,
+        # y_a = n_a (w_a c) - n_b (w_b s) and y_b = n_b (w_b c) + n_a (w_a s), n = x rstd
+        coef = []
+        for (cos, sin), pair in zip(tables, weights):
+            ca = cb = cos
+            sa = sb = sin
+            if pair:
+                wa, wb = self._pairs_of(*(self._unpack(x) for x in pair))
                 ca, sa, cb, sb = ([self._f("mul.rn.f32", x, y) for x, y in zip(ws, tb)]
                                   for ws, tb in ((wa, cos), (wa, sin), (wb, cos), (wb, sin)))
             # the subtracted product's sine enters negated (the other one's for the inverse rotation)
@@ -410,52 +415,56 @@ class RotaryHeads(TunedKernel):
             coef.append([self._twos(x) for x in (ca, sa, cb, sb)])
 
         for r in range(self.rounds):
-            vals = [[self._twos(h) for h in self._pairs_of(*(self._unpack(x) for x in raw[r][i]))]
-                    for i in range(self.items)]
-            if self.eps is not None:
-                acc = t("b64")
-                ins(f"mov.b64 {acc}, 0")
-                for pair in vals:
-                    for x in pair[0] + pair[1]:
-                        ins(f"fma.rn.f32x2 {acc}, {x}, {x}, {acc}")
-                lo, hi, rstd = t("f32"), t("f32"), t("f32")
-                ins(f"mov.b64 {{{lo}, {hi}}}, {acc}")
-                if V > 1:
-                    ins(f"add.rn.f32 {rstd}, {lo}, {hi}")
-                else:                                          # one element a register, doubled
-                    ins(f"mov.f32 {rstd}, {lo}")
-                step = self.lanes // 2
-                while step:
-                    o = t("f32")
-                    ins(f"shfl.sync.bfly.b32 {o}, {rstd}, {step}, 0x1f, 0xffffffff")
-                    ins(f"add.rn.f32 {rstd}, {rstd}, {o}")
-                    step //= 2
-                ins(f"mul.rn.f32 {rstd}, {rstd}, {F32.imm(1.0 / D)}")
-                ins(f"add.rn.f32 {rstd}, {rstd}, {F32.imm(float(self.eps))}")
-                ins(f"rsqrt.approx.f32 {rstd}, {rstd}")        # relative error at most 2^-22.9
-                rr = t("b64")
-                ins(f"mov.b64 {rr}, {{{rstd}, {rstd}}}")
-                for pair in vals:
-                    for half in pair:
-                        for m, x in enumerate(half):
-                            half[m] = t("b64")
-                            ins(f"mul.rn.f32x2 {half[m]}, {x}, {rr}")
-            for i, (na, nb_) in enumerate(vals):
+            for i in range(self.items):
+                na, nb_ = (self._twos(h) for h in self._pairs_of(*(self._unpack(x) for x in raw[r][i])))
                 out_a, out_b = [], []
                 for m, (a, b) in enumerate(zip(na, nb_)):
+                    if rstd:
+                        for x in (a, b):
+                            ins(f"mul.rn.f32x2 {x}, {x}, {rstd[r]}")
                     ca, sa, cb, sb = (c[m] for c in coef[i])
                     pa_, pb_, ya, yb = t("b64"), t("b64"), t("b64"), t("b64")
                     ins(f"mul.rn.f32x2 {pa_}, {a}, {ca}")
                     ins(f"mul.rn.f32x2 {pb_}, {b}, {cb}")
                     ins(f"fma.rn.f32x2 {ya}, {b}, {sb}, {pa_}")
                     ins(f"fma.rn.f32x2 {yb}, {a}, {sa}, {pb_}")
-                    if turns[i]:
+                    if turns[i]:                               # an item past the rotated part keeps its product
                         ins(f"selp.b64 {ya}, {ya}, {pa_}, {turns[i]}")
                         ins(f"selp.b64 {yb}, {yb}, {pb_}, {turns[i]}")
                     out_a.append(ya)
                     out_b.append(yb)
                 v0, v1 = self._vectors_of(self._ones(out_a), self._ones(out_b))
                 store(r, i, (self._pack(v0), self._pack(v1)))
+
+    def _rstd(self, items: list) -> str:
+        """rsqrt(mean(x^2) + eps) of the lane's head, twice in a 64-bit register: the squares of the lane's
+        elements in two chains, then an xor butterfly among the head's lanes."""
+        em, t, ins = self.em, self.em.tmp, self.em.ins
+        sums = [t("b64"), t("b64")]
+        for acc in sums:
+            ins(f"mov.b64 {acc}, 0")
+        for item in items:
+            for acc, regs in zip(sums, item):
+                for x in self._twos(self._unpack(regs)):
+                    ins(f"fma.rn.f32x2 {acc}, {x}, {x}, {acc}")
+        ins(f"add.rn.f32x2 {sums[0]}, {sums[0]}, {sums[1]}")
+        lo, hi, rstd, rr = t("f32"), t("f32"), t("f32"), t("b64")
+        ins(f"mov.b64 {{{lo}, {hi}}}, {sums[0]}")
+        if self.V > 1:
+            ins(f"add.rn.f32 {rstd}, {lo}, {hi}")
+        else:                                                  # one element a register, doubled
+            ins(f"mov.f32 {rstd}, {lo}")
+        step = self.lanes // 2
+        while step:
+            o = t("f32")
+            ins(f"shfl.sync.bfly.b32 {o}, {rstd}, {step}, 0x1f, 0xffffffff")
+            ins(f"add.rn.f32 {rstd}, {rstd}, {o}")
+            step //= 2
+        ins(f"mul.rn.f32 {rstd}, {rstd}, {F32.imm(1.0 / self.D)}")
+        ins(f"add.rn.f32 {rstd}, {rstd}, {F32.imm(float(self.eps))}")
+        ins(f"rsqrt.approx.f32 {rstd}, {rstd}")                # relative error at most 2^-22.9
+        ins(f"mov.b64 {rr}, {{{rstd}, {rstd}}}")
+        return rr
 
     def _f(self, op: str, *args: str) -> str:
         r = self.em.tmp("f32")
