@@ -67,7 +67,8 @@ class RotaryHeads(TunedKernel):
         """Two rounds a unit while that leaves a warp for every scheduler, else one.  Measured at 32768 x 80
         heads of 128 bf16 with norm: one round 292 us (the coefficients' loads and the launch of twice
         the CTAs), two 225, four 239; at 3 x 1021 x 20 heads of 80: 8.7, 5.8, 6.2.  CTAs of 64, 128 and 256
-        threads: 224, 225, 246 us."""
+        threads: 224, 225, 246 us.  A loop over further rounds in the same warp, the next one's rows loaded
+        ahead, takes 249 us at its best: what it saves in table loads it loses in warps."""
         units = self.T * sum(-(-h // (2 * self.per_round)) for *_, h in self.segments)
         return 2 if self.items == 1 and units >= 4 * SM_COUNT else 1
 
@@ -122,6 +123,11 @@ class RotaryHeads(TunedKernel):
 
     def guard(self, generic: str) -> None:
         em = self.em
+        if self.eps is None and self.items == 1 and self.V <= 4:
+            # room for 48 registers: left alone, the assembler keeps 32 by issuing the loads late (2 x 1777 x 16
+            # heads of 96 f32: 8.6 us against 8.0).  Vectors of eight and the norm find theirs by themselves (the
+            # norm's 72 capped at 64: 230 us against 225)
+            em.entry_attrs += [f".maxntid {self.threads}, 1, 1", ".minnctapersm 10"]
         p = em.tmp("pred")
         em.ins(f"setp.ne.u32 {p}, {self.special('%ntid.x')}, {self.threads}")
         em.ins(f"@{p} bra {generic}")
