@@ -159,3 +159,38 @@ def heads_package(synth, path, spec, table):
     return build(path, spec["B"], spec["S"], spec["heads"], spec["kv"], spec["D"], rotary=spec["R"],
                  interleaved=spec["interleaved"], dtype=spec["dtype"], table=table, values=spec["values"],
                  heads_first=spec["heads_first"], **more)
+
+
+def custom_epilogue_package(path, M, N, K):
+    """linear[M, N] = row <= col ? max(scale[0] * z + shift[col], cap[row, col]) : -1, with f32 scale, shift and
+    cap: an epilogue that no builder writes, of a constant load, a vector over columns, an array over
+    elements and a selection by coordinates."""
+    from thompiler import ir, schedules, synth
+    L, V, B, assign = schedules.L, schedules.V, schedules.B, schedules.assign
+    row = schedules.clamped(V("row"), M) if M % 64 else V("row")
+    col = schedules.clamped(V("col"), N) if N % 64 else V("col")
+    f32 = schedules.F32T
+    epi = ir.Lambda(("z", "row", "col"), (
+        ir.Load(("sc",), "scale", (L(0),), f32), ir.Load(("sh",), "shift", (col,), f32),
+        ir.Load(("cp",), "cap", (row, col), f32), ir.Let("minus", L(-1.0, "float"), f32),
+        assign("zs", "multiply", "z", "sc"), assign("zt", "add", "zs", "sh"), assign("zm", "maximum", "zt", "cp"),
+        ir.Select("y", (ir.Branch(V("zm"), B("<=", V("row"), V("col"))), ir.Branch(V("minus"), None)))), ("y",))
+    body = schedules.linear_body(M, N, K, "f16", False, epi)
+    tiles = -(-M // 64) * -(-N // 64)
+    inputs = {"x": ((M, K), "f16", None), "w": ((N, K), "f16", {"dist": "normal", "std": K ** -0.5}),
+              "scale": ((1,), "f32", None), "shift": ((N,), "f32", None), "cap": ((M, N), "f32", None)}
+    return synth._layer_write(path, "custom", "custom", "k_linear", body, inputs, {"linear": ((M, N), "f32", None)},
+                              -(-tiles // 8) * 8, 128, 2e-2, 2e-3, smem=2 * 64 * 64 * 2,
+                              aligned=dict.fromkeys((*inputs, "linear"), 16))
+
+
+def custom_expected(x):
+    z = x["x"].astype(np.float64) @ x["w"].astype(np.float64).T
+    mag = np.abs(x["x"].astype(np.float64)) @ np.abs(x["w"].astype(np.float64)).T
+    s = float(x["scale"].reshape(-1)[0])
+    t = s * z + x["shift"].astype(np.float64)
+    # the product's steps (as in linear_expected), then a product and a sum in f32
+    err = abs(s) * (x["x"].shape[1] / 16 + 8) * 2.0 ** -22 * mag + 2.0 ** -23 * (np.abs(s * z) + np.abs(t))
+    rows, cols = np.indices(t.shape)
+    keep = rows <= cols
+    return np.where(keep, np.maximum(t, x["cap"]), -1.0), np.where(keep, err + 2.0 ** -24 * np.abs(t), 0.0)

@@ -5,7 +5,8 @@ whose other contents must not change; rows of empty slots keep what they held.""
 import numpy as np
 import pytest
 
-from layer_cases import HEADS, LINEAR, check, heads_expected, heads_package, heads_spec, linear_expected
+from layer_cases import (HEADS, LINEAR, check, custom_epilogue_package, custom_expected, heads_expected, heads_package,
+                         heads_spec, linear_expected)
 from thompiler import synth
 from thompiler.device import DeviceKernel
 from thompiler.families.tuning import TUNING
@@ -91,6 +92,30 @@ def test_linear(tmp_path, monkeypatch, case, launch):
     k(ptrs, _stream())                                    # the same bits again
     torch.cuda.synchronize()
     assert torch.equal(first, y)
+    k.close()
+
+
+@pytest.mark.parametrize("kernel", ["generic", "stream", "rows", "pair"])
+@pytest.mark.parametrize("M,N,K", [(20, 200, 264), (32, 64, 64), (600, 328, 200)])
+def test_custom_epilogue(tmp_path, monkeypatch, kernel, M, N, K):
+    """Epilogues of other statements, buffers and types than the builder's are replayed by every kernel."""
+    import torch
+    from thompiler import problems
+    if kernel != "generic":
+        monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    d = custom_epilogue_package(tmp_path, M, N, K)
+    k = _kernel(d, "generic" if kernel == "generic" else "own")
+    if kernel not in k.family:
+        pytest.skip(f"no {kernel} plan for this size")
+    x = problems.make_inputs(problems.load_package(d))
+    t = {n: torch.from_numpy(v).cuda() for n, v in x.items()}
+    whole, y = _out((M, N), "f32")
+    k({n: v.data_ptr() for n, v in dict(t, linear=y).items()}, _stream())
+    torch.cuda.synchronize()
+    assert k.error_word() == 0
+    _untouched(whole)
+    want, allowed = custom_expected(x)
+    check(_np(y), want, allowed, k.family)
     k.close()
 
 

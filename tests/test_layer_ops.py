@@ -10,7 +10,8 @@ import subprocess
 import numpy as np
 import pytest
 
-from layer_cases import HEADS, LINEAR, check, heads_expected, heads_package, heads_spec, linear_expected
+from layer_cases import (HEADS, LINEAR, check, custom_epilogue_package, custom_expected, heads_expected, heads_package,
+                         heads_spec, linear_expected)
 from oracle.interp import run_package as oracle_run
 from thompiler import ir, load, problems, rotary, synth
 from thompiler.compiler import compile_kernel
@@ -43,6 +44,13 @@ def test_heads_tree_is_the_definition(tmp_path, case):
     assert set(got) == set(want)
     for name, (w, allowed) in want.items():
         check(got[name], w, allowed, name)
+
+
+def test_custom_epilogue_tree(tmp_path):
+    d = custom_epilogue_package(tmp_path, 40, 72, 136)
+    x = problems.make_inputs(problems.load_package(d))
+    want, allowed = custom_expected(x)
+    check(oracle_run(d)["linear"], want, allowed, "linear")
 
 
 def test_tree_survives_the_reader(tmp_path):
@@ -132,6 +140,34 @@ def test_misaligned_buffer_is_refused_by_name(tmp_path):
                 k(dict(good, **{name: good[name] + align // 2}))
             assert e.value.stage == "request"
     assert min(want.values()) == 8                        # the last one moves four f16 elements at a time
+
+
+@pytest.mark.parametrize("kernel", ["stream", "rows", "pair", "heads"])
+def test_waits_for_the_previous_kernel(tmp_path, monkeypatch, kernel):
+    """Launches may overlap the previous kernel's end: no access to global data, and in the kernel whose CTAs
+    share SMs with others' no tensor memory taken, before the wait for it; the next kernel may come
+    only after that memory is taken."""
+    from test_pdl_order import GLOBAL, HOST_TABLES, _body
+    from thompiler.emitter import read_sidecar
+    from thompiler.families.tuning import TUNING
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    d = (synth.qk_norm_rope_package(tmp_path, 2, 64, 4, 2, 128, values=True) if kernel == "heads" else
+         synth.linear_package(tmp_path, 16, 512, 512, bias=True, residual=True))
+    ptx = compile_kernel(load.load(str(_ir(d))))
+    assert kernel in (read_sidecar(ptx) or {})["family"] and read_sidecar(ptx)["pdl"] is True
+    lines = [ln.strip() for ln in _body(ptx)]
+    generic = next(i for i, ln in enumerate(lines) if "generic lowering of the same IR" in ln)
+    assert next(ln for ln in lines[generic + 1:] if ln and not ln.startswith("//")) == "griddepcontrol.wait;"
+    lines = lines[:generic]
+    at = lambda text: [i for i, ln in enumerate(lines) if text in ln]        # noqa: E731
+    waits, first = at("griddepcontrol.wait"), at("griddepcontrol.wait")[0]
+    for ln in lines[:first]:
+        assert not GLOBAL.match(ln) or any(x in ln for x in HOST_TABLES) or "atom.global.or.b32" in ln, ln
+    if kernel == "rows":
+        (alloc,), (trigger,) = at("tcgen05.alloc"), at("griddepcontrol.launch_dependents")
+        assert len(waits) == 2 and waits[0] < alloc < trigger
+        assert not any("$L_" in ln and ln.endswith(":") for ln in lines[waits[-1]:alloc])     # one straight piece
+        assert waits[-1] < alloc
 
 
 # ---- storage types -----------------------------------------------------------------------

@@ -484,7 +484,7 @@ class LinearRows(ByElement):
     Eight warps copy both operands with 16-byte cp.async into the 128-byte swizzle -- no tensor maps, so
     nothing is kept for a buffer's address, and any number of weights share the kernel in captured
     graphs -- each thread's copies of a stage arriving on its mbarrier as they land; a ninth warp
-    allocates the tensor memory (after the first loads are on their way), waits, fences the proxies
+    allocates the tensor memory (while the first loads are on their way), waits, fences the proxies
     and issues the MMAs.  Out-of-range rows and K are zero-filled by the copies.  Every wait is bounded."""
 
     family = "tcgen05-linear-rows"
@@ -668,12 +668,14 @@ class LinearRows(ByElement):
 
         # ---------------- MMA issuer (warp 8) ----------------
         place(role_mma)
+        # tensor memory only once the previous kernel is done: its CTAs may share the SM and may still have to
+        # allocate theirs, and this grid would keep it until that kernel ends
+        self.pdl_wait()
         slot, tmem = t("b32"), t("b32")
         ins(f"add.u32 {slot}, {bars}, {slot_off}")
         ins(f"tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [{slot}], {pl.tmem_cols}")
         ins("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned")
-        # the next kernel's CTAs may share the SM from here on, not before: one that took the tensor memory
-        # this CTA still had to allocate would keep it until this grid ends
+        # for the same reason the next kernel's CTAs may come from here on, not before
         self.pdl_trigger()
         ins("bar.warp.sync -1")
         ins(f"ld.shared.u32 {tmem}, [{slot}]")
