@@ -271,6 +271,80 @@ def test_a_layer(tmp_path, dtype):
         k.close()
 
 
+@pytest.mark.parametrize("kernel,M,N", [("stream", 5, 512), ("stream", 16, 1024), ("rows", 5, 512), ("rows", 200, 512),
+                                        ("pair", 300, 512)])
+def test_chain_reads_what_the_launch_before_wrote(tmp_path, monkeypatch, kernel, M, N):
+    """Launches that overlap, each reading the one before it, in a graph replayed many times: the bits of the
+    same calls made one by one.  (Loads that the assembler may move above the wait for the previous kernel
+    fail this at every replay.)"""
+    import torch
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    layers = 8 if kernel == "pair" else 40                # the pair kernel keeps 8 sets of tensor maps
+    case = (M, N, N, "bf16", "bf16", False, "silu", True, False)
+    k = _kernel(synth.linear_package(tmp_path, *case), "own")
+    _family(k, kernel)
+    t = _linear_inputs(case)
+    ws = [(torch.randn(N, N, device="cuda") * N ** -0.5).to(torch.bfloat16) for _ in range(layers)]
+    ys = [torch.empty(M, N, device="cuda", dtype=torch.bfloat16) for _ in ws]
+
+    def call(src, w, y):
+        k({"x": src.data_ptr(), "w": w.data_ptr(), "res": t["res"].data_ptr(), "linear": y.data_ptr()}, _stream())
+    refs, src = [], t["x"]
+    for w, y in zip(ws, ys):
+        call(src, w, y)
+        torch.cuda.synchronize()
+        refs.append(y.clone())
+        src = y
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        src = t["x"]
+        for w, y in zip(ws, ys):
+            call(src, w, y)
+            src = y
+    for i in range(50):
+        for y in ys:
+            y.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for n, (a, b) in enumerate(zip(ys, refs)):
+            assert torch.equal(a, b), f"replay {i}, layer {n}"
+    assert k.error_word() == 0
+    del graph
+    k.close()
+
+
+def test_heads_chain(tmp_path):
+    """The same for rotations: forward and inverse in turn, each of the one before it."""
+    import torch
+    spec = heads_spec((1, 64, 8, 0, 128, 128, "f32", False, False, False, False, False))
+    ks = [_kernel(heads_package(synth, tmp_path / str(inv), dict(spec, inverse=inv), 64), "own") for inv in (False, True)]
+    t = _heads_inputs(spec, 64)
+    ys = [torch.empty_like(t["qkv"]) for _ in range(40)]
+
+    def run(sync=False):
+        src = t["qkv"]
+        for i, y in enumerate(ys):
+            ks[i % 2]({"cos": t["cos"].data_ptr(), "sin": t["sin"].data_ptr(), "pos": t["pos"].data_ptr(),
+                       "qkv": src.data_ptr(), "q": y.data_ptr()}, _stream())
+            if sync:
+                torch.cuda.synchronize()
+            src = y
+    run(True)
+    refs = [y.clone() for y in ys]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for i in range(50):
+        for y in ys:
+            y.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ys, refs)), i
+    del graph
+    for k in ks:
+        k.close()
+
+
 @pytest.mark.parametrize("kernel", ["stream", "rows"])
 def test_few_row_kernels_share_a_graph_with_many_weights(tmp_path, monkeypatch, kernel):
     """One compiled kernel for all layers of a model: twenty weights captured into one graph with no call

@@ -158,11 +158,15 @@ def test_waits_for_the_previous_kernel(tmp_path, monkeypatch, kernel):
     lines = [ln.strip() for ln in _body(ptx)]
     generic = next(i for i, ln in enumerate(lines) if "generic lowering of the same IR" in ln)
     assert next(ln for ln in lines[generic + 1:] if ln and not ln.startswith("//")) == "griddepcontrol.wait;"
+    # no load whose data would have to be constant while the previous kernel still writes
+    assert not [ln for ln in lines if "ld.global.nc" in ln and not any(x in ln for x in HOST_TABLES)]
     lines = lines[:generic]
     at = lambda text: [i for i, ln in enumerate(lines) if text in ln]        # noqa: E731
     waits, first = at("griddepcontrol.wait"), at("griddepcontrol.wait")[0]
     for ln in lines[:first]:
-        assert not GLOBAL.match(ln) or any(x in ln for x in HOST_TABLES) or "atom.global.or.b32" in ln, ln
+        # prefetches into L2 read nothing; a refused launch only records its error
+        assert (not GLOBAL.match(ln) or any(x in ln for x in HOST_TABLES) or "atom.global.or.b32" in ln
+                or "prefetch.global.L2" in ln), ln
     if kernel == "rows":
         (alloc,), (trigger,) = at("tcgen05.alloc"), at("griddepcontrol.launch_dependents")
         assert len(waits) == 2 and waits[0] < alloc < trigger

@@ -25,11 +25,17 @@ from thompiler.walk import Walker
 
 class TunedKernel:
     family = "tuned"
+    # the generic path of the module, too, reads with ordinary loads.  A kernel launched to overlap the previous
+    # one begins while that one still writes, so its inputs are not constant for its lifetime, which is what
+    # ``ld.global.nc`` promises: the assembler may move such a load above griddepcontrol.wait, and did (a chain
+    # of linear-stream launches in a graph read the previous launch's input)
+    coherent = False
 
     def __init__(self, kernel: KernelInfo) -> None:
         self.k = kernel
         self.em = Emitter()
         self.w = Walker(self.em, kernel)
+        self.w.coherent = self.coherent
         self.pdl = False            # set by pdl_wait: the tuned body waits for the previous grid
 
     # programmatic dependent launch ----------------------------------------------

@@ -38,6 +38,7 @@ def _pow2_at_least(n: int) -> int:
 
 class RotaryHeads(TunedKernel):
     family = "rotary-heads"
+    coherent = True
 
     def __init__(self, kernel: KernelInfo, B, S, heads, kv, D, R, P, ty, interleaved, values, heads_first, inverse, eps):
         super().__init__(kernel)
@@ -305,7 +306,7 @@ class RotaryHeads(TunedKernel):
         self.pdl_wait()
         pos, pa, inside = t("b32"), t("b64"), t("pred")               # the position; does the unit store at all?
         ins(f"mad.wide.u32 {pa}, {token}, 4, {em.buffer_reg('pos')}")
-        ins(f"ld.global.nc.u32 {pos}, [{pa}]")
+        ins(f"ld.global.u32 {pos}, [{pa}]")
         raw, live = [], []
         for r in range(self.rounds):
             ok = t("pred")
@@ -333,7 +334,7 @@ class RotaryHeads(TunedKernel):
                     regs = em.tmps("b32", self._raw())
                     for x in regs:
                         ins(f"mov.u32 {x}, 0")
-                    self._vector("ld.global.nc", regs, a, f"@{pi} ")
+                    self._vector("ld.global", regs, a, f"@{pi} ")
                     pair.append(regs)
                 raws.append(pair)
                 lives.append(pi)
@@ -386,7 +387,7 @@ class RotaryHeads(TunedKernel):
                 for c in range(0, V, step):
                     g = regs[c:c + step]
                     vec, body = (f".v{step}", f"{{{', '.join(g)}}}") if step > 1 else ("", g[0])
-                    ins(f"@{q} ld.global.nc{vec}.f32 {body}, [{a}{f'+{4 * c}' if c else ''}]")
+                    ins(f"@{q} ld.global{vec}.f32 {body}, [{a}{f'+{4 * c}' if c else ''}]")
                 tab.append(regs)
             tables.append(tab)
             pair = []
@@ -397,7 +398,7 @@ class RotaryHeads(TunedKernel):
                 regs = em.tmps("b32", self._raw())
                 for x in regs:
                     ins(f"mov.u32 {x}, 0")
-                self._vector("ld.global.nc", regs, a, f"@{have[i]} " if have[i] else "")
+                self._vector("ld.global", regs, a, f"@{have[i]} " if have[i] else "")
                 pair.append(regs)
             weights.append(pair)
 

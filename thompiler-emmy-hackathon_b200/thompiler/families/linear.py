@@ -175,6 +175,7 @@ class Replay:
 
 class LinearPair(TcMatmulPair):
     family = "tcgen05-linear-pair"
+    coherent = True
 
     def __init__(self, p: Product):
         TunedKernel.__init__(self, p.kernel)
@@ -221,7 +222,7 @@ class LinearPair(TcMatmulPair):
     def estimate(self) -> float:
         """Microseconds (``choose`` says how the constants came about)."""
         waves = min(self.plans(self.p))[0]
-        return 1.4 + ((self.p.w.nbytes / 4.6e6) ** 4 + (waves * self.kblocks * 0.31) ** 4) ** 0.25 + 4.1 * waves
+        return 1.3 + ((self.p.w.nbytes / 4.3e6) ** 4 + (waves * self.kblocks * 0.31) ** 4) ** 0.25 + 4.0 * waves
 
     def guard(self, generic: str) -> None:
         super().guard(generic)
@@ -287,7 +288,7 @@ class LinearPair(TcMatmulPair):
                 if pred is not None and not into:
                     for x in four:
                         ins(f"mov.u32 {x}, 0")
-                ins(f"{f'@{pred} ' if pred else ''}ld.global.nc.v4.b32 {{{', '.join(four)}}}, [{self.at[src]}+{c * nb}]")
+                ins(f"{f'@{pred} ' if pred else ''}ld.global.v4.b32 {{{', '.join(four)}}}, [{self.at[src]}+{c * nb}]")
                 regs += four
             out[src] = regs
         return out
@@ -374,6 +375,8 @@ ROW_STEP = PRODUCERS // 8                    # rows that the producers copy a pi
 class ByElement(TunedKernel):
     """What the kernels for few rows share: a thread finishes single elements of C."""
 
+    coherent = True
+
     def __init__(self, p: Product):
         super().__init__(p.kernel)
         self.p = p
@@ -417,10 +420,10 @@ class ByElement(TunedKernel):
         at = f"@{pred} " if pred else ""
         em.ins(f"mov.u32 {r}, 0")
         if ty.nbytes == 4:
-            em.ins(f"{at}ld.global.nc.b32 {r}, [{a}]")
+            em.ins(f"{at}ld.global.b32 {r}, [{a}]")
         else:
             h = em.tmp("b16")
-            em.ins(f"{at}ld.global.nc.b16 {h}, [{a}]")
+            em.ins(f"{at}ld.global.b16 {h}, [{a}]")
             em.ins(f"{at}cvt.u32.u16 {r}, {h}")
         return [r]
 
@@ -569,6 +572,30 @@ class LinearRows(ByElement):
         ins(f"@{q} bra {role_mma}")
 
         # ---------------- producers (warps 0..7), then the epilogue ----------------
+        # the first stages of w start towards L2 while the previous kernel ends: a prefetch changes no value and
+        # returns none (what that kernel may still write passes through L2)
+        row, half_w, line, ok = t("b32"), t("b32"), t("b64"), t("pred")
+        ins(f"and.b32 {row}, {tid}, {BM - 1}")
+        ins(f"add.u32 {row}, {row}, {n0}")
+        ins(f"setp.lt.u32 {ok}, {row}, {p.N}")
+        ins(f"shr.u32 {half_w}, {tid}, {BM.bit_length() - 1}")
+        if G == 2:
+            ins(f"mad.lo.u32 {row}, {half_w}, {p.N}, {row}")
+        ins(f"mul.wide.u32 {line}, {row}, {p.K * 2}")
+        ins(f"add.u64 {line}, {line}, {em.buffer_reg(p.w.name)}")
+        first_k = t("b64")
+        ins(f"mul.wide.u32 {first_k}, {kb}, {BK * 2}")
+        ins(f"add.u64 {line}, {line}, {first_k}")
+        # only where a stage is mostly w (gated 16 x 8192 x 4096: 22.9 us without, 22.2 with; 128 x 4096 x 4096,
+        # half of it x: 12.1 and 12.3); with one accumulator the second half of the threads takes the odd stages
+        for i in range(0, ST if BT <= 32 * G else 0, 2 if G == 1 else 1):
+            want, s_ = t("pred"), t("b32")
+            ins(f"add.u32 {s_}, {half_w}, {i}" if G == 1 else f"mov.u32 {s_}, {i}")
+            ins(f"setp.lt.and.u32 {want}, {s_}, {nk}, {ok}")
+            a = t("b64")
+            ins(f"mul.wide.u32 {a}, {s_}, {BK * 2}")
+            ins(f"add.u64 {a}, {a}, {line}")
+            ins(f"@{want} prefetch.global.L2 [{a}]")
         # thread -> 16-byte piece c of rows r0, r0 + 32, ..: a warp copies four whole 128-byte rows at a time
         self.pdl_wait()
         r0, c, soff, k8 = t("b32"), t("b32"), t("b32"), t("b32")
@@ -942,19 +969,19 @@ class RowsPlan:
         return min(out, key=lambda x: x[:3])[3] if out else None
 
     def estimate(self, p: Product) -> float:
-        """Microseconds.  Reading w once from memory, and an SM's slabs through its copies (81 bytes a cycle)
-        or tensor cores (140 cycles a K block at least), overlap by halves (the power mean); then the
-        join of a cut K and the epilogue, by the tokens a CTA holds."""
+        """Microseconds.  Reading w once from memory, and an SM's slabs through its copies (77 bytes a cycle)
+        or tensor cores, overlap in part (the power mean); then the join of a cut K and the epilogue, by
+        the tokens a CTA holds."""
         per_sm = -(-self.ctas // SM_COUNT)
-        block = max(self.stage_bytes / 81, 0.35 * self.BT * self.G, 140) / 1900
-        memory, sm = p.w.nbytes / 8.9e6, per_sm * -(-self.kblocks // self.S) * block
+        block = max(self.stage_bytes / 77, 0.57 * self.BT * self.G) / 1900
+        memory, sm = p.w.nbytes / 8.2e6, per_sm * -(-self.kblocks // self.S) * block
         tokens = self.BT * self.G / 100
-        join = 0.3 + 1.5 * tokens if self.S > 1 else 0
-        return 2.2 + (memory ** 1.34 + sm ** 1.34) ** (1 / 1.34) + join + 2.0 * tokens * per_sm / self.S
+        join = (0.1 + 1.55 * tokens if self.S > 1 else 0) + (0.9 if self.S == 8 else 0)
+        return 2.1 + (memory ** 1.5 + sm ** 1.5) ** (1 / 1.5) + join + 2.0 * tokens * per_sm / self.S
 
 
 class LinearStream(ByElement):
-    """A handful of rows of x (up to 32) against all of w, bound by reading w once.
+    """A handful of rows of x (up to 24) against all of w, bound by reading w once.
 
     A CTA owns 16 rows of w (16 of each half when gated) and all of K; its eight warps take K in turns
     of ``U`` 32-wide chunks.  A lane loads 16 bytes of row g and of row g + 8 (g = lane / 4) at
@@ -965,8 +992,9 @@ class LinearStream(ByElement):
     as soon as its MMAs have read them.  The eight warps' sums meet in shared memory, added in
     warp order; a thread finishes one element at a time.
 
-    (mma.sync, because nothing is bound by its rate here: at 1 x 4096 x 4096 the tensor memory's
-    allocation, the operand barriers and the cluster's join of ``LinearRows`` cost a fifth of the time.)"""
+    (mma.sync, because nothing is bound by its rate here: 7 % of its cycles at 1 x 4096 x 4096, where w
+    arrives at 6.7 TB/s, 1.02 of the copy rate.  ``LinearRows`` takes 6.5 us there against 5.0: its CTAs
+    fill the SM's shared memory, so the next launch's cannot come early and send for its w.)"""
 
     family = "linear-stream"
 
@@ -1048,6 +1076,37 @@ class LinearStream(ByElement):
         if p.N % 16:
             inside = t("pred")
             ins(f"setp.lt.u32 {inside}, {n}, {p.N}")
+        # the first turns' lines of w, four lanes a row, start towards L2 while the previous kernel ends: a
+        # prefetch changes no value and returns none (what that kernel may still write passes through L2)
+        line_k = t("b32")
+        ins(f"shl.b32 {line_k}, {k8}, 6")
+        ins(f"mad.lo.u32 {line_k}, {warp}, {32 * U}, {line_k}")
+        lines = []
+        for h in (0, 1):
+            lr, la, lo = t("b32"), t("b64"), t("b64")
+            ins(f"add.u32 {lr}, {row}, {8 * h}")
+            ins(f"mul.wide.u32 {la}, {lr}, {p.K * 2}")
+            ins(f"mul.wide.u32 {lo}, {line_k}, 2")
+            ins(f"add.u64 {la}, {la}, {lo}")
+            ins(f"add.u64 {la}, {la}, {em.buffer_reg(p.w.name)}")
+            for i in range(G):
+                a = la
+                if i:
+                    a = t("b64")
+                    ins(f"add.u64 {a}, {la}, {p.N * p.K * 2}")
+                lines.append((a, high if h else None))
+        for turn in range(min(pl.ahead, -(-p.K // (256 * U)))):
+            fits, at_k = t("pred"), t("b32")
+            ins(f"add.u32 {at_k}, {line_k}, {256 * U * turn}")
+            ins(f"setp.lt.u32 {fits}, {at_k}, {p.K}")
+            if U < 8:                                          # a turn is fewer than four lines of a row
+                ins(f"setp.lt.and.u32 {fits}, {k8}, {U // 2}, {fits}")
+            for a, other in lines:
+                ok = fits
+                if other:
+                    ok = t("pred")
+                    ins(f"and.pred {ok}, {fits}, {other}")
+                ins(f"@{ok} prefetch.global.L2 [{a}+{512 * U * turn}]")
         self.pdl_wait()
 
         w_regs = [[[em.tmps("b32", 4) for _ in range(2)] for _ in range(G)] for _ in range(U)]
@@ -1078,9 +1137,9 @@ class LinearStream(ByElement):
             for i in range(G):
                 for h in (0, 1):
                     one(w_regs[u][i][h], wp[i], 64 * u + h * 8 * p.K * 2, both(high if h else None),
-                        "ld.global.nc.L1::no_allocate.L2::256B")
+                        "ld.global.L1::no_allocate.L2::256B")
             for i in range(NT):
-                one(x_regs[u][i], xp[i], 64 * u, both(tokens[i]), "ld.global.nc")
+                one(x_regs[u][i], xp[i], 64 * u, both(tokens[i]), "ld.global")
 
         for u in range(U):
             load(u, True)
@@ -1158,26 +1217,33 @@ class StreamPlan:
         self.NT = -(-p.M // 8)
         self.U = 8 if self.NT == 1 and self.G == 1 else 4
         self.ctas = -(-p.N // 16)
+        # turns whose lines are asked for before the previous kernel is done.  Us with none / one / two / four:
+        # 1 x 4096 x 4096 6.6 / 5.5 / 5.0 / 5.0, 8 x 1024 x 4096 4.6 / 2.9 / 3.0 / 3.0; with more CTAs than are
+        # resident at once, 1 x 8192 x 8192 22.1 / 20.5 / 21.2 / 25.7
+        self.ahead = 2 if self.ctas <= 2 * SM_COUNT else 1
         self.smem = 8 * self.G * self.NT * 8 * 80
 
     @classmethod
     def of(cls, p: Product) -> "StreamPlan | None":
-        return cls(p) if p.M <= 32 else None
+        return cls(p) if p.M <= 24 else None       # 32 x 4096 x 4096: 12.7 us, the rows kernel 8.0
 
     def estimate(self, p: Product) -> float:
-        turns = -(-self.ctas // (2 * SM_COUNT)) * p.K * self.G * 0.55e-3
-        return 1.5 + max(p.w.nbytes / 10.5e6, turns) + p.w.nbytes * self.NT * 0.068e-6
+        """Microseconds: w from memory, or the turns of the CTAs resident at once; past eight tokens x takes
+        as many loads as w."""
+        turns = -(-self.ctas // (2 * SM_COUNT)) * p.K * self.G * 0.44e-3
+        more = (self.NT - 1) * 0.05 + (0.016 if self.NT > 1 else 0)
+        return 1.15 + ((p.w.nbytes / 7.05e6) ** 4 + turns ** 4) ** 0.25 + p.w.nbytes * more / 1e6
 
 
 def choose(p: Product) -> TunedKernel:
     """The kernel and plan whose estimated time is least.
 
     The estimates' forms follow what bounds each kernel; their constants are a least-squares fit (of log
-    time) to 1,178 timings on a B200 of every plan at M = 1 .. 2048, (N, K) from 512 x 512 to 8192 x 4096,
-    plain and gated, back to back in graphs.  Over those 154 sizes the choice costs 1.7 % against the best
-    plan on average and 32 % at worst.  Some of both sides, in us (rows / stream / pair): 1 x 512 x 512
-    2.6 / 1.7 / 5.2; 1 x 4096 x 4096 7.2 / 6.5 / 21; 16 x 4096 x 4096 7.6 / 8.4 / 17; 128 x 4096 x 4096
-    12.5 / - / 18.6; 512 x 4096 x 4096 21.8 / - / 20.3; 2048 x 4096 x 4096 - / - / 51."""
+    time) to 1,284 timings on a B200 of every plan at M = 1 .. 2048, (N, K) from 512 x 512 to 8192 x 4096,
+    plain and gated, back to back in graphs.  Over those 187 sizes the choice costs 1.1 % against the best
+    plan on average and 18 % at worst.  Some of both sides, in us (stream / rows / pair): 1 x 512 x 512
+    1.4 / 2.5 / 5.3; 1 x 4096 x 4096 5.0 / 6.5 / 21; 16 x 4096 x 4096 7.4 / 7.0 / 17; 128 x 4096 x 4096
+    - / 12.1 / 18.6; 512 x 4096 x 4096 - / 21.8 / 20.3; 2048 x 4096 x 4096 - / - / 51."""
     pair = LinearPair(p)
     plans = [(pair.estimate(), "pair", lambda: pair)]
     rows, stream = RowsPlan.best(p), StreamPlan.of(p)

@@ -46,7 +46,7 @@ def emit_load(w: "Walker", load: ir.Load) -> None:
     vals = regs = [em.value(n, F32.reg if ty is BF16 else ty.reg) for n in load.names]
     if ty is BF16:
         regs = em.tmps(ty.reg, width)
-    op = "ld.global.nc" if (space == "global" and readonly) else f"ld.{space}"
+    op = "ld.global.nc" if (space == "global" and readonly and not w.coherent) else f"ld.{space}"
     if width == 1:
         em.ins(f"{op}.{ty.mov} {regs[0]}, [{addr}]")
     else:

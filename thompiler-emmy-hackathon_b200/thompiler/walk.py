@@ -45,6 +45,7 @@ class Walker:
         self.fragments: dict = {}
         self.consts: dict[str, int] = {}
         self.wgmma = None                      # tensor-memory plan of Wgmma* accumulators
+        self.coherent = False                  # Loads of read-only buffers as ordinary loads (families.base)
         self.load_hook: Callable[[Any, ir.Load], bool] | None = None
         self.write_hook: Callable[[Any, ir.Write], bool] | None = None
         self._writes = Counter(s.output for s in ir.walk_stmts(kernel.body) if isinstance(s, ir.Write))
