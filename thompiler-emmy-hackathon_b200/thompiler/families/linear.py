@@ -992,9 +992,9 @@ class LinearStream(ByElement):
     as soon as its MMAs have read them.  The eight warps' sums meet in shared memory, added in
     warp order; a thread finishes one element at a time.
 
-    (mma.sync, because nothing is bound by its rate here: 7 % of its cycles at 1 x 4096 x 4096, where w
-    arrives at 6.7 TB/s, 1.02 of the copy rate.  ``LinearRows`` takes 6.5 us there against 5.0: its CTAs
-    fill the SM's shared memory, so the next launch's cannot come early and send for its w.)"""
+    (mma.sync, because nothing is bound by its rate here: 7 % of its cycles at 1 x 4096 x 4096, which takes
+    6.1 us, 5.5 TB/s.  ``LinearRows`` takes 6.8 there: the operand barriers and the cluster's join are a
+    fifth of its time, and its CTAs fill the SM's shared memory, so the next launch's cannot come early.)"""
 
     family = "linear-stream"
 
@@ -1218,8 +1218,8 @@ class StreamPlan:
         self.U = 8 if self.NT == 1 and self.G == 1 else 4
         self.ctas = -(-p.N // 16)
         # turns whose lines are asked for before the previous kernel is done.  Us with none / one / two / four:
-        # 1 x 4096 x 4096 6.6 / 5.5 / 5.0 / 5.0, 8 x 1024 x 4096 4.6 / 2.9 / 3.0 / 3.0; with more CTAs than are
-        # resident at once, 1 x 8192 x 8192 22.1 / 20.5 / 21.2 / 25.7
+        # 1 x 4096 x 4096 6.7 / 6.3 / 6.1 / 6.1, 4 x 1024 x 4096 4.1 / 4.0 / 3.7 / 3.6; with more CTAs than are
+        # resident at once, 1 x 8192 x 8192 22.4 / 20.7 / 22.0 / 26.1
         self.ahead = 2 if self.ctas <= 2 * SM_COUNT else 1
         self.smem = 8 * self.G * self.NT * 8 * 80
 
@@ -1230,19 +1230,19 @@ class StreamPlan:
     def estimate(self, p: Product) -> float:
         """Microseconds: w from memory, or the turns of the CTAs resident at once; past eight tokens x takes
         as many loads as w."""
-        turns = -(-self.ctas // (2 * SM_COUNT)) * p.K * self.G * 0.44e-3
-        more = (self.NT - 1) * 0.05 + (0.016 if self.NT > 1 else 0)
-        return 1.15 + ((p.w.nbytes / 7.05e6) ** 4 + turns ** 4) ** 0.25 + p.w.nbytes * more / 1e6
+        turns = -(-self.ctas // (2 * SM_COUNT)) * p.K * self.G * 0.63e-3
+        more = p.w.nbytes * (self.NT - 1) * 0.056e-6
+        return 1.5 + ((p.w.nbytes / 6.7e6) ** 4 + turns ** 4) ** 0.25 + more
 
 
 def choose(p: Product) -> TunedKernel:
     """The kernel and plan whose estimated time is least.
 
     The estimates' forms follow what bounds each kernel; their constants are a least-squares fit (of log
-    time) to 1,284 timings on a B200 of every plan at M = 1 .. 2048, (N, K) from 512 x 512 to 8192 x 4096,
-    plain and gated, back to back in graphs.  Over those 187 sizes the choice costs 1.1 % against the best
-    plan on average and 18 % at worst.  Some of both sides, in us (stream / rows / pair): 1 x 512 x 512
-    1.4 / 2.5 / 5.3; 1 x 4096 x 4096 5.0 / 6.5 / 21; 16 x 4096 x 4096 7.4 / 7.0 / 17; 128 x 4096 x 4096
+    time) to 1,290 timings on a B200 of every plan at M = 1 .. 2048, (N, K) from 512 x 512 to 8192 x 4096,
+    plain and gated, back to back in graphs.  Over those 193 sizes the choice costs 1.4 % against the best
+    plan on average and 32 % at worst.  Some of both sides, in us (stream / rows / pair): 1 x 512 x 512
+    1.7 / 2.5 / 5.3; 1 x 4096 x 4096 6.1 / 6.8 / 21; 16 x 4096 x 4096 7.7 / 7.0 / 17; 128 x 4096 x 4096
     - / 12.1 / 18.6; 512 x 4096 x 4096 - / 21.8 / 20.3; 2048 x 4096 x 4096 - / - / 51."""
     pair = LinearPair(p)
     plans = [(pair.estimate(), "pair", lambda: pair)]
