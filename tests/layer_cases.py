@@ -126,6 +126,7 @@ LINEAR = [
     (2048, 2048, 1024, "f16", "f32", False, None, True, False),
     (2049, 1000, 64, "bf16", "bf16", True, "relu", True, False),
     (2560, 2560, 1024, "bf16", "bf16", True, None, False, False),
+    (1300, 264, 16384, "bf16", "bf16", True, None, True, False),       # bands of four and of two rows of tiles
 ]
 
 # (B, S, heads, kv, D, R, dtype, interleaved, values, heads_first, inverse, norm)

@@ -201,6 +201,12 @@ class LinearPair(TcMatmulPair):
         self.units = self.full_tiles + 2 * self.hrem
         self.pairs = min(self.units, PAIR_SLOTS)
         self.ctas = 2 * self.pairs
+        # tiles are walked in bands of as many rows as keep a band's x within 32 MB, so that it stays in L2 (two
+        # halves of 63 MB) while w passes once a band.  TFLOP/s at the power limit, all rows / 4 / 8 / 16: 16384 x
+        # 4096 x 4096 1030 / 1351 / 1335 / 1332, 8192^3 1192 / 1282 / 1318 / 1282, gated 8192 x 8192 x 4096
+        # 1276 / 1300 / 1359 / 1390, 4096 x 4096 x 8192 1121 / 1133 / 1142 / 1120
+        band = max(4, (32 << 20) // (PM * p.K * 2))
+        self.band = band if self.tiles_m > band else 0
         self.replay = Replay(self, p) if p.epilogue is not None else None
 
     @staticmethod

@@ -49,6 +49,7 @@ class TcMatmulPair(TcMatmul):
     family = "tcgen05-matmul-pair"
     tail_ranks = 2
     epilogue = None              # a RegStore epilogue to apply (thompiler.families.linear)
+    band = 0                     # rows of tiles walked together (0: all of them, column by column)
 
     @classmethod
     def match(cls, kernel: KernelInfo):
@@ -142,6 +143,24 @@ class TcMatmulPair(TcMatmul):
         super().guard(generic)
         self.em.entry_attrs.append(".reqnctapercluster 2, 1, 1")
 
+    def decode_band(self, tile: str) -> tuple[str, str, str]:
+        """Tile -> (row, column, K slice 0) in bands of ``band`` rows of tiles, column by column within one."""
+        em, t, ins = self.em, self.em.tmp, self.em.ins
+        b, first, rest, rows, tm, tn, ts = (t("b32") for _ in range(7))
+        ins(f"div.u32 {b}, {tile}, {self.band * self.tiles_n}")
+        ins(f"rem.u32 {rest}, {tile}, {self.band * self.tiles_n}")
+        ins(f"mul.lo.u32 {first}, {b}, {self.band}")
+        if self.tiles_m % self.band:                   # the last band has fewer rows
+            ins(f"sub.u32 {rows}, {self.tiles_m}, {first}")
+            ins(f"min.u32 {rows}, {rows}, {self.band}")
+        else:
+            ins(f"mov.u32 {rows}, {self.band}")
+        ins(f"rem.u32 {tm}, {rest}, {rows}")
+        ins(f"add.u32 {tm}, {tm}, {first}")
+        ins(f"div.u32 {tn}, {rest}, {rows}")
+        ins(f"mov.u32 {ts}, 0")
+        return tm, tn, ts
+
     def tile_begin(self, row: str, rank: str, tm: str, tn: str, whole: str, part: str) -> None:
         """Hook: an epilogue thread (its row of the CTA's 128) is about to wait for a tile's sums."""
 
@@ -231,6 +250,8 @@ class TcMatmulPair(TcMatmul):
         kit = Kit(em, errp, end)
 
         def decode(tile: str):
+            if self.band:
+                return self.decode_band(tile)
             tm_, tn_, ts_, r = t("b32"), t("b32"), t("b32"), t("b32")
             ins(f"rem.u32 {tm_}, {tile}, {tiles_m}")
             ins(f"div.u32 {r}, {tile}, {tiles_m}")
