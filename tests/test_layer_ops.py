@@ -225,3 +225,30 @@ def test_rotary_refusals(kw):
         rotary.frequencies(**kw)
     with pytest.raises(ValueError):
         rotary.tables(0, 8)
+
+
+@pytest.mark.parametrize("index,tuned", [
+    (("col",), True), (("col<72",), True), (("col<16",), False), (("col<72", 72), True), (("col<16", 72), False),
+    (("row<40", "col<72"), True), (("row<8", "col"), False), (("row", "col<64"), False), (("col", "row"), False)], ids=str)
+def test_epilogue_index_is_taken_for_what_it_is(tmp_path, index, tuned):
+    """An epilogue's load that is clamped short of C's sizes reads other elements than the row's and column's
+    own: the tuned kernels leave it to the generic lowering."""
+    from thompiler import schedules
+    from thompiler.emitter import read_sidecar
+    M, N, K = 40, 72, 64
+    V, L, f32 = schedules.V, schedules.L, schedules.F32T
+
+    def at(t):
+        name, _, n = t.partition("<")
+        return schedules.clamped(V(name), int(n)) if n else V(name)
+    if len(index) == 2 and isinstance(index[1], int):
+        idx, shape = (schedules.B("+", at(index[0]), L(index[1])),), (2 * N,)
+    else:
+        idx, shape = tuple(at(t) for t in index), (N,) if len(index) == 1 else (M, N)
+    epi = ir.Lambda(("z", "row", "col"), (ir.Load(("e",), "extra", idx, f32),
+                                                    schedules.assign("y", "add", "z", "e")), ("y",))
+    inputs = {"x": ((M, K), "f16", None), "w": ((N, K), "f16", None), "extra": (shape, "f32", None)}
+    d = synth._layer_write(tmp_path, "extra", "extra", "k_linear", schedules.linear_body(M, N, K, "f16", False, epi),
+                           inputs, {"linear": ((M, N), "f32", None)}, 8, 128, 2e-2, 2e-3, smem=2 * 64 * 64 * 2)
+    side = read_sidecar(compile_kernel(load.load(str(_ir(d))))) or {}
+    assert ("linear" in side.get("family", "")) == tuned

@@ -81,16 +81,17 @@ class Replay:
         """(buffer, over columns only?, first column) of a load, or None for a constant."""
         if all(isinstance(i, ir.Literal) for i in load.index):
             return None
-        index = [schedules.unclamped(i) for i in load.index]
         row, col = ir.Var("row"), ir.Var("col")
-        if len(index) == 2 and index == [row, col]:
+        # clamped at C's own sizes an index is itself wherever the element is stored; at others it is not
+        rows, cols = (row, schedules.clamped(row, p.M)), (col, schedules.clamped(col, p.N))
+        if len(load.index) == 2 and load.index[0] in rows and load.index[1] in cols:
             return load.input, False, 0
-        if len(index) == 1:
-            e = index[0]
-            if e == col:
+        if len(load.index) == 1:
+            e = load.index[0]
+            if e in cols:
                 return load.input, True, 0
             if isinstance(e, ir.BinaryExpr) and e.op == "+" and isinstance(e.right, ir.Literal) \
-                    and schedules.unclamped(e.left) == col and e.right.value % 8 == 0:
+                    and e.left in cols and e.right.value % 8 == 0:
                 return load.input, True, e.right.value
         raise LookupError(load.input)
 

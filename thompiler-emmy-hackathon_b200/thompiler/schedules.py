@@ -41,15 +41,6 @@ def clamped(e, n: int):
     return ir.TernaryExpr(B("<", e, L(n)), e, L(n - 1))
 
 
-def unclamped(e):
-    """``e`` without a ``clamped`` around it."""
-    if (isinstance(e, ir.TernaryExpr) and isinstance(e.cond, ir.BinaryExpr) and e.cond.op == "<"
-            and e.cond.left == e.if_true and isinstance(e.cond.right, ir.Literal)
-            and isinstance(e.if_false, ir.Literal) and e.if_false.value == e.cond.right.value - 1):
-        return e.if_true
-    return e
-
-
 def _load(name, buf, index, dtype):
     """One element as an f32 value (bf16 elements widen as they are loaded, f16 ones by a copy)."""
     if dtype == "f16":
