@@ -432,6 +432,25 @@ def test_not_finite(tmp_path, monkeypatch, kernel):
     k.close()
 
 
+@pytest.mark.parametrize("act", ["relu", "gelu_tanh"])
+@pytest.mark.parametrize("kernel", ["stream", "rows", "pair", "generic"])
+def test_activations_keep_nan(tmp_path, monkeypatch, kernel, act):
+    """A NaN row of x is a NaN row of the result, not the zeros of a maximum."""
+    import torch
+    if kernel != "generic":
+        monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    case = (9, 72, 64, "f16", "f32", False, act, False, False)
+    k = _kernel(synth.linear_package(tmp_path, *case), "generic" if kernel == "generic" else "own")
+    t = _linear_inputs(case)
+    t["x"][4, 63] = float("nan")
+    y = torch.zeros(9, 72, device="cuda")
+    k({n: v.data_ptr() for n, v in dict(t, linear=y).items()}, _stream())
+    torch.cuda.synchronize()
+    assert k.error_word() == 0
+    assert bool(y[4].isnan().all()) and int(y.isnan().sum()) == 72
+    k.close()
+
+
 def test_heads_not_finite(tmp_path):
     """Of a head that rotates half of its elements, a NaN in the rest stays where it is; with the norm it
     takes the head and no other."""

@@ -252,3 +252,13 @@ def test_epilogue_index_is_taken_for_what_it_is(tmp_path, index, tuned):
                            inputs, {"linear": ((M, N), "f32", None)}, 8, 128, 2e-2, 2e-3, smem=2 * 64 * 64 * 2)
     side = read_sidecar(compile_kernel(load.load(str(_ir(d))))) or {}
     assert ("linear" in side.get("family", "")) == tuned
+
+
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu_tanh"])
+def test_activations_keep_nan(tmp_path, act):
+    """A NaN in x reaches its row of the result through every activation, and no other row."""
+    d = synth.linear_package(tmp_path, 3, 72, 64, activation=act)
+    x = problems.make_inputs(problems.load_package(d))
+    x["x"][1, 5] = np.nan
+    got = oracle_run(d, x)["linear"]
+    assert np.isnan(got[1]).all() and np.isfinite(got[[0, 2]]).all()

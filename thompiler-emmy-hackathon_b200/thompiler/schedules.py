@@ -69,8 +69,9 @@ def activation(z: str, name: str | None) -> tuple[list, str]:
     """Statements that apply an activation to the f32 value ``z``, and the result's name."""
     if name is None:
         return [], z
-    if name == "relu":
-        return [assign("act", "relu", z)], "act"
+    if name == "relu":                                  # z < 0 ? 0 : z keeps a NaN; max(z, 0) would hide it
+        return [ir.Let("none", L(0.0, "float"), F32T),
+                ir.Select("act", (ir.Branch(V("none"), B("<", V(z), L(0.0, "float"))), ir.Branch(V(z), None)))], "act"
     if name == "silu":
         return [assign("sg", "sigmoid", z), assign("act", "multiply", z, "sg")], "act"
     if name == "gelu_tanh":
