@@ -173,6 +173,25 @@ def test_heads(tmp_path, case, launch):
 
 # ---- as they are used --------------------------------------------------------------------------
 
+ODD_HEADS = [(2, 9, 3, 2, 7, 4, "f32", False, True, True, False, False), (1, 33, 2, 1, 33, 32, "bf16", True, True, False, False, True),
+             (3, 4, 1, 1, 129, 2, "f16", False, False, True, True, False)]
+
+
+@pytest.mark.parametrize("case", ODD_HEADS, ids=str)
+def test_heads_of_odd_length(tmp_path, case):
+    """An odd number of elements a head has no pairs to move at a time: the generic lowering serves it."""
+    import torch
+    spec, table = heads_spec(case), 50
+    k = _kernel(heads_package(synth, tmp_path, spec, table), "own")
+    assert k.family == "generic"
+    t, out = _heads_inputs(spec, table), _heads_outputs(spec)
+    t["pos"][-1, -1] = -1
+    k(dict({n: v.data_ptr() for n, v in t.items()}, **{n: v.data_ptr() for n, (_, v) in out.items()}), _stream())
+    torch.cuda.synchronize()
+    _heads_check(spec, table, t, out, "odd")
+    k.close()
+
+
 def _family(k, *names):
     assert any(n in k.family for n in names), k.family
 
@@ -279,7 +298,7 @@ def test_chain_reads_what_the_launch_before_wrote(tmp_path, monkeypatch, kernel,
     fail this at every replay.)"""
     import torch
     monkeypatch.setattr(TUNING, "linear_kernel", kernel)
-    layers = 8 if kernel == "pair" else 40                # the pair kernel keeps 8 sets of tensor maps
+    layers = 40
     case = (M, N, N, "bf16", "bf16", False, "silu", True, False)
     k = _kernel(synth.linear_package(tmp_path, *case), "own")
     _family(k, kernel)
@@ -376,6 +395,88 @@ def test_few_row_kernels_share_a_graph_with_many_weights(tmp_path, monkeypatch, 
             src = y
     assert k.error_word() == 0
     del graph
+    k.close()
+
+
+def test_pair_kernel_serves_many_weights(tmp_path, monkeypatch):
+    """The kernel for many rows keeps 128 sets of tensor maps: 150 weights one after another re-encode the
+    oldest, a hundred of them then share a graph."""
+    import torch
+    monkeypatch.setattr(TUNING, "linear_kernel", "pair")
+    M, N = 200, 264
+    case = (M, N, N, "bf16", "bf16", False, None, True, False)
+    k = _kernel(synth.linear_package(tmp_path, *case), "own")
+    _family(k, "pair")
+    t = _linear_inputs(case)
+    ws = [(torch.randn(N, N, device="cuda") * N ** -0.5).to(torch.bfloat16) for _ in range(150)]
+    ys = [torch.empty(M, N, device="cuda", dtype=torch.bfloat16) for _ in ws]
+    for w in ws:
+        w.fill_diagonal_(0.5)
+
+    def run(first, last):
+        for w, y in zip(ws[first:last], ys[first:last]):
+            k({"x": t["x"].data_ptr(), "w": w.data_ptr(), "res": t["res"].data_ptr(), "linear": y.data_ptr()},
+              _stream())
+
+    def verify(first, last):
+        for i in range(first, last):
+            _linear_check(case, {"x": t["x"], "w": ws[i], "res": t["res"]}, ys[i], f"weight {i}")
+    run(0, 150)
+    torch.cuda.synchronize()
+    verify(0, 150)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(50, 150)
+    t["x"].copy_(_linear_inputs(case, 1)["x"])
+    for y in ys:
+        y.fill_(float("nan"))
+    run(0, 50)                                            # others around it leave the graph's sets alone
+    graph.replay()
+    torch.cuda.synchronize()
+    assert k.error_word() == 0
+    verify(0, 150)
+    del graph
+    k.close()
+
+
+@pytest.mark.parametrize("launch", ["generic", "stream", "rows", "pair"])
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+def test_residual_in_place_and_shared_inputs(tmp_path, monkeypatch, launch, gated):
+    """``res`` may be ``linear`` itself (every element is read by the thread that then stores it), and x."""
+    import torch
+    if launch != "generic":
+        monkeypatch.setattr(TUNING, "linear_kernel", launch)
+    for M in (20, 24):
+        case = (M, 1032, 1032, "bf16", "bf16", True, "silu", True, gated)
+        k = _kernel(synth.linear_package(tmp_path / str(M), *case), "generic" if launch == "generic" else "own")
+        assert launch in k.family
+        t = _linear_inputs(case)
+        want = dict(t, res=t["res"].clone())
+        ptrs = {n: v.data_ptr() for n, v in t.items()}
+        k(dict(ptrs, linear=ptrs["res"]), _stream())
+        torch.cuda.synchronize()
+        _linear_check(case, want, t["res"], f"{k.family} in place")
+        y = torch.empty_like(t["res"])
+        k(dict(ptrs, res=ptrs["x"], linear=y.data_ptr()), _stream())
+        torch.cuda.synchronize()
+        _linear_check(case, dict(t, res=t["x"]), y, f"{k.family} x + f(x)")
+        assert k.error_word() == 0
+        k.close()
+
+
+def test_residual_in_place_many_tiles(tmp_path):
+    """The same over tiles that share rows and columns of several CTAs."""
+    import torch
+    case = (1300, 2056, 520, "f16", "f16", False, None, True, False)
+    k = _kernel(synth.linear_package(tmp_path, *case), "own")
+    t = _linear_inputs(case)
+    before = t["res"].clone()
+    for _ in range(3):
+        t["res"].copy_(before)
+        ptrs = {n: v.data_ptr() for n, v in t.items()}
+        k(dict(ptrs, linear=ptrs["res"]), _stream())
+        torch.cuda.synchronize()
+        _linear_check(case, dict(t, res=before), t["res"], k.family)
     k.close()
 
 

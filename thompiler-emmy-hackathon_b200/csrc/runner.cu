@@ -345,10 +345,10 @@ int tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const cha
         if (old_.empty()) return -1;
         for (int k = 0; k < r->sets; ++k) {
             TmapSet &o = r->s[k];
-            if (k == v || o.ptrs.empty() || !in_flight(o)) continue;
+            if (k == v || o.ptrs.empty()) continue;
             bool mix = true;
             for (int i = 0; i < ntmaps && mix; ++i) mix = o.ptrs[i] == old_[i] || o.ptrs[i] == want[i];
-            if (mix) return k;
+            if (mix && in_flight(o)) return k;
         }
         return -1;
     };

@@ -21,11 +21,11 @@ TMAP_SETS = 8                 # tensor-map sets a tuned module keeps (launches i
 TMAP_RING, TMAP_TABLE = "thc_tmap_ring", "thc_tmap_ptr"
 
 
-def declare_tmap_ring(em, nmaps: int) -> None:
-    """Module globals of TMAP_SETS sets of ``nmaps`` tensor maps and the buffer addresses each set
+def declare_tmap_ring(em, nmaps: int, sets: int = TMAP_SETS) -> None:
+    """Module globals of ``sets`` sets of ``nmaps`` tensor maps and the buffer addresses each set
     is encoded for (the runner fills them: thr_tmap_bind)."""
-    em.module(f".global .align 64 .b8 {TMAP_RING}[{TMAP_SETS * nmaps * 128}]")
-    em.module(f".global .align 8 .u64 {TMAP_TABLE}[{TMAP_SETS * nmaps}]")
+    em.module(f".global .align 64 .b8 {TMAP_RING}[{sets * nmaps * 128}]")
+    em.module(f".global .align 8 .u64 {TMAP_TABLE}[{sets * nmaps}]")
 
 
 def select_tmap_set(em, params: list[str], generic: str) -> str:
@@ -58,6 +58,40 @@ def select_tmap_set(em, params: list[str], generic: str) -> str:
         em.ins(f"selp.u32 {sel}, {k}, {sel}, {hit}")
     em.ins(f"setp.eq.u32 {eq}, {sel}, {TMAP_SETS}")
     em.ins(f"@{eq} bra {generic}")
+    return sel
+
+
+def find_tmap_set(em, params: list[str], generic: str, sets: int) -> str:
+    """``select_tmap_set`` for a table too long for every thread to read: each lane of a warp (all of them
+    here) compares ``sets / 32`` sets, loaded first, and a vote gives the lowest that matches."""
+    p, lane = em.tmp("pred"), em.tmp("b32")
+    raws = []
+    for name in params:
+        raws.append(em.tmp("b64"))
+        em.ins(f"ld.param.u64 {raws[-1]}, [p_{name}]")
+    em.ins(f"setp.eq.u64 {p}, {raws[0]}, 0")
+    em.ins(f"@{p} bra {generic}")
+    n, mine = len(params), em.tmp("b64")
+    em.ins(f"mov.u32 {lane}, %laneid")
+    em.ins(f"mov.u64 {mine}, {TMAP_TABLE}")
+    em.ins(f"mad.wide.u32 {mine}, {lane}, {8 * n}, {mine}")
+    table = [[em.tmp("b64") for _ in raws] for _ in range(sets // 32)]
+    for k, entry in enumerate(table):
+        for i, r in enumerate(entry):
+            em.ins(f"ld.global.nc.u64 {r}, [{mine}+{8 * (32 * k * n + i)}]")
+    sel = em.tmp("b32")
+    em.ins(f"mov.u32 {sel}, {sets}")
+    for k in reversed(range(len(table))):           # the lowest matching set wins
+        hit, votes, first = em.tmp("pred"), em.tmp("b32"), em.tmp("b32")
+        for i, (raw, r) in enumerate(zip(raws, table[k])):
+            em.ins(f"setp.eq{'.and' if i else ''}.u64 {hit}, {raw}, {r}{f', {hit}' if i else ''}")
+        em.ins(f"vote.sync.ballot.b32 {votes}, {hit}, 0xffffffff")
+        em.ins(f"setp.ne.u32 {p}, {votes}, 0")
+        em.ins(f"brev.b32 {first}, {votes}")
+        em.ins(f"clz.b32 {first}, {first}")
+        em.ins(f"@{p} add.u32 {sel}, {first}, {32 * k}")
+    em.ins(f"setp.eq.u32 {p}, {sel}, {sets}")
+    em.ins(f"@{p} bra {generic}")
     return sel
 
 

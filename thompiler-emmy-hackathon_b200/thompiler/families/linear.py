@@ -177,6 +177,10 @@ class Replay:
 class LinearPair(TcMatmulPair):
     family = "tcgen05-linear-pair"
     coherent = True
+    # one compiled product serves every layer of a model.  Past the sets each call re-encodes one: 32 weights of
+    # 4096 x 4096 at 512 rows, one after another, take 208 us a call with 8 sets (the other families') and 18.2
+    # with 128; one weight 17.6 and 17.8
+    map_sets = 128
 
     def __init__(self, p: Product):
         TunedKernel.__init__(self, p.kernel)

@@ -46,7 +46,7 @@ from __future__ import annotations
 from thompiler import ir
 from thompiler.families.base import TunedKernel
 from thompiler.families.kit import (TMAP_RING, TMAP_SETS, TMAP_TABLE, declare_tmap_ring, elect_one,
-                                    select_tmap_set, tmap_address)
+                                    find_tmap_set, select_tmap_set, tmap_address)
 from thompiler.families.tuning import TUNING
 from thompiler.lowering.types import F16, F32
 from thompiler.load import KernelInfo
@@ -72,6 +72,7 @@ def idesc_f16(n: int, b_mn_major: bool) -> int:
 
 class TcMatmul(TunedKernel):
     family = "tcgen05-matmul"
+    map_sets = TMAP_SETS
     tail_ranks = 1               # CTAs sharing one output tile (2 for the CTA-pair kernel)
 
     def __init__(self, kernel: KernelInfo, a, b, c, M, N, K, S, b_kmajor, static_smem):
@@ -218,7 +219,7 @@ class TcMatmul(TunedKernel):
         side = {"grid": [self.ctas, 1, 1], "block": [THREADS, 1, 1], "smem_bytes": self.smem,
                 "tmaps": [tm_a, tm_b, tm_c],
                 "tmap_ptrs": {"global": TMAP_TABLE, "params": [a.name, b.name, self.c.name]},
-                "tmap_sets": TMAP_SETS, "error_word": "thc_error", "tile": [BM, self.BN, BK],
+                "tmap_sets": self.map_sets, "error_word": "thc_error", "tile": [BM, self.BN, BK],
                 "stages": self.stages}
         if self.rem:
             side["counters"] = ["thc_tile_arrivals"]           # the split tail's (tile, rank) counters
@@ -236,7 +237,7 @@ class TcMatmul(TunedKernel):
 
     def guard(self, generic: str) -> None:
         em = self.em
-        declare_tmap_ring(em, 3)
+        declare_tmap_ring(em, 3, self.map_sets)
         em.module(".global .align 4 .u32 thc_error")
         if self.rem:                 # per tensor-map set, so launches on other buffers run concurrently
             em.module(f".global .align 4 .u32 thc_tile_arrivals[{TMAP_SETS * self.tail_counters}]")
@@ -247,7 +248,9 @@ class TcMatmul(TunedKernel):
         em.ins(f"setp.ne.u32 {p}, {r}, {THREADS}")
         em.ins(f"@{p} bra {generic}")
         # the tensor-map set encoded for these buffers (else the generic lowering)
-        self.tmap_set = select_tmap_set(em, [x.name for x in (self.a, self.b, self.c)], generic)
+        bufs = [x.name for x in (self.a, self.b, self.c)]
+        self.tmap_set = (select_tmap_set(em, bufs, generic) if self.map_sets == TMAP_SETS
+                         else find_tmap_set(em, bufs, generic, self.map_sets))
 
     def tail_bases(self, cnt: str, ws: str) -> None:
         """Point ``cnt`` / ``ws`` at the selected tensor-map set's split-tail counters / partials."""

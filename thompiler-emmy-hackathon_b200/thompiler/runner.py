@@ -310,8 +310,8 @@ class TensorMaps:
 class Launch:
     """One kernel's launches on device pointers.  What stays the same from call to call is a C record made
     once, so ``launch(ptrs, stream)`` packs the pointers and makes one C call (with its tensor maps'
-    binding, when the plan has any).  ``plan``'s grid, block and shared memory are read again whenever
-    they are replaced; a buffer that meta.json wants aligned is refused when it is not."""
+    binding, when the plan has any).  ``plan``'s grid, block, shared memory and overlap are read again
+    whenever they are replaced; a buffer that meta.json wants aligned is refused when it is not."""
 
     def __init__(self, function: Function, plan: LaunchPlan, kmeta: dict, tmaps: TensorMaps | None):
         self.function, self.plan, self.order, self.tmaps = function, plan, tuple(kmeta["arg_order"]), tmaps
@@ -332,11 +332,11 @@ class Launch:
             d.tmaps, d.ntmaps, d.ptr_table = t.specs, t.n, t.table
         self._descs.append(d)                 # kept: a call in another thread may still be reading the last one
         self._at = ctypes.addressof(d)
-        self._geometry = (plan.grid, plan.block, plan.smem)
+        self._geometry = (plan.grid, plan.block, plan.smem, plan.pdl)
 
     def __call__(self, ptrs: dict[str, int], stream: int = 0) -> None:
         plan = self.plan
-        if (plan.grid, plan.block, plan.smem) != self._geometry:
+        if (plan.grid, plan.block, plan.smem, plan.pdl) != self._geometry:
             self._prepare()
         st = self._call(self._at, self._pack(*self._get(ptrs)), stream)
         if st:

@@ -15,6 +15,9 @@ substituted (the shipped r01 and r02 IRs differ only in ``Dim(1024)`` vs
 row per CTA for row reductions.  An arg may carry an ``init`` record
 (``{"dist": "uniform", "low", "high", "seed"}``) for non-normal inputs;
 ``seed`` args keep the runner's standard-normal meaning.
+
+The layer operators (``linear_package``, ``rope_package``, ``qk_norm_rope_package``) have no shipped
+IR; ``schedules`` holds their statement trees.
 """
 
 from __future__ import annotations
@@ -311,7 +314,8 @@ def linear_package(outdir, M: int, N: int, K: int, dtype: str = "f16", out_dtype
     activation is None, "relu", "silu" or "gelu_tanh".  gated: w[2N, K] and bias[2N] hold two
     projections, and the result is act(first) * second (+ res).  M is any number of rows from one
     on; N and K are multiples of 8 (16-byte rows).  The entry is ``k_linear`` over x, w, (bias,)
-    (res,) linear, buffers that do not overlap and start on 16-byte boundaries."""
+    (res,) linear, on 16-byte boundaries; ``linear`` overlaps none of the others, but may be ``res``
+    itself where their types are the same."""
     _positive(M=M, N=N, K=K)
     out_dtype = out_dtype or dtype
     if dtype not in ("f16", "bf16") or out_dtype not in (dtype, "f32"):
@@ -399,7 +403,8 @@ def rope_package(outdir, B: int, S: int, heads: int, kv_heads: int, D: int, rota
     [0, table) -- an empty slot's -1 -- leaves that token's rows of the outputs as they were.
     ``inverse`` rotates by the negative angle: the gradient of the rotation.  The entry is
     ``k_rope`` over cos, sin, pos, qkv, q, (k, (v)); each buffer starts on a multiple of the vectors that
-    the kernel moves (16 bytes, less where the sizes leave less: ``align`` in meta.json)."""
+    the kernel moves (16 bytes, less where the sizes leave less: ``align`` in meta.json), and the outputs
+    overlap nothing."""
     return _heads_package(outdir, "k_rope", B, S, heads, kv_heads, D, rotary, interleaved, dtype, table, values,
                           heads_first, inverse, None)
 
