@@ -439,6 +439,25 @@ def test_pair_kernel_serves_many_weights(tmp_path, monkeypatch):
     k.close()
 
 
+def test_pair_kernel_refuses_buffers_without_maps(tmp_path, monkeypatch):
+    """A launch in the kernel's own geometry on buffers whose tensor maps nobody bound writes nothing and says
+    so in the error word (the generic lowering needs meta.json's grid)."""
+    import torch
+    monkeypatch.setattr(TUNING, "linear_kernel", "pair")
+    case = (200, 264, 264, "bf16", "bf16", False, None, False, False)
+    k = _kernel(synth.linear_package(tmp_path, *case), "own")
+    t = _linear_inputs(case)
+    y = torch.full((200, 264), SENTINEL, device="cuda", dtype=torch.bfloat16)
+    ptrs = {n: v.data_ptr() for n, v in dict(t, linear=y).items()}
+    k.fn.launch(k.plan.grid, k.plan.block, k.plan.smem, [ptrs[n] for n in k.arg_order], _stream())
+    torch.cuda.synchronize()
+    assert k.error_word() == 1 << 4 and bool((y == SENTINEL).all())
+    k(ptrs, _stream())
+    torch.cuda.synchronize()
+    _linear_check(case, t, y, k.family)
+    k.close()
+
+
 @pytest.mark.parametrize("launch", ["generic", "stream", "rows", "pair"])
 @pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
 def test_residual_in_place_and_shared_inputs(tmp_path, monkeypatch, launch, gated):

@@ -156,16 +156,18 @@ def test_waits_for_the_previous_kernel(tmp_path, monkeypatch, kernel):
     ptx = compile_kernel(load.load(str(_ir(d))))
     assert kernel in (read_sidecar(ptx) or {})["family"] and read_sidecar(ptx)["pdl"] is True
     lines = [ln.strip() for ln in _body(ptx)]
+    # the tables that the host writes in stream order, by name or through a register that points into one
+    tables = (*HOST_TABLES, *(f"[{m[1]}+" for ln in lines if (m := re.match(r"mov\.u64 (%\w+), thc_tmap_ptr;", ln))))
     generic = next(i for i, ln in enumerate(lines) if "generic lowering of the same IR" in ln)
     assert next(ln for ln in lines[generic + 1:] if ln and not ln.startswith("//")) == "griddepcontrol.wait;"
     # no load whose data would have to be constant while the previous kernel still writes
-    assert not [ln for ln in lines if "ld.global.nc" in ln and not any(x in ln for x in HOST_TABLES)]
+    assert not [ln for ln in lines if "ld.global.nc" in ln and not any(x in ln for x in tables)]
     lines = lines[:generic]
     at = lambda text: [i for i, ln in enumerate(lines) if text in ln]        # noqa: E731
     waits, first = at("griddepcontrol.wait"), at("griddepcontrol.wait")[0]
     for ln in lines[:first]:
         # prefetches into L2 read nothing; a refused launch only records its error
-        assert (not GLOBAL.match(ln) or any(x in ln for x in HOST_TABLES) or "atom.global.or.b32" in ln
+        assert (not GLOBAL.match(ln) or any(x in ln for x in tables) or "atom.global.or.b32" in ln
                 or "prefetch.global.L2" in ln), ln
     if kernel == "rows":
         (alloc,), (trigger,) = at("tcgen05.alloc"), at("griddepcontrol.launch_dependents")

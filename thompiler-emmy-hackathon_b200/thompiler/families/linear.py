@@ -236,11 +236,11 @@ class LinearPair(TcMatmulPair):
         return 1.3 + ((self.p.w.nbytes / 4.3e6) ** 4 + (waves * self.kblocks * 0.31) ** 4) ** 0.25 + 4.0 * waves
 
     def guard(self, generic: str) -> None:
-        super().guard(generic)
+        bad = self.em.label("unbound")               # no maps for these buffers, or a source off its boundary
+        super().guard(generic, bad)
         if self.replay:
-            bad = self.em.label("misaligned")
             self.replay.check_alignment(bad)
-            self.refuse(bad, 4)
+        self.refuse(bad, 4)
 
     # ---- the epilogue, a box of columns at a time -----------------------------------------
 

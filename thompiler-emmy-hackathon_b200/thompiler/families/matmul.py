@@ -235,7 +235,7 @@ class TcMatmul(TunedKernel):
         """Split-tail partials per tensor-map set."""
         return self.rem * self.tail_ranks * self.parts * BM * self.BN * 4
 
-    def guard(self, generic: str) -> None:
+    def guard(self, generic: str, unbound: str | None = None) -> None:
         em = self.em
         declare_tmap_ring(em, 3, self.map_sets)
         em.module(".global .align 4 .u32 thc_error")
@@ -247,10 +247,10 @@ class TcMatmul(TunedKernel):
         r = self.special("%ntid.x")
         em.ins(f"setp.ne.u32 {p}, {r}, {THREADS}")
         em.ins(f"@{p} bra {generic}")
-        # the tensor-map set encoded for these buffers (else the generic lowering)
+        # the tensor-map set encoded for these buffers (else ``unbound``, the generic lowering by default)
         bufs = [x.name for x in (self.a, self.b, self.c)]
-        self.tmap_set = (select_tmap_set(em, bufs, generic) if self.map_sets == TMAP_SETS
-                         else find_tmap_set(em, bufs, generic, self.map_sets))
+        self.tmap_set = (select_tmap_set(em, bufs, unbound or generic) if self.map_sets == TMAP_SETS
+                         else find_tmap_set(em, bufs, unbound or generic, self.map_sets))
 
     def tail_bases(self, cnt: str, ws: str) -> None:
         """Point ``cnt`` / ``ws`` at the selected tensor-map set's split-tail counters / partials."""

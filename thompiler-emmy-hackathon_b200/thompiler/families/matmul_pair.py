@@ -139,8 +139,8 @@ class TcMatmulPair(TcMatmul):
         assert side["tmap_ptrs"]["params"] == [a.name, b.name, self.c.name]
         return side
 
-    def guard(self, generic: str) -> None:
-        super().guard(generic)
+    def guard(self, generic: str, unbound: str | None = None) -> None:
+        super().guard(generic, unbound)
         self.em.entry_attrs.append(".reqnctapercluster 2, 1, 1")
 
     def decode_band(self, tile: str) -> tuple[str, str, str]:
