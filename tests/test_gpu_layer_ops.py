@@ -68,16 +68,16 @@ def _linear_check(case, t, got, what):
     check(_np(got), want, allowed, what)
 
 
-@pytest.mark.parametrize("launch", ["own", "meta", "generic", "stream", "rows", "pair"])
+@pytest.mark.parametrize("launch", ["own", "meta", "generic", "stream", "rows", "split", "pair"])
 @pytest.mark.parametrize("case", LINEAR, ids=str)
 def test_linear(tmp_path, monkeypatch, case, launch):
-    """``stream``, ``rows`` and ``pair`` force one of the tuned kernels, also at sizes it is not chosen for."""
+    """``stream``, ``rows``, ``split`` and ``pair`` force one of the tuned kernels, also at sizes it is not chosen for."""
     import torch
     M, N = case[:2]
-    if launch in ("stream", "rows", "pair"):
+    if launch in ("stream", "rows", "split", "pair"):
         monkeypatch.setattr(TUNING, "linear_kernel", launch)
     k = _kernel(synth.linear_package(tmp_path, *case), launch)
-    if launch in ("stream", "rows", "pair") and not k.family.endswith(launch):
+    if launch in ("stream", "rows", "split", "pair") and not k.family.endswith(launch):
         pytest.skip(f"no {launch} plan for this size")
     t = _linear_inputs(case)
     whole, y = _out((M, N), case[4])
@@ -95,7 +95,7 @@ def test_linear(tmp_path, monkeypatch, case, launch):
     k.close()
 
 
-@pytest.mark.parametrize("kernel", ["generic", "stream", "rows", "pair"])
+@pytest.mark.parametrize("kernel", ["generic", "stream", "rows", "split", "pair"])
 @pytest.mark.parametrize("M,N,K", [(20, 200, 264), (32, 64, 64), (600, 328, 200)])
 def test_custom_epilogue(tmp_path, monkeypatch, kernel, M, N, K):
     """Epilogues of other statements, buffers and types than the builder's are replayed by every kernel."""
@@ -291,7 +291,7 @@ def test_a_layer(tmp_path, dtype):
 
 
 @pytest.mark.parametrize("kernel,M,N", [("stream", 5, 512), ("stream", 16, 1024), ("rows", 5, 512), ("rows", 200, 512),
-                                        ("pair", 300, 512)])
+                                        ("split", 300, 512), ("split", 20, 1024), ("pair", 300, 512)])
 def test_chain_reads_what_the_launch_before_wrote(tmp_path, monkeypatch, kernel, M, N):
     """Launches that overlap, each reading the one before it, in a graph replayed many times: the bits of the
     same calls made one by one.  (Loads that the assembler may move above the wait for the previous kernel
@@ -439,11 +439,12 @@ def test_pair_kernel_serves_many_weights(tmp_path, monkeypatch):
     k.close()
 
 
-def test_pair_kernel_refuses_buffers_without_maps(tmp_path, monkeypatch):
+@pytest.mark.parametrize("kernel", ["split", "pair"])
+def test_refuses_buffers_without_maps(tmp_path, monkeypatch, kernel):
     """A launch in the kernel's own geometry on buffers whose tensor maps nobody bound writes nothing and says
     so in the error word (the generic lowering needs meta.json's grid)."""
     import torch
-    monkeypatch.setattr(TUNING, "linear_kernel", "pair")
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
     case = (200, 264, 264, "bf16", "bf16", False, None, False, False)
     k = _kernel(synth.linear_package(tmp_path, *case), "own")
     t = _linear_inputs(case)
@@ -458,7 +459,7 @@ def test_pair_kernel_refuses_buffers_without_maps(tmp_path, monkeypatch):
     k.close()
 
 
-@pytest.mark.parametrize("launch", ["generic", "stream", "rows", "pair"])
+@pytest.mark.parametrize("launch", ["generic", "stream", "rows", "split", "pair"])
 @pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
 def test_residual_in_place_and_shared_inputs(tmp_path, monkeypatch, launch, gated):
     """``res`` may be ``linear`` itself (every element is read by the thread that then stores it), and x."""
@@ -499,7 +500,7 @@ def test_residual_in_place_many_tiles(tmp_path):
     k.close()
 
 
-@pytest.mark.parametrize("kernel", ["stream", "rows", "pair"])
+@pytest.mark.parametrize("kernel", ["stream", "rows", "split", "pair"])
 def test_two_streams_at_once(tmp_path, monkeypatch, kernel):
     """Calls of one kernel in flight on two streams, on buffers of their own."""
     import torch
@@ -521,7 +522,7 @@ def test_two_streams_at_once(tmp_path, monkeypatch, kernel):
     k.close()
 
 
-@pytest.mark.parametrize("kernel", ["stream", "rows", "pair", "generic"])
+@pytest.mark.parametrize("kernel", ["stream", "rows", "split", "pair", "generic"])
 def test_not_finite(tmp_path, monkeypatch, kernel):
     """NaN and infinities stay in the rows and columns they belong to: a NaN row of x, an infinite row of w,
     an infinite residual; the padding of K, M and N adds none."""
@@ -553,7 +554,7 @@ def test_not_finite(tmp_path, monkeypatch, kernel):
 
 
 @pytest.mark.parametrize("act", ["relu", "gelu_tanh"])
-@pytest.mark.parametrize("kernel", ["stream", "rows", "pair", "generic"])
+@pytest.mark.parametrize("kernel", ["stream", "rows", "split", "pair", "generic"])
 def test_activations_keep_nan(tmp_path, monkeypatch, kernel, act):
     """A NaN row of x is a NaN row of the result, not the zeros of a maximum."""
     import torch

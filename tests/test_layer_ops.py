@@ -111,6 +111,19 @@ def test_linear_assembles(tmp_path, case, tuned):
     _ptxas(compile_kernel(load.load(str(_ir(d))), tuned=tuned), tmp_path)
 
 
+@pytest.mark.parametrize("kernel", ["stream", "rows", "split", "pair"])
+@pytest.mark.parametrize("case", [LINEAR[i] for i in (4, 5, 7)] + [(20, 264, 200, "bf16", "f32", True, "relu", True, False)],
+                         ids=str)
+def test_each_linear_kernel_assembles(tmp_path, monkeypatch, case, kernel):
+    from thompiler.emitter import read_sidecar
+    from thompiler.families.tuning import TUNING
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    ptx = compile_kernel(load.load(str(_ir(synth.linear_package(tmp_path, *case)))))
+    if not (kernel == "stream" and case[0] > 24):
+        assert read_sidecar(ptx)["family"].endswith(kernel)
+    _ptxas(ptx, tmp_path)
+
+
 @pytest.mark.parametrize("tuned", [True, False], ids=["tuned", "generic"])
 @pytest.mark.parametrize("case", HEADS, ids=str)
 def test_heads_assemble(tmp_path, case, tuned):
@@ -142,7 +155,7 @@ def test_misaligned_buffer_is_refused_by_name(tmp_path):
     assert min(want.values()) == 8                        # the last one moves four f16 elements at a time
 
 
-@pytest.mark.parametrize("kernel", ["stream", "rows", "pair", "heads"])
+@pytest.mark.parametrize("kernel", ["stream", "rows", "split", "pair", "heads"])
 def test_waits_for_the_previous_kernel(tmp_path, monkeypatch, kernel):
     """Launches may overlap the previous kernel's end: no access to global data, and in the kernel whose CTAs
     share SMs with others' no tensor memory taken, before the wait for it; the next kernel may come

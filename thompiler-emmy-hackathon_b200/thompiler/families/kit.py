@@ -61,16 +61,17 @@ def select_tmap_set(em, params: list[str], generic: str) -> str:
     return sel
 
 
-def find_tmap_set(em, params: list[str], generic: str, sets: int) -> str:
-    """``select_tmap_set`` for a table too long for every thread to read: each lane of a warp (all of them
-    here) compares ``sets / 32`` sets, loaded first, and a vote gives the lowest that matches."""
+def load_tmap_table(em, params: list[str], missing: str, sets: int, pred: str) -> tuple[list[str], list[list[str]]]:
+    """For a table too long for every thread to read: the warp in which ``pred`` holds (all its lanes) issues
+    the loads of ``sets / 32`` sets a lane, for ``match_tmap_set``.  A null first parameter branches to
+    ``missing``."""
     p, lane = em.tmp("pred"), em.tmp("b32")
     raws = []
     for name in params:
         raws.append(em.tmp("b64"))
         em.ins(f"ld.param.u64 {raws[-1]}, [p_{name}]")
     em.ins(f"setp.eq.u64 {p}, {raws[0]}, 0")
-    em.ins(f"@{p} bra {generic}")
+    em.ins(f"@{p} bra {missing}")
     n, mine = len(params), em.tmp("b64")
     em.ins(f"mov.u32 {lane}, %laneid")
     em.ins(f"mov.u64 {mine}, {TMAP_TABLE}")
@@ -78,10 +79,16 @@ def find_tmap_set(em, params: list[str], generic: str, sets: int) -> str:
     table = [[em.tmp("b64") for _ in raws] for _ in range(sets // 32)]
     for k, entry in enumerate(table):
         for i, r in enumerate(entry):
-            em.ins(f"ld.global.nc.u64 {r}, [{mine}+{8 * (32 * k * n + i)}]")
-    sel = em.tmp("b32")
-    em.ins(f"mov.u32 {sel}, {sets}")
-    for k in reversed(range(len(table))):           # the lowest matching set wins
+            em.ins(f"@{pred} ld.global.nc.u64 {r}, [{mine}+{8 * (32 * k * n + i)}]")
+    return raws, table
+
+
+def match_tmap_set(em, raws: list[str], table: list[list[str]]) -> str:
+    """A register with the lowest set whose addresses equal the parameters, by a vote of the warp, or the
+    number of sets when there is none."""
+    sel, p = em.tmp("b32"), em.tmp("pred")
+    em.ins(f"mov.u32 {sel}, {32 * len(table)}")
+    for k in reversed(range(len(table))):
         hit, votes, first = em.tmp("pred"), em.tmp("b32"), em.tmp("b32")
         for i, (raw, r) in enumerate(zip(raws, table[k])):
             em.ins(f"setp.eq{'.and' if i else ''}.u64 {hit}, {raw}, {r}{f', {hit}' if i else ''}")
@@ -90,8 +97,6 @@ def find_tmap_set(em, params: list[str], generic: str, sets: int) -> str:
         em.ins(f"brev.b32 {first}, {votes}")
         em.ins(f"clz.b32 {first}, {first}")
         em.ins(f"@{p} add.u32 {sel}, {first}, {32 * k}")
-    em.ins(f"setp.eq.u32 {p}, {sel}, {sets}")
-    em.ins(f"@{p} bra {generic}")
     return sel
 
 

@@ -21,8 +21,9 @@ from __future__ import annotations
 
 from thompiler import ir, schedules
 from thompiler.families.base import TunedKernel
-from thompiler.families.kit import Kit, desc_hi, elect_one, idesc_f16
-from thompiler.families.matmul import BK, BM, EPI_WARPS, SM_COUNT, STAGE_TILE
+from thompiler.families.kit import (Kit, declare_tmap_ring, desc_hi, elect_one, idesc_f16, load_tmap_table,
+                                    match_tmap_set)
+from thompiler.families.matmul import BK, BM, EPI_WARPS, SM_COUNT, STAGE_TILE, THREADS
 from thompiler.families.matmul_pair import PAIR_SLOTS, PAIR_WIDTHS, PM, SMEM_LIMIT, TcMatmulPair
 from thompiler.families.tuning import TUNING
 from thompiler.load import KernelInfo
@@ -177,6 +178,7 @@ class Replay:
 class LinearPair(TcMatmulPair):
     family = "tcgen05-linear-pair"
     coherent = True
+    offset = None                # columns from the tile's first to those that this thread finishes
     # one compiled product serves every layer of a model.  Past the sets each call re-encodes one: 32 weights of
     # 4096 x 4096 at 512 rows, one after another, take 208 us a call with 8 sets (the other families') and 18.2
     # with 128; one weight 17.6 and 17.8
@@ -233,14 +235,91 @@ class LinearPair(TcMatmulPair):
     def estimate(self) -> float:
         """Microseconds (``choose`` says how the constants came about)."""
         waves = min(self.plans(self.p))[0]
-        return 1.3 + ((self.p.w.nbytes / 4.3e6) ** 4 + (waves * self.kblocks * 0.31) ** 4) ** 0.25 + 4.0 * waves
+        block = 0.263 * (1 + 0.226 * self.ctas / SM_COUNT)
+        fixed = 5.35 * min(waves, 1) + 0.96 * max(waves - 1, 0)          # later epilogues run under the next MMAs
+        return ((self.p.w.nbytes / 6.55e6) ** 4 + (waves * self.kblocks * block) ** 4) ** 0.25 + fixed
 
     def guard(self, generic: str) -> None:
-        bad = self.em.label("unbound")               # no maps for these buffers, or a source off its boundary
-        super().guard(generic, bad)
+        self.guard_launch(generic, THREADS, 2)
+
+    def guard_launch(self, generic: str, threads: int, cluster: int) -> str:
+        """The checks of a launch of ``threads`` in clusters of ``cluster``; the label to which one that cannot be
+        served goes."""
+        em = self.em
+        declare_tmap_ring(em, 3, self.map_sets)
+        em.module(".global .align 4 .u32 thc_error")
+        em.module(".extern .shared .align 1024 .b8 smem_pool[]")
+        em.entry_attrs.append(f".reqnctapercluster {cluster}, 1, 1")
+        q = em.tmp("pred")
+        em.ins(f"setp.ne.u32 {q}, {self.special('%ntid.x')}, {threads}")
+        em.ins(f"@{q} bra {generic}")
+        bad = em.label("unserved")
+        em.ins(f"setp.lt.u32 {q}, {self.special('%tid.x')}, 32")
+        self.table = load_tmap_table(em, [b.name for b in (self.a, self.b, self.c)], bad, self.map_sets, q)
         if self.replay:
             self.replay.check_alignment(bad)
         self.refuse(bad, 4)
+        return bad
+
+    # ---- barriers, tensor memory and maps ----------------------------------------------------
+
+    def set_up(self, bars, warp, tid, empty_off, accf_off, acce_off, slot_off, sel_off, _, p) -> None:
+        """full and empty per stage, full per accumulator: one arrival; empty per accumulator: both CTAs'
+        epilogue warps."""
+        self.start(bars, warp, tid, [1] * (2 * self.stages + 2) + [2 * EPI_WARPS] * 2, slot_off, sel_off, self.tmem_cols)
+
+    def start(self, bars, warp, tid, counts: list[int], slot_off: int, sel_off: int, cols: int) -> None:
+        """At once: warp 0 searches the table of maps, warp 1 takes the pair's tensor memory, warp 2 initialises
+        the barriers; then the cluster meets."""
+        em = self.em
+        t, ins, place, lab = em.tmp, em.ins, em.place, em.label
+        done, search, init = lab("lp_ready"), lab("lp_search"), lab("lp_init")
+        q, at = t("pred"), t("b32")
+        ins(f"setp.eq.u32 {q}, {warp}, 0")
+        ins(f"@{q} bra {search}")
+        ins(f"setp.eq.u32 {q}, {warp}, 2")
+        ins(f"@{q} bra {init}")
+        ins(f"setp.ne.u32 {q}, {warp}, 1")
+        ins(f"@{q} bra {done}")
+        ins(f"add.u32 {at}, {bars}, {slot_off}")
+        ins(f"tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [{at}], {cols}")
+        ins("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned")
+        ins(f"bra {done}")
+        place(init)
+        i, count = t("b32"), t("b32")
+        ins(f"sub.u32 {i}, {tid}, 64")
+        ins(f"setp.ge.u32 {q}, {i}, {len(counts)}")
+        ins(f"@{q} bra {done}")
+        ones = counts.count(1)                                 # these come first
+        ins(f"setp.lt.u32 {q}, {i}, {ones}")
+        ins(f"selp.u32 {count}, 1, {counts[-1]}, {q}")
+        ins(f"mad.lo.u32 {at}, {i}, 8, {bars}")
+        ins(f"mbarrier.init.shared::cta.b64 [{at}], {count}")
+        ins("fence.mbarrier_init.release.cluster")
+        ins("fence.proxy.async.shared::cta")
+        ins(f"bra {done}")
+        place(search)
+        sel = match_tmap_set(em, *self.table)
+        ins(f"st.shared.u32 [{bars}+{sel_off}], {sel}")
+        place(done)
+        ins("bar.warp.sync -1")
+        ins("tcgen05.fence::before_thread_sync")
+        ins("barrier.cluster.arrive.release")
+        ins("barrier.cluster.wait.acquire")
+        ins("tcgen05.fence::after_thread_sync")
+        self.tmap_set = t("b32")
+        ins(f"ld.shared.u32 {self.tmap_set}, [{bars}+{sel_off}]")
+
+    def check_maps(self, end: str) -> None:
+        """No set of maps for these buffers: record it and leave."""
+        em = self.em
+        q, a, bound = em.tmp("pred"), em.tmp("b64"), em.label("bound")
+        em.ins(f"setp.lt.u32 {q}, {self.tmap_set}, {self.map_sets}")
+        em.ins(f"@{q} bra {bound}")
+        em.ins(f"mov.u64 {a}, thc_error")
+        em.ins(f"atom.global.or.b32 {em.tmp('b32')}, [{a}], {1 << 4}")
+        em.ins(f"bra {end}")
+        em.place(bound)
 
     # ---- the epilogue, a box of columns at a time -----------------------------------------
 
@@ -254,6 +333,8 @@ class LinearPair(TcMatmulPair):
         ins(f"mul.lo.u32 {self.col}, {tn}, {self.tile_cols}")
         if self.hrem:
             ins(f"@!{whole} mad.lo.u32 {self.col}, {part}, {self.BN // 2}, {self.col}")
+        if self.offset:
+            ins(f"add.u32 {self.col}, {self.col}, {self.offset}")
         self.row_ok = self.left = None
         if p.M % PM:
             self.row_ok = t("pred")
@@ -365,13 +446,16 @@ class LinearPair(TcMatmulPair):
             ins(f"add.u32 {col}, {self.col}, {c0 + j}")
             out.append(self.replay.element(z[0], z[1] if len(z) > 1 else None, self.row, col,
                                            lambda src, j=j: (mine[src], j)))
-        packed = []
-        step = 4 // self.c.ty.nbytes
-        for j in range(0, cw, step):
-            x = t("b32")
-            ins(f"mov.b32 {x}, {out[j]}" if step == 1 else f"cvt.rn.{self.c.ty.ptx}x2.f32 {x}, {out[j + 1]}, {out[j]}")
-            packed.append(x)
-        return packed
+        return self._packed(out)
+
+    def _packed(self, vals: list[str]) -> list[str]:
+        """f32 values as the 32-bit words of C's type."""
+        em, out, step = self.em, [], 4 // self.c.ty.nbytes
+        for j in range(0, len(vals), step):
+            out.append(em.tmp("b32"))
+            em.ins(f"mov.b32 {out[-1]}, {vals[j]}" if step == 1 else
+                   f"cvt.rn.{self.c.ty.ptx}x2.f32 {out[-1]}, {vals[j + 1]}, {vals[j]}")
+        return out
 
 
 # ---- few rows ----------------------------------------------------------------------------
@@ -980,15 +1064,16 @@ class RowsPlan:
         return min(out, key=lambda x: x[:3])[3] if out else None
 
     def estimate(self, p: Product) -> float:
-        """Microseconds.  Reading w once from memory, and an SM's slabs through its copies (77 bytes a cycle)
-        or tensor cores, overlap in part (the power mean); then the join of a cut K and the epilogue, by
-        the tokens a CTA holds."""
+        """Microseconds.  Reading w once from memory, and an SM's slabs through its copies (78 bytes a cycle,
+        less as more SMs copy) or tensor cores, overlap in part (the power mean); then the join of a cut
+        K and the epilogue, by the tokens a CTA holds."""
+        load = self.ctas / SM_COUNT
         per_sm = -(-self.ctas // SM_COUNT)
-        block = max(self.stage_bytes / 77, 0.57 * self.BT * self.G) / 1900
-        memory, sm = p.w.nbytes / 8.2e6, per_sm * -(-self.kblocks // self.S) * block
+        block = max(self.stage_bytes / 78 * (1 + 0.12 * load / per_sm), 0.93 * self.BT * self.G) / 1900
+        memory, sm = p.w.nbytes / 7.6e6, per_sm * -(-self.kblocks // self.S) * block
         tokens = self.BT * self.G / 100
-        join = (0.1 + 1.55 * tokens if self.S > 1 else 0) + (0.9 if self.S == 8 else 0)
-        return 2.1 + (memory ** 1.5 + sm ** 1.5) ** (1 / 1.5) + join + 2.0 * tokens * per_sm / self.S
+        join = (0.28 + 1.18 * tokens if self.S > 1 else 0) + (1.12 if self.S == 8 else 0)
+        return 2.09 + (memory ** 1.95 + sm ** 1.95) ** (1 / 1.95) + join + 0.63 * tokens * per_sm / self.S
 
 
 class LinearStream(ByElement):
@@ -1249,12 +1334,14 @@ class StreamPlan:
 def choose(p: Product) -> TunedKernel:
     """The kernel and plan whose estimated time is least.
 
-    The estimates' forms follow what bounds each kernel; their constants are a least-squares fit (of log
-    time) to 1,290 timings on a B200 of every plan at M = 1 .. 2048, (N, K) from 512 x 512 to 8192 x 4096,
-    plain and gated, back to back in graphs.  Over those 193 sizes the choice costs 1.4 % against the best
-    plan on average and 32 % at worst.  Some of both sides, in us (stream / rows / pair): 1 x 512 x 512
-    1.7 / 2.5 / 5.3; 1 x 4096 x 4096 6.1 / 6.8 / 21; 16 x 4096 x 4096 7.7 / 7.0 / 17; 128 x 4096 x 4096
-    - / 12.1 / 18.6; 512 x 4096 x 4096 - / 21.8 / 20.3; 2048 x 4096 x 4096 - / - / 51."""
+    The estimates' forms follow what bounds each kernel; their constants are least-squares fits (of log
+    time) to 1,745 timings on a B200 of every plan at M = 1 .. 1024, (N, K) from 512 x 512 to 8192 x 8192,
+    plain and gated, back to back in graphs.  Over those 251 sizes the choice costs 1.5 % against the best
+    plan on average and 32 % at worst; over 44 sizes drawn at random (M 24 .. 2513, ragged) it missed the
+    fastest kernel five times, by 3 to 22 %.  Some of all sides, in us (stream / rows / split / pair):
+    1 x 512 x 512 1.7 / 2.5 / - / 5.3; 1 x 4096 x 4096 6.1 / 6.8 / - / 21; 16 x 4096 x 4096 7.7 / 7.0 / - / 17;
+    128 x 4096 x 4096 - / 10.3 / 12.0 / 16.5; 512 x 4096 x 8192 - / 32.1 / 28.4 / 31.4; 835 x 440 x 4048 gated
+    - / 29.8 / 11.8 / 24.2; 1024 x 4096 x 4096 - / 28.8 / - / 26.3; 2048 x 4096 x 4096 - / - / - / 51."""
     pair = LinearPair(p)
     plans = [(pair.estimate(), "pair", lambda: pair)]
     rows, stream = RowsPlan.best(p), StreamPlan.of(p)
@@ -1262,6 +1349,10 @@ def choose(p: Product) -> TunedKernel:
         plans.append((rows.estimate(p), "rows", lambda: LinearRows(p, rows)))
     if stream is not None:
         plans.append((stream.estimate(p), "stream", lambda: LinearStream(p, stream)))
+    from thompiler.families.linear_split import LinearSplit, SplitPlan
+    split = SplitPlan.best(p)
+    if split is not None:
+        plans.append((split.estimate(p), "split", lambda: LinearSplit(p, split)))
     forced = [x for x in plans if x[1] == TUNING.linear_kernel]
     return min(forced or plans, key=lambda x: x[0])[2]()
 

@@ -46,7 +46,7 @@ from __future__ import annotations
 from thompiler import ir
 from thompiler.families.base import TunedKernel
 from thompiler.families.kit import (TMAP_RING, TMAP_SETS, TMAP_TABLE, declare_tmap_ring, elect_one,
-                                    find_tmap_set, select_tmap_set, tmap_address)
+                                    select_tmap_set, tmap_address)
 from thompiler.families.tuning import TUNING
 from thompiler.lowering.types import F16, F32
 from thompiler.load import KernelInfo
@@ -235,9 +235,9 @@ class TcMatmul(TunedKernel):
         """Split-tail partials per tensor-map set."""
         return self.rem * self.tail_ranks * self.parts * BM * self.BN * 4
 
-    def guard(self, generic: str, unbound: str | None = None) -> None:
+    def guard(self, generic: str) -> None:
         em = self.em
-        declare_tmap_ring(em, 3, self.map_sets)
+        declare_tmap_ring(em, 3)
         em.module(".global .align 4 .u32 thc_error")
         if self.rem:                 # per tensor-map set, so launches on other buffers run concurrently
             em.module(f".global .align 4 .u32 thc_tile_arrivals[{TMAP_SETS * self.tail_counters}]")
@@ -247,10 +247,8 @@ class TcMatmul(TunedKernel):
         r = self.special("%ntid.x")
         em.ins(f"setp.ne.u32 {p}, {r}, {THREADS}")
         em.ins(f"@{p} bra {generic}")
-        # the tensor-map set encoded for these buffers (else ``unbound``, the generic lowering by default)
-        bufs = [x.name for x in (self.a, self.b, self.c)]
-        self.tmap_set = (select_tmap_set(em, bufs, unbound or generic) if self.map_sets == TMAP_SETS
-                         else find_tmap_set(em, bufs, unbound or generic, self.map_sets))
+        # the tensor-map set encoded for these buffers (else the generic lowering)
+        self.tmap_set = select_tmap_set(em, [x.name for x in (self.a, self.b, self.c)], generic)
 
     def tail_bases(self, cnt: str, ws: str) -> None:
         """Point ``cnt`` / ``ws`` at the selected tensor-map set's split-tail counters / partials."""

@@ -139,8 +139,8 @@ class TcMatmulPair(TcMatmul):
         assert side["tmap_ptrs"]["params"] == [a.name, b.name, self.c.name]
         return side
 
-    def guard(self, generic: str, unbound: str | None = None) -> None:
-        super().guard(generic, unbound)
+    def guard(self, generic: str) -> None:
+        super().guard(generic)
         self.em.entry_attrs.append(".reqnctapercluster 2, 1, 1")
 
     def decode_band(self, tile: str) -> tuple[str, str, str]:
@@ -169,6 +169,49 @@ class TcMatmulPair(TcMatmul):
         on in boxes of ``cw``: ``stage(buffer, values, column, offset)`` writes one, ``free(last)`` releases
         the accumulator where ``last`` holds."""
         raise NotImplementedError
+
+    def set_up(self, bars, warp, tid, empty_off, accf_off, acce_off, slot_off, tail_done_off, tail_last_off, p) -> None:
+        """Barriers and tensor memory of the pair, ready in both CTAs for every thread that leaves."""
+        em = self.em
+        t, ins, place, lab = em.tmp, em.ins, em.place, em.label
+        ST = self.stages
+        skip = lab("mp_noinit")
+        ins(f"setp.ne.u32 {p}, {tid}, 0")
+        ins(f"@{p} bra {skip}")
+        for s in range(ST):
+            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{8 * s}], 1")
+            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{empty_off + 8 * s}], 1")
+        for b in range(2):
+            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{accf_off + 8 * b}], 1")
+            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{acce_off + 8 * b}], {2 * EPI_WARPS}")
+        if self.rem:
+            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{tail_done_off}], {32 * EPI_WARPS}")
+            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{tail_last_off}], 1")
+        ins("fence.mbarrier_init.release.cluster")
+        ins("fence.proxy.async.shared::cta")
+        place(skip)
+        # TMEM: warp 1 of both CTAs allocates the pair's 2 x BN accumulator columns
+        noalloc = lab("mp_noalloc")
+        ins(f"setp.ne.u32 {p}, {warp}, 1")
+        ins(f"@{p} bra {noalloc}")
+        slot = t("b32")
+        ins(f"add.u32 {slot}, {bars}, {slot_off}")
+        ins(f"tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [{slot}], {self.tmem_cols}")
+        ins("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned")
+        place(noalloc)
+        ins("tcgen05.fence::before_thread_sync")
+        ins("bar.sync 0")
+        # both CTAs' barriers are initialised before either signals the other's
+        ins("barrier.cluster.arrive.release")
+        ins("barrier.cluster.wait.acquire")
+        ins("tcgen05.fence::after_thread_sync")
+
+    def check_maps(self, end: str) -> None:
+        """Hook: every thread, before the first access to global data."""
+
+    @property
+    def tmem_cols(self) -> int:
+        return 512 if 2 * self.BN > 256 else 256
 
     # ---- the tuned body -------------------------------------------------------------
 
@@ -199,37 +242,7 @@ class TcMatmulPair(TcMatmul):
         empty_off, accf_off, acce_off, slot_off = 8 * ST, 16 * ST, 16 * ST + 16, 16 * ST + 32
         tail_done_off, tail_last_off, tail_flag_off = 16 * ST + 40, 16 * ST + 48, 16 * ST + 56
         p = t("pred")
-        skip = lab("mp_noinit")
-        ins(f"setp.ne.u32 {p}, {tid}, 0")
-        ins(f"@{p} bra {skip}")
-        for s in range(ST):
-            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{8 * s}], 1")
-            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{empty_off + 8 * s}], 1")
-        for b in range(2):
-            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{accf_off + 8 * b}], 1")
-            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{acce_off + 8 * b}], {2 * EPI_WARPS}")
-        if self.rem:
-            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{tail_done_off}], {32 * EPI_WARPS}")
-            ins(f"mbarrier.init.shared::cta.b64 [{bars}+{tail_last_off}], 1")
-        ins("fence.mbarrier_init.release.cluster")
-        ins("fence.proxy.async.shared::cta")
-        place(skip)
-        # TMEM: warp 1 of both CTAs allocates the pair's 2 x BN accumulator columns
-        tmem_cols = 512 if 2 * BN > 256 else 256
-        noalloc = lab("mp_noalloc")
-        ins(f"setp.ne.u32 {p}, {warp}, 1")
-        ins(f"@{p} bra {noalloc}")
-        slot = t("b32")
-        ins(f"add.u32 {slot}, {bars}, {slot_off}")
-        ins(f"tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [{slot}], {tmem_cols}")
-        ins("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned")
-        place(noalloc)
-        ins("tcgen05.fence::before_thread_sync")
-        ins("bar.sync 0")
-        # both CTAs' barriers are initialised before either signals the other's
-        ins("barrier.cluster.arrive.release")
-        ins("barrier.cluster.wait.acquire")
-        ins("tcgen05.fence::after_thread_sync")
+        self.set_up(bars, warp, tid, empty_off, accf_off, acce_off, slot_off, tail_done_off, tail_last_off, p)
         # barriers and TMEM are set up while the stream's previous kernel may still run; from
         # here on the pair reads and writes global data
         self.pdl_wait()
@@ -247,6 +260,7 @@ class TcMatmulPair(TcMatmul):
         errp = t("b64")
         ins(f"mov.u64 {errp}, thc_error")
         end = lab("mp_end")
+        self.check_maps(end)
         kit = Kit(em, errp, end)
 
         def decode(tile: str):
@@ -579,7 +593,7 @@ class TcMatmulPair(TcMatmul):
         ins(f"setp.ne.u32 {p}, {warp}, 1")
         ins(f"@{p} bra {nod}")
         ins("tcgen05.fence::after_thread_sync")
-        ins(f"tcgen05.dealloc.cta_group::2.sync.aligned.b32 {tmem}, {tmem_cols}")
+        ins(f"tcgen05.dealloc.cta_group::2.sync.aligned.b32 {tmem}, {self.tmem_cols}")
         place(nod)
 
 

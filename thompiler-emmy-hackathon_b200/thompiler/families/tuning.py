@@ -27,7 +27,7 @@ class Tuning:
     # CTA-pair kernel: a partial last wave whose tiles, halved, fit one wave of pairs has its
     # 256-wide tiles cut along N into two 256 x 128 units (else, or when False, the K split)
     matmul_half_tail: bool = True
-    # fused linear products: "stream", "rows" or "pair" forces that kernel where it can run ("": by estimate)
+    # fused linear products: "stream", "rows", "split" or "pair" forces that kernel where it can run ("": by estimate)
     linear_kernel: str = ""
     # programmatic dependent launch: tuned bodies signal griddepcontrol.launch_dependents and wait
     # (griddepcontrol.wait) before global accesses, and their launches may overlap the previous kernel
