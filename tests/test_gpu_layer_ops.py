@@ -95,6 +95,43 @@ def test_linear(tmp_path, monkeypatch, case, launch):
     k.close()
 
 
+# sizes whose last wave of tiles is cut: (whole strips of tiles or -1, tiles in halves, width of the units)
+TAILS = [((1119, 5632, 136, "bf16", "bf16", False, "relu", True, False), (-1, 36, 128)),
+         ((1119, 5592, 264, "bf16", "bf16", True, None, True, False), (-1, 36, 128)),
+         ((1285, 4656, 264, "f16", "f16", True, "silu", True, False), (10, 0, 192)),
+         ((1302, 4784, 136, "bf16", "f32", False, None, True, False), (12, 0, 192)),
+         ((2338, 3592, 72, "f16", "f16", False, None, False, False), (7, 0, 128)),
+         ((258, 4832, 200, "bf16", "bf16", True, "silu", True, True), (-1, 2, 128)),
+         ((264, 4800, 200, "f16", "f16", False, "gelu_tanh", False, True), (37, 0, 128)),
+         ((259, 4912, 136, "bf16", "f32", True, "silu", False, True), (0, 0, 192)),
+         ((200, 1000, 136, "f16", "f16", False, "silu", True, True), (0, 0, 128)),
+         ((1285, 4656, 16384, "bf16", "bf16", True, None, True, False), (10, 0, 192))]      # in bands of four rows
+
+
+@pytest.mark.parametrize("case,cut", TAILS, ids=str)
+def test_pair_tails(tmp_path, monkeypatch, case, cut):
+    import torch
+    from thompiler.families.linear import LinearPair, Product
+    from thompiler.load import load
+    monkeypatch.setattr(TUNING, "linear_kernel", "pair")
+    d = synth.linear_package(tmp_path, *case)
+    assert min(LinearPair.plans(Product.read(load(next(d.glob("*.ir.json"))))))[3:] == cut
+    k = _kernel(d, "own")
+    _family(k, "pair")
+    M, N = case[:2]
+    t = _linear_inputs(case)
+    whole, y = _out((M, N), case[4])
+    k({n: v.data_ptr() for n, v in dict(t, linear=y).items()}, _stream())
+    torch.cuda.synchronize()
+    assert k.error_word() == 0
+    _untouched(whole)
+    rows = sorted(r for r in {0, 127, 128, 255, 256, M - 1, *range(0, M, 61), *range(max(0, M - 130), M, 17)} if r < M)
+    some = {n: v[rows] if n in ("x", "res") else v for n, v in t.items()}
+    _linear_check((len(rows), *case[1:]), some, y[rows], f"{cut}")
+    assert bool(y.float().isfinite().all())
+    k.close()
+
+
 @pytest.mark.parametrize("kernel", ["generic", "stream", "rows", "split", "pair"])
 @pytest.mark.parametrize("M,N,K", [(20, 200, 264), (32, 64, 64), (600, 328, 200)])
 def test_custom_epilogue(tmp_path, monkeypatch, kernel, M, N, K):

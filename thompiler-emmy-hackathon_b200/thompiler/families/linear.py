@@ -19,15 +19,20 @@ waited for; bound by the tensor cores while K is above about a thousand.
 
 from __future__ import annotations
 
+from math import gcd
+
 from thompiler import ir, schedules
 from thompiler.families.base import TunedKernel
 from thompiler.families.kit import (Kit, declare_tmap_ring, desc_hi, elect_one, idesc_f16, load_tmap_table,
                                     match_tmap_set)
 from thompiler.families.matmul import BK, BM, EPI_WARPS, SM_COUNT, STAGE_TILE, THREADS
-from thompiler.families.matmul_pair import PAIR_SLOTS, PAIR_WIDTHS, PM, SMEM_LIMIT, TcMatmulPair
+from thompiler.families.matmul_pair import PAIR_SLOTS, PM, SMEM_LIMIT, TcMatmulPair
 from thompiler.families.tuning import TUNING
 from thompiler.load import KernelInfo
 from thompiler.lowering.types import BF16, F16, F32, Ty
+
+
+TILE_TIMES = ((256, 1.0), (192, 0.79), (128, 0.65))      # of a pair's tile widths, of the widest's
 
 
 class Product:
@@ -190,7 +195,7 @@ class LinearPair(TcMatmulPair):
         self.a, self.b, self.c = p.x, p.w, p.c
         self.M, self.N, self.K, self.S, self.Ks = p.M, p.N, p.K, 1, p.K
         self.b_kmajor, self.static_smem = True, p.static_smem
-        _, self.BN, self.hrem = min(self.plans(p))
+        _, _, self.BN, strips, self.hrem, self.tail_cols = min(self.plans(p))
         self.HN = self.BN // 2
         self.a_bytes, self.b_bytes = BM * BK * 2, self.HN * BK * 2
         stage = self.a_bytes + self.b_bytes
@@ -202,10 +207,15 @@ class LinearPair(TcMatmulPair):
         self.rank_cols = p.N if p.gated else self.HN
         self.tiles_m, self.tiles_n = -(-p.M // PM), -(-p.N // self.tile_cols)
         self.kblocks = -(-p.K // BK)
-        self.tiles = self.tiles_m * self.tiles_n
         self.rem, self.parts = 0, 1                  # no K split: its partials would pass the epilogue twice
-        self.full_tiles = self.tiles - self.hrem
+        self.full_tiles = self.tiles_m * self.tiles_n - self.hrem
         self.units = self.full_tiles + 2 * self.hrem
+        if self.tail_cols:
+            self.b_box = gcd(self.HN, self.tail_cols // 2)
+        if strips >= 0:
+            self.strips, self.tiles_n = strips, max(1, strips)
+            self.full_tiles = self.tiles_m * strips
+            self.units = self.full_tiles + self.tiles_m * -(-(p.N - strips * self.tile_cols) // self.tail_out())
         self.pairs = min(self.units, PAIR_SLOTS)
         self.ctas = 2 * self.pairs
         # tiles are walked in bands of as many rows as keep a band's x within 32 MB, so that it stays in L2 (two
@@ -216,20 +226,44 @@ class LinearPair(TcMatmulPair):
         self.band = band if self.tiles_m > band else 0
         self.replay = Replay(self, p) if p.epilogue is not None else None
 
+    def tail_out(self) -> int:
+        return self.tail_cols // 2 if self.p.gated else self.tail_cols
+
+    def tail_rank_cols(self) -> int:
+        return self.rank_cols if self.p.gated else self.tail_cols // 2
+
     @staticmethod
-    def plans(p: Product) -> list[tuple[float, int, int]]:
-        """(waves of a 256-wide tile's time, width, halved tiles) of each tile width: the tiles a
-        pair runs in a row, each as long as its width at that width's measured efficiency; a last
-        wave whose tiles halved fit one wave runs as halves, which take 0.7 of a whole."""
-        out = []
-        for bn, pref in PAIR_WIDTHS:
+    def plans(p: Product) -> list[tuple]:
+        """(time, work, width, whole strips of tiles or -1, tiles in halves, width of the tail's units) of each
+        way to cut C, time and work in units of a 256-wide tile's: of the pair that runs most and in all.
+        A last wave that would fill badly takes narrower units: two to each of its tiles, or strips of columns
+        after the whole ones.  Us of as many units of 256, 192 and 128 columns, 2048 x 2304 W x 4096, W = 1 and
+        3 waves: 27.7 and 75.0, 22.0 and 58.7, 18.1 and 47.0."""
+        out, G = [], 2 if p.gated else 1
+        rows = -(-p.M // PM)
+
+        def busiest(full: int, units: int, cost: float) -> float:
+            """Unit u runs on pair u mod PAIR_SLOTS; the first ``full`` are whole tiles."""
+            whole = [-(-max(full - i, 0) // PAIR_SLOTS) for i in range(PAIR_SLOTS)]
+            return max(w + cost * (-(-max(units - i, 0) // PAIR_SLOTS) - w) for i, w in enumerate(whole))
+
+        for bn, cost in TILE_TIMES:
             if p.gated and bn != 256:
                 continue
-            tiles = -(-p.M // PM) * -(-p.N // (bn // 2 if p.gated else bn))
-            waves, rem = divmod(tiles, PAIR_SLOTS)
-            half = waves and rem and 2 * rem <= PAIR_SLOTS and bn == 256 and not p.gated and TUNING.matmul_half_tail
-            time = waves + (0 if not rem else 0.7 if half else 1)
-            out.append((time * bn / 256 / pref, bn, rem if half else 0))
+            strips = -(-p.N // (bn // G))
+            tiles = rows * strips
+            out.append((-(-tiles // PAIR_SLOTS) * cost, tiles * cost, bn, -1, 0, 0))
+            if bn != 256 or tiles <= PAIR_SLOTS and not p.gated or not TUNING.matmul_half_tail:
+                continue
+            for width, cost in TILE_TIMES[1:]:
+                if width // G % (128 // p.c.ty.nbytes):      # stores go in pairs of 64-byte boxes
+                    continue
+                rem = tiles % PAIR_SLOTS
+                if width == 128 and rem and tiles > PAIR_SLOTS:
+                    out.append((busiest(tiles - rem, tiles + rem, cost), tiles - rem + 2 * rem * cost, bn, -1, rem, width))
+                for a in range(max(0, strips - 2 - 2 * PAIR_SLOTS // rows), strips):
+                    full, tail = rows * a, rows * -(-(p.N - a * (bn // G)) // (width // G))
+                    out.append((busiest(full, full + tail, cost), full + tail * cost, bn, a, 0, width))
         return out
 
     def estimate(self) -> float:
@@ -331,15 +365,15 @@ class LinearPair(TcMatmulPair):
         ins(f"mad.lo.u32 {self.row}, {tm}, {PM}, {row}")
         ins(f"mad.lo.u32 {self.row}, {rank}, {BM}, {self.row}")
         ins(f"mul.lo.u32 {self.col}, {tn}, {self.tile_cols}")
-        if self.hrem:
-            ins(f"@!{whole} mad.lo.u32 {self.col}, {part}, {self.BN // 2}, {self.col}")
+        if self.tail_cols:
+            ins(f"@!{whole} mad.lo.u32 {self.col}, {part}, {self.tail_out()}, {self.col}")
         if self.offset:
             ins(f"add.u32 {self.col}, {self.col}, {self.offset}")
         self.row_ok = self.left = None
         if p.M % PM:
             self.row_ok = t("pred")
             ins(f"setp.lt.u32 {self.row_ok}, {self.row}, {p.M}")
-        if p.N % self.tile_cols:
+        if p.N % self.tile_cols or self.strips is not None and (p.N - self.strips * self.tile_cols) % self.tail_out():
             self.left = t("b32")                     # columns from the tile's first one to N
             ins(f"sub.s32 {self.left}, {p.N}, {self.col}")
         self.at = {}
@@ -403,7 +437,7 @@ class LinearPair(TcMatmulPair):
         for b in (0, 1):
             def values(b=b):
                 nonlocal now
-                sums = self._sums(ta, b * cw, cw)
+                sums = self._sums(ta, b * cw, cw, width)
                 if b == 0:
                     following = self._fetch(cw, cw)
                 else:
@@ -425,9 +459,9 @@ class LinearPair(TcMatmulPair):
         ins(f"add.u32 {i}, {i}, 1")
         ins(f"@{more} bra {top}")
 
-    def _sums(self, taddr: str, c0: int, cw: int) -> list[list[str]]:
+    def _sums(self, taddr: str, c0: int, cw: int, width: int) -> list[list[str]]:
         em, out = self.em, []
-        for base in (c0, c0 + self.HN) if self.p.gated else (c0,):
+        for base in (c0, c0 + width) if self.p.gated else (c0,):
             v, a = em.tmps("b32", cw), em.tmp("b32")
             em.ins(f"add.u32 {a}, {taddr}, {base}")
             em.ins(f"tcgen05.ld.sync.aligned.32x32b.x{cw}.b32 {{{', '.join(v)}}}, [{a}]")

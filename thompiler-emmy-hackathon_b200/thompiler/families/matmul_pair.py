@@ -48,6 +48,9 @@ SMEM_LIMIT = 227 * 1024
 class TcMatmulPair(TcMatmul):
     family = "tcgen05-matmul-pair"
     tail_ranks = 2
+    # a cut tail: the columns of a unit (0: half a tile), the strip of tiles that it begins with (None: the last
+    # ``hrem`` tiles, each in two), and the rows of B that a load takes (0: a CTA's share of a tile)
+    tail_cols, strips, b_box = 0, None, 0
     epilogue = None              # a RegStore epilogue to apply (thompiler.families.linear)
     band = 0                     # rows of tiles walked together (0: all of them, column by column)
 
@@ -132,7 +135,7 @@ class TcMatmulPair(TcMatmul):
         a, b = self.a, self.b
         side["tmaps"][0]["box"] = [BK, BM]
         if self.b_kmajor:
-            side["tmaps"][1]["box"] = [BK, self.HN]
+            side["tmaps"][1]["box"] = [BK, self.b_box or self.HN]
         side["grid"] = [self.ctas, 1, 1]
         side["cluster"] = [2, 1, 1]
         side["tile"] = [PM, self.BN, BK]
@@ -208,6 +211,14 @@ class TcMatmulPair(TcMatmul):
 
     def check_maps(self, end: str) -> None:
         """Hook: every thread, before the first access to global data."""
+
+    def tail_out(self) -> int:
+        """Columns of C in a unit of a cut tail."""
+        return self.tail_cols or self.BN // 2
+
+    def tail_rank_cols(self) -> int:
+        """Rows of B between the CTAs of a pair in such a unit."""
+        return self.tail_out() // 2
 
     @property
     def tmem_cols(self) -> int:
@@ -294,12 +305,26 @@ class TcMatmulPair(TcMatmul):
                 ins(f"@!{whole} div.u32 {lo}, {lo}, {parts}")
                 ins(f"@!{whole} mad.lo.u32 {hi_}, {part}, {kblocks}, {kblocks}")
                 ins(f"@!{whole} div.u32 {hi_}, {hi_}, {parts}")
-            if self.hrem:
+            if self.strips is not None:          # (row of tiles, column in units) of the tail
+                ins(f"sub.u32 {v}, {u}, {full_tiles}")
+                ins(f"@!{whole} rem.u32 {tile_}, {v}, {tiles_m}")
+                ins(f"@!{whole} div.u32 {part}, {v}, {tiles_m}")
+            elif self.hrem:
                 ins(f"sub.u32 {v}, {u}, {full_tiles}")
                 ins(f"@!{whole} shr.u32 {tile_}, {v}, 1")
                 ins(f"@!{whole} add.u32 {tile_}, {tile_}, {full_tiles}")
                 ins(f"@!{whole} and.b32 {part}, {v}, 1")
             return tile_, lo, hi_, whole, part
+
+        cut = self.hrem or self.strips is not None
+        tail_cols = self.tail_cols or BN // 2
+
+        def placed(tile: str, whole: str):
+            tm_, tn_, ts_ = decode(tile)
+            if self.strips is not None:
+                ins(f"@!{whole} mov.u32 {tm_}, {tile}")
+                ins(f"@!{whole} mov.u32 {tn_}, {self.strips}")
+            return tm_, tn_, ts_
 
         role_mma, role_epi = lab("mp_mma"), lab("mp_epi")
         ins(f"setp.eq.u32 {p}, {warp}, 1")
@@ -319,19 +344,19 @@ class TcMatmulPair(TcMatmul):
         ins(f"@{p} bra {end}")
         place(ptop)
         ptile, kb, kend, pwhole, ppart = unit(pu)
-        tm_, tn_, ts_ = decode(ptile)
+        tm_, tn_, ts_ = placed(ptile, pwhole)
         m0, n0, k0 = t("b32"), t("b32"), t("b32")
         ins(f"mul.lo.u32 {m0}, {tm_}, {PM}")
         ins(f"mad.lo.u32 {m0}, {rank}, {BM}, {m0}")
         ins(f"mul.lo.u32 {n0}, {tn_}, {self.tile_cols}")
-        if self.hrem:
+        if cut:
             # half unit h: columns 128 h .. of the tile, 64 per CTA; the box still spans 128 rows
-            # (the second 64 are not read; past N they are the tensor map's zero fill)
+            # (the second 64 are not read; past N they are the tensor map's zero fill) unless b_box divides them
             nh = t("b32")
-            ins(f"mad.lo.u32 {nh}, {ppart}, {BN // 2}, {n0}")
-            ins(f"mad.lo.u32 {nh}, {rank}, {HN // 2}, {nh}")
+            ins(f"mad.lo.u32 {nh}, {ppart}, {self.tail_out()}, {n0}")
+            ins(f"mad.lo.u32 {nh}, {rank}, {self.tail_rank_cols()}, {nh}")
         ins(f"mad.lo.u32 {n0}, {rank}, {self.rank_cols}, {n0}")
-        if self.hrem:
+        if cut:
             ins(f"@!{pwhole} mov.u32 {n0}, {nh}")
         ins(f"mul.lo.u32 {k0}, {ts_}, {self.Ks}")
         ktop = lab("mp_prod_k")
@@ -345,9 +370,22 @@ class TcMatmulPair(TcMatmul):
         ins(f"mad.lo.u32 {sa}, {stage}, {a_bytes}, {a_st}")
         ins(f"mad.lo.u32 {sb}, {stage}, {b_bytes}, {b_st}")
         ins(f"mad.lo.u32 {kc}, {kb}, {BK}, {k0}")
-        ins(f"@{post} mbarrier.arrive.expect_tx.shared::cta.b64 _, [{eb}], {2 * (a_bytes + b_bytes)}")
+        if self.b_box:                                   # a unit's own rows of B, b_box a load
+            expect = t("b32")
+            ins(f"selp.u32 {expect}, {2 * (a_bytes + b_bytes)}, {2 * (a_bytes + tail_cols * BK)}, {pwhole}")
+            ins(f"@{post} mbarrier.arrive.expect_tx.shared::cta.b64 _, [{eb}], {expect}")
+        else:
+            ins(f"@{post} mbarrier.arrive.expect_tx.shared::cta.b64 _, [{eb}], {2 * (a_bytes + b_bytes)}")
         ins(f"@{is0} {tma_ld} [{sa}], [{tma}, {{{kc}, {m0}}}], [{fb}]")
-        if self.b_kmajor:
+        if self.b_box:
+            for nb in range(0, HN, self.b_box):
+                when, nn = is0, t("b32")
+                if nb >= tail_cols // 2:
+                    when = t("pred")
+                    ins(f"and.pred {when}, {is0}, {pwhole}")
+                ins(f"add.u32 {nn}, {n0}, {nb}")
+                ins(f"@{when} {tma_ld} [{sb}+{nb * BK * 2}], [{tmb}, {{{kc}, {nn}}}], [{fb}]")
+        elif self.b_kmajor:
             ins(f"@{is0} {tma_ld} [{sb}], [{tmb}, {{{kc}, {n0}}}], [{fb}]")
         else:
             for nb in range(HN // 64):
@@ -389,8 +427,8 @@ class TcMatmulPair(TcMatmul):
         _, kb2, kend2, mwhole, _ = unit(mu)
         idr = t("b32")
         ins(f"mov.u32 {idr}, {idesc}")
-        if self.hrem:
-            ins(f"@!{mwhole} mov.u32 {idr}, {idesc_f16(PM, BN // 2, b_mn_major=not self.b_kmajor, bf16=bf16)}")
+        if cut:
+            ins(f"@!{mwhole} mov.u32 {idr}, {idesc_f16(PM, tail_cols, b_mn_major=not self.b_kmajor, bf16=bf16)}")
         kfirst = t("b32")
         ins(f"mov.u32 {kfirst}, {kb2}")
         buf, ab = t("b32"), t("b32")
@@ -467,7 +505,7 @@ class TcMatmulPair(TcMatmul):
         ins(f"@{p} bra {edone}")
         place(etop)
         tile3, _, _, whole3, part3 = unit(eu)
-        tm3, tn3, ts3 = decode(tile3)
+        tm3, tn3, ts3 = placed(tile3, whole3)
         self.tile_begin(row, rank, tm3, tn3, whole3, part3)
         buf3, ab3, lab3 = t("b32"), t("b32"), t("b32")
         ins(f"and.b32 {buf3}, {lt3}, 1")
@@ -562,15 +600,15 @@ class TcMatmulPair(TcMatmul):
             return v
 
         tail = lab("mp_epi_tail")
-        if self.rem or self.hrem:
+        if self.rem or cut:
             ins(f"@!{whole3} bra {tail}")
         store(self.tile_cols)
-        if self.hrem:
+        if cut:
             # a half unit: 128 columns of the tile, starting at 128 h
             ins(f"bra {enext}")
             place(tail)
-            ins(f"mad.lo.u32 {col0}, {part3}, {BN // 2}, {col0}")
-            store(BN // 2)
+            ins(f"mad.lo.u32 {col0}, {part3}, {self.tail_out()}, {col0}")
+            store(self.tail_out())
         if self.rem:
             ins(f"bra {enext}")
             self._pair_tail(tail, enext, tile3, part3, rank, taddr, row, bars, ls, store_boxes, free_accumulator,
