@@ -44,6 +44,8 @@ class Product:
         self.M, self.K = self.x.shape
         self.N = self.c.shape[1]
         self.gated, self.epilogue = gated, epilogue
+        # log2 of the 16-byte pieces that every row of x and w starts on: 3 where rows are whole 128-byte lines
+        self.pieces = min(3, ((self.K * 2 // 16) & -(self.K * 2 // 16)).bit_length() - 1)
         # the generic path's slabs, where they are static arrays of their own
         self.static_smem = 0 if kernel.dynamic_smem_bytes else (3 if gated else 2) * 64 * 64 * 2
 
@@ -268,10 +270,11 @@ class LinearPair(TcMatmulPair):
 
     def estimate(self) -> float:
         """Microseconds (``choose`` says how the constants came about)."""
-        waves = min(self.plans(self.p))[0]
-        block = 0.263 * (1 + 0.226 * self.ctas / SM_COUNT)
-        fixed = 5.35 * min(waves, 1) + 0.96 * max(waves - 1, 0)          # later epilogues run under the next MMAs
-        return ((self.p.w.nbytes / 6.55e6) ** 4 + (waves * self.kblocks * block) ** 4) ** 0.25 + fixed
+        waves, g = min(self.plans(self.p))[0], int(self.p.gated)
+        block = 0.273 * (1 + 0.25 * self.ctas / SM_COUNT) * (1.4, 1.05, 1.05, 1)[self.p.pieces]
+        later = max(waves - 1, 0)                    # whose epilogues run under the next MMAs
+        return (2.27 + 1.71 * g + 2.47 * min(waves, 1) + (0.5 + 0.61 * g) * later
+                + ((self.p.w.nbytes / 6.64e6) ** 4 + (waves * self.kblocks * block) ** 4) ** 0.25)
 
     def guard(self, generic: str) -> None:
         self.guard_launch(generic, THREADS, 2)
@@ -1065,8 +1068,9 @@ class RowsPlan:
         self.exchange = self.G * BT * BM * 4 if S > 1 else 0
         self.tmem_cols = max(32, 1 << (self.G * BT - 1).bit_length())
         # two CTAs an SM where the launch has more than one for each, or clusters so large that the SMs of a
-        # processing cluster do not divide into them
-        half = self.ctas > SM_COUNT or S == 8
+        # processing cluster do not divide into them: of clusters of four, one CTA an SM, 33 are resident at
+        # once, and a launch of 34 takes twice as long (64 x 4352 x 4096: 14.1 us, 64 x 4224 x 4096 8.3)
+        half = self.ctas > (SM_COUNT if S < 4 else 128) or S == 8
         room = (SMEM_LIMIT // 2 - 1024 if half else SMEM_LIMIT) - self.exchange - 1024 - 256 - p.static_smem
         self.stages = min(12, -(-self.kblocks // S) + 1, room // self.stage_bytes)
         self.smem = self.stages * self.stage_bytes + self.exchange + 1024 + 256
@@ -1078,8 +1082,9 @@ class RowsPlan:
     @property
     def possible(self) -> bool:
         return (self.stages >= 2 and self.S <= self.kblocks and self.exchange <= EXCHANGE_LIMIT
-                and self.G * self.BT <= 512 and self.ctas <= (SM_COUNT if self.smem > SMEM_LIMIT // 2 - 1024
-                                                              else 2 * SM_COUNT))
+                and self.G * self.BT <= 512
+                and self.ctas <= (2 * SM_COUNT if self.smem <= SMEM_LIMIT // 2 - 1024 else
+                                  SM_COUNT if self.S < 4 else 128))
 
     @classmethod
     def best(cls, p: Product) -> "RowsPlan | None":
@@ -1098,16 +1103,20 @@ class RowsPlan:
         return min(out, key=lambda x: x[:3])[3] if out else None
 
     def estimate(self, p: Product) -> float:
-        """Microseconds.  Reading w once from memory, and an SM's slabs through its copies (78 bytes a cycle,
-        less as more SMs copy) or tensor cores, overlap in part (the power mean); then the join of a cut
-        K and the epilogue, by the tokens a CTA holds."""
-        load = self.ctas / SM_COUNT
+        """Microseconds.  Reading w once from memory, and an SM's slabs through its copies (77 bytes a cycle,
+        less where rows straddle lines -- 256 x 4096 x 2048, 2080, 2064 and 2056 take 7.8, 8.4, 9.2 and
+        12.6 us, the split kernel 7.7, 7.9, 8.0 and 9.5 -- and where few stages are in flight) or tensor
+        cores, overlap in part (the power mean); then the join of a cut K (large clusters wait for SMs
+        that belong together) and the epilogue, by the tokens a CTA holds."""
         per_sm = -(-self.ctas // SM_COUNT)
-        block = max(self.stage_bytes / 78 * (1 + 0.12 * load / per_sm), 0.93 * self.BT * self.G) / 1900
-        memory, sm = p.w.nbytes / 7.6e6, per_sm * -(-self.kblocks // self.S) * block
+        blocks = -(-self.kblocks // self.S)
+        block = max(self.stage_bytes / 77.4 * (1.85, 1.25, 1.14, 1)[p.pieces], 1.385 * self.BT * self.G)
+        if blocks > self.stages:
+            block = max(block, 1142 / self.stages)
+        memory, sm = p.w.nbytes / 8.28e6, per_sm * blocks * block / 1900
         tokens = self.BT * self.G / 100
-        join = (0.28 + 1.18 * tokens if self.S > 1 else 0) + (1.12 if self.S == 8 else 0)
-        return 2.09 + (memory ** 1.95 + sm ** 1.95) ** (1 / 1.95) + join + 0.63 * tokens * per_sm / self.S
+        join = (0.34 + 0.89 * tokens if self.S > 1 else 0) + (1.86 if self.S == 8 and self.ctas >= 112 else 0)
+        return 2.16 + (memory ** 1.73 + sm ** 1.73) ** (1 / 1.73) + join + 0.66 * tokens * per_sm / self.S
 
 
 class LinearStream(ByElement):
@@ -1360,9 +1369,9 @@ class StreamPlan:
     def estimate(self, p: Product) -> float:
         """Microseconds: w from memory, or the turns of the CTAs resident at once; past eight tokens x takes
         as many loads as w."""
-        turns = -(-self.ctas // (2 * SM_COUNT)) * p.K * self.G * 0.63e-3
-        more = p.w.nbytes * (self.NT - 1) * 0.056e-6
-        return 1.5 + ((p.w.nbytes / 6.7e6) ** 4 + turns ** 4) ** 0.25 + more
+        turns = -(-self.ctas // (2 * SM_COUNT)) * p.K * self.G * 0.534e-3 * (1 + 0.36 * (self.NT - 1))
+        more = p.w.nbytes * (self.NT - 1) * 0.046e-6
+        return 1.53 + ((p.w.nbytes / 6.46e6) ** 4 + turns ** 4) ** 0.25 + more
 
 
 def choose(p: Product) -> TunedKernel:
@@ -1370,9 +1379,9 @@ def choose(p: Product) -> TunedKernel:
 
     The estimates' forms follow what bounds each kernel; their constants are least-squares fits (of log
     time) to 1,745 timings on a B200 of every plan at M = 1 .. 1024, (N, K) from 512 x 512 to 8192 x 8192,
-    plain and gated, back to back in graphs.  Over those 251 sizes the choice costs 1.5 % against the best
-    plan on average and 32 % at worst; over 44 sizes drawn at random (M 24 .. 2513, ragged) it missed the
-    fastest kernel five times, by 3 to 22 %.  Some of all sides, in us (stream / rows / split / pair):
+    plain and gated, back to back in graphs.  Over those 251 sizes the choice costs 1.2 % against the best
+    plan on average and 20 % at worst; over 60 others drawn at random (M 23 .. 2400, ragged N and K) against
+    the fastest kernel 1.2 % and 30 %.  Some of all sides, in us (stream / rows / split / pair):
     1 x 512 x 512 1.7 / 2.5 / - / 5.3; 1 x 4096 x 4096 6.1 / 6.8 / - / 21; 16 x 4096 x 4096 7.7 / 7.0 / - / 17;
     128 x 4096 x 4096 - / 10.3 / 12.0 / 16.5; 512 x 4096 x 8192 - / 32.1 / 28.4 / 31.4; 835 x 440 x 4048 gated
     - / 29.8 / 11.8 / 24.2; 1024 x 4096 x 4096 - / 28.8 / - / 26.3; 2048 x 4096 x 4096 - / - / - / 51."""

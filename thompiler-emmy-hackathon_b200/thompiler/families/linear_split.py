@@ -69,7 +69,7 @@ class SplitPlan:
     def estimate(self, p: Product) -> float:
         """Microseconds: w from memory, or the K blocks of a pair (slower as more SMs draw on L2); then the
         launch, the exchange and the epilogue."""
-        block = (0.249 if self.BN == 256 else 0.16) * (1 + 0.44 * self.ctas / 128)
+        block = (0.249 if self.BN == 256 else 0.16) * (1 + 0.44 * self.ctas / 128) * (1.25, 1.05, 1.05, 1)[p.pieces]
         blocks = self.kblocks - self.kblocks // 2
         return 2.7 + 2.8 * self.BN / 256 + ((p.w.nbytes / 7.1e6) ** 4 + (blocks * block) ** 4) ** 0.25
 
