@@ -1116,7 +1116,8 @@ class RowsPlan:
         memory, sm = p.w.nbytes / 8.28e6, per_sm * blocks * block / 1900
         tokens = self.BT * self.G / 100
         join = (0.34 + 0.89 * tokens if self.S > 1 else 0) + (1.86 if self.S == 8 and self.ctas >= 112 else 0)
-        return 2.16 + (memory ** 1.73 + sm ** 1.73) ** (1 / 1.73) + join + 0.66 * tokens * per_sm / self.S
+        epilogue = (0.66 * tokens + 1.2 * max(0, tokens - 1.28)) * per_sm / self.S
+        return 2.16 + (memory ** 1.73 + sm ** 1.73) ** (1 / 1.73) + join + epilogue
 
 
 class LinearStream(ByElement):
@@ -1379,7 +1380,7 @@ def choose(p: Product) -> TunedKernel:
 
     The estimates' forms follow what bounds each kernel; their constants are least-squares fits (of log
     time) to 1,745 timings on a B200 of every plan at M = 1 .. 1024, (N, K) from 512 x 512 to 8192 x 8192,
-    plain and gated, back to back in graphs.  Over those 251 sizes the choice costs 1.2 % against the best
+    plain and gated, back to back in graphs.  Over those 251 sizes the choice costs 1.0 % against the best
     plan on average and 20 % at worst; over 60 others drawn at random (M 23 .. 2400, ragged N and K) against
     the fastest kernel 1.2 % and 30 %.  Some of all sides, in us (stream / rows / split / pair):
     1 x 512 x 512 1.7 / 2.5 / - / 5.3; 1 x 4096 x 4096 6.1 / 6.8 / - / 21; 16 x 4096 x 4096 7.7 / 7.0 / - / 17;

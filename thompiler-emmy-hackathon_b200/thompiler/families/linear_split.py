@@ -10,7 +10,7 @@ epilogue) are both half as long, for one exchange:
 
   the CTAs meet when both pairs' last MMA is done (the stages are free), send, and meet again.
 
-512 x 4096 x 8192 bf16 on 128 SMs: 28.5 us, ``LinearPair`` with 256 x 128 tiles on as many 31.1: each
+512 x 4096 x 8192 bf16 on 128 SMs: 28.5 us, ``LinearPair`` with 256 x 128 tiles on as many 31.4: each
 SM reads 24 KB a K block there for 256 cycles of MMAs, more than L2 delivers, where a 256 x 256
 tile reads 32 KB for 512.  The exchange is bound by the SMs' network: 64 KB a CTA take 4,050 cycles,
 2.1 us, as 128-byte and as 512-byte stores.  Clusters of eight (K in four) are slower everywhere:
@@ -56,8 +56,8 @@ class SplitPlan:
 
     @property
     def possible(self) -> bool:
-        """Two K blocks, a store's columns for each pair, and every cluster resident at once: 32 are, 36 take
-        twice as long (512 x 4608 x 4096: 31 us, 512 x 4096 x 4096 16.8)."""
+        """Two K blocks, a store's columns for each pair, and every cluster resident at once: 32 are (33 on the
+        GPU measured), 34 take twice as long (256 x 8704 x 2048: 22.2 us, 256 x 8192 x 2048 12.6)."""
         return self.own >= self.box and self.kblocks >= 2 and self.stages >= 6 and self.ctas <= 128
 
     @classmethod
