@@ -129,6 +129,18 @@ LINEAR = [
     (1300, 264, 16384, "bf16", "bf16", True, None, True, False),       # bands of four and of two rows of tiles
 ]
 
+# sizes whose last wave of tiles is cut: (whole strips of tiles or -1, tiles in halves, width of the units)
+TAILS = [((1119, 5632, 136, "bf16", "bf16", False, "relu", True, False), (-1, 36, 128)),
+         ((1119, 5592, 264, "bf16", "bf16", True, None, True, False), (-1, 36, 128)),
+         ((1285, 4656, 264, "f16", "f16", True, "silu", True, False), (10, 0, 192)),
+         ((1302, 4784, 136, "bf16", "f32", False, None, True, False), (12, 0, 192)),
+         ((2338, 3592, 72, "f16", "f16", False, None, False, False), (7, 0, 128)),
+         ((258, 4832, 200, "bf16", "bf16", True, "silu", True, True), (-1, 2, 128)),
+         ((264, 4800, 200, "f16", "f16", False, "gelu_tanh", False, True), (37, 0, 128)),
+         ((259, 4912, 136, "bf16", "f32", True, "silu", False, True), (0, 0, 192)),
+         ((200, 1000, 136, "f16", "f16", False, "silu", True, True), (0, 0, 128)),
+         ((1285, 4656, 16384, "bf16", "bf16", True, None, True, False), (10, 0, 192))]      # in bands of four rows
+
 # (B, S, heads, kv, D, R, dtype, interleaved, values, heads_first, inverse, norm)
 HEADS = [
     (1, 1, 1, 0, 2, 2, "f32", False, False, False, False, False),

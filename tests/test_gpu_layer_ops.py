@@ -5,8 +5,8 @@ whose other contents must not change; rows of empty slots keep what they held.""
 import numpy as np
 import pytest
 
-from layer_cases import (HEADS, LINEAR, check, custom_epilogue_package, custom_expected, heads_expected, heads_package,
-                         heads_spec, linear_expected)
+from layer_cases import (HEADS, LINEAR, TAILS, check, custom_epilogue_package, custom_expected, heads_expected,
+                         heads_package, heads_spec, linear_expected)
 from thompiler import synth
 from thompiler.device import DeviceKernel
 from thompiler.families.tuning import TUNING
@@ -93,19 +93,6 @@ def test_linear(tmp_path, monkeypatch, case, launch):
     torch.cuda.synchronize()
     assert torch.equal(first, y)
     k.close()
-
-
-# sizes whose last wave of tiles is cut: (whole strips of tiles or -1, tiles in halves, width of the units)
-TAILS = [((1119, 5632, 136, "bf16", "bf16", False, "relu", True, False), (-1, 36, 128)),
-         ((1119, 5592, 264, "bf16", "bf16", True, None, True, False), (-1, 36, 128)),
-         ((1285, 4656, 264, "f16", "f16", True, "silu", True, False), (10, 0, 192)),
-         ((1302, 4784, 136, "bf16", "f32", False, None, True, False), (12, 0, 192)),
-         ((2338, 3592, 72, "f16", "f16", False, None, False, False), (7, 0, 128)),
-         ((258, 4832, 200, "bf16", "bf16", True, "silu", True, True), (-1, 2, 128)),
-         ((264, 4800, 200, "f16", "f16", False, "gelu_tanh", False, True), (37, 0, 128)),
-         ((259, 4912, 136, "bf16", "f32", True, "silu", False, True), (0, 0, 192)),
-         ((200, 1000, 136, "f16", "f16", False, "silu", True, True), (0, 0, 128)),
-         ((1285, 4656, 16384, "bf16", "bf16", True, None, True, False), (10, 0, 192))]      # in bands of four rows
 
 
 @pytest.mark.parametrize("case,cut", TAILS, ids=str)

@@ -10,8 +10,8 @@ import subprocess
 import numpy as np
 import pytest
 
-from layer_cases import (HEADS, LINEAR, check, custom_epilogue_package, custom_expected, heads_expected, heads_package,
-                         heads_spec, linear_expected)
+from layer_cases import (HEADS, LINEAR, TAILS, check, custom_epilogue_package, custom_expected, heads_expected,
+                         heads_package, heads_spec, linear_expected)
 from oracle.interp import run_package as oracle_run
 from thompiler import ir, load, problems, rotary, synth
 from thompiler.compiler import compile_kernel
@@ -277,3 +277,29 @@ def test_activations_keep_nan(tmp_path, act):
     x["x"][1, 5] = np.nan
     got = oracle_run(d, x)["linear"]
     assert np.isnan(got[1]).all() and np.isfinite(got[[0, 2]]).all()
+
+
+@pytest.mark.parametrize("case,cut", TAILS, ids=str)
+def test_cut_tails_cover_every_column_once(tmp_path, monkeypatch, case, cut):
+    """The units of a cut tail are C's columns after the whole tiles, each once, and nothing in the kernel's
+    index arithmetic divides by a count that the cut made zero."""
+    from thompiler.families.linear import LinearPair, Product
+    from thompiler.families.matmul_pair import PM
+    from thompiler.families.tuning import TUNING
+    monkeypatch.setattr(TUNING, "linear_kernel", "pair")
+    k = load.load(str(_ir(synth.linear_package(tmp_path, *case))))
+    f = LinearPair(Product.read(k))
+    M, N = case[:2]
+    strips, halves, width = cut
+    assert (f.strips if strips >= 0 else -1, f.hrem, f.tail_cols) == cut and f.tiles_m == -(-M // PM)
+    if strips >= 0:
+        per_row = (f.units - f.full_tiles) // f.tiles_m
+        assert f.full_tiles == strips * f.tiles_m and f.units == f.full_tiles + per_row * f.tiles_m
+        left = N - strips * f.tile_cols
+        assert (per_row - 1) * f.tail_out() < left <= per_row * f.tail_out()
+    else:
+        assert f.full_tiles + halves == f.tiles_m * -(-N // f.tile_cols) and f.units == f.full_tiles + 2 * halves
+        assert 2 * f.tail_out() == f.tile_cols
+    assert f.HN % f.b_box == 0 and (f.tail_cols // 2) % f.b_box == 0
+    ptx = compile_kernel(k)
+    assert "tcgen05-linear-pair" in ptx and not re.findall(r"\b(?:div|rem)\.u32 [^;]*, 0;", ptx)
