@@ -14,7 +14,9 @@ tensor memory and the store staging.  A gated tile is 256 x 128: CTA 0 of a pair
 of w's first half as its share of B, CTA 1 the matching 128 of the second, so accumulator
 columns c and 128 + c are one output's two sums without moving a byte.  What the epilogue reads
 (bias, residual) is loaded a box ahead of its use, the first box before the accumulator is
-waited for; bound by the tensor cores while K is above about a thousand.
+waited for; bound by the tensor cores while K is above about a thousand: 2048 x 6144 x 4096 bf16 +
+bias 68.4-69.7 us, 1,480-1,510 TFLOP/s.  ``linear_split`` holds the kernel for few tiles;
+``LinearRows`` and ``LinearStream`` are for few rows; ``choose`` decides.
 """
 
 from __future__ import annotations
