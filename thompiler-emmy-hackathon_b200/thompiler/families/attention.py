@@ -582,7 +582,7 @@ class TcAttention(TunedKernel):
         elect_one(em, lead)
         tmap_o = tmap_address(em, self.tmap_set, 4, 3)
         sc = t("f32")
-        ins(f"ld.global.nc.f32 {sc}, [{em.buffer_reg(self.pscale.name)}]")
+        ins(f"ld.global.f32 {sc}, [{em.buffer_reg(self.pscale.name)}]")
         ins(f"rcp.rn.f32 {sc}, {sc}")
         ins(f"mul.rn.f32 {sc}, {sc}, 0f{_f32bits(LOG2E)}")
         mref, mref8, l = t("f32"), t("f32"), t("f32")

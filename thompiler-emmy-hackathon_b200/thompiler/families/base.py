@@ -25,17 +25,16 @@ from thompiler.walk import Walker
 
 class TunedKernel:
     family = "tuned"
-    # the generic path of the module, too, reads with ordinary loads.  A kernel launched to overlap the previous
-    # one begins while that one still writes, so its inputs are not constant for its lifetime, which is what
-    # ``ld.global.nc`` promises: the assembler may move such a load above griddepcontrol.wait, and did (a chain
-    # of linear-stream launches in a graph read the previous launch's input)
-    coherent = False
 
     def __init__(self, kernel: KernelInfo) -> None:
         self.k = kernel
         self.em = Emitter()
         self.w = Walker(self.em, kernel)
-        self.w.coherent = self.coherent
+        # both paths of the module read with ordinary loads.  A kernel launched to overlap the previous one begins
+        # while that one still writes, so its inputs are not constant for its lifetime, which is what
+        # ``ld.global.nc`` promises: the assembler may move such a load above griddepcontrol.wait, and did (a chain
+        # of linear-stream launches in a graph read the previous launch's input)
+        self.w.coherent = True
         self.pdl = False            # set by pdl_wait: the tuned body waits for the previous grid
 
     # programmatic dependent launch ----------------------------------------------
@@ -88,7 +87,8 @@ class TunedKernel:
             side = dict(em.sidecar or {}, **side, family=self.family)
         if self.pdl:
             # both paths wait for the previous grid before touching global data, so any launch of
-            # the module (the tuned one or meta.json's) may overlap the stream's previous kernel
+            # the module (the tuned one or meta.json's, unless a family records pdl_meta: false) may
+            # overlap the stream's previous kernel
             side = dict(side if side is not None else (em.sidecar or {}), pdl=True)
         em.sidecar = side if side is not None else em.sidecar
         return em.render(prologue.header(), self.k.name, prologue.params(self.k))

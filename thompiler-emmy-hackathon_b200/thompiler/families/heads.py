@@ -38,7 +38,6 @@ def _pow2_at_least(n: int) -> int:
 
 class RotaryHeads(TunedKernel):
     family = "rotary-heads"
-    coherent = True
 
     def __init__(self, kernel: KernelInfo, B, S, heads, kv, D, R, P, ty, interleaved, values, heads_first, inverse, eps):
         super().__init__(kernel)

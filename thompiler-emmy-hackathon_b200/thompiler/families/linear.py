@@ -186,7 +186,6 @@ class Replay:
 
 class LinearPair(TcMatmulPair):
     family = "tcgen05-linear-pair"
-    coherent = True
     offset = None                # columns from the tile's first to those that this thread finishes
     # one compiled product serves every layer of a model.  Past the sets each call re-encodes one: 32 weights of
     # 4096 x 4096 at 512 rows, one after another, take 208 us a call with 8 sets (the other families') and 18.2
@@ -508,8 +507,6 @@ ROW_STEP = PRODUCERS // 8                    # rows that the producers copy a pi
 
 class ByElement(TunedKernel):
     """What the kernels for few rows share: a thread finishes single elements of C."""
-
-    coherent = True
 
     def __init__(self, p: Product):
         super().__init__(p.kernel)

@@ -14,7 +14,7 @@ meta.json zeroes C before every launch (then writing the full sum is the same re
 Tuned body: C = A B with every output's full K sum kept in a register of one thread -- no
 split-K, no atomics.  A CTA of 256 threads (16 x 16) owns a BM x BN tile of C (64 x 64, each
 thread 4 x 4 outputs, or 32 x 32 with 2 x 2 when that gives more CTAs to fill the SMs).  K goes
-in steps of 16: the next step's A and B chunks are loaded (``ld.global.nc.v4``) into registers
+in steps of 16: the next step's A and B chunks are loaded (``ld.global.v4``) into registers
 while the current step's tiles in shared memory feed ``fma.rn.f32`` (A stored k-major, so a
 thread's RM rows of one k are one vector load; B row-major, RN columns one vector load); the
 two shared buffers alternate.  Sums run in ascending k, in f32 -- within rtol 1e-3 of the
@@ -265,8 +265,8 @@ class MatmulF32(TunedKernel):
                 ins(f"add.u64 {ka}, {ka}, {aoff}")
                 ins(f"mul.wide.u32 {kb}, {step}, {BK * N * 4}")
                 ins(f"add.u64 {kb}, {kb}, {boff}")
-                ins(f"@{is_a} ld.global.nc.v4.f32 {{{', '.join(v)}}}, [{ka}]")
-                ins(f"@!{is_a} ld.global.nc.v4.f32 {{{', '.join(v)}}}, [{kb}]")
+                ins(f"@{is_a} ld.global.v4.f32 {{{', '.join(v)}}}, [{ka}]")
+                ins(f"@!{is_a} ld.global.v4.f32 {{{', '.join(v)}}}, [{kb}]")
 
         def sstore(buf: str) -> None:
             """The loaded chunks into shared buffer ``buf`` (0 / 1): A transposed, B as it is."""

@@ -5,8 +5,8 @@ buffers, each thread handling U consecutive elements -- the reference problems' 
 schedule, e.g. problems/p01_vector_add: ``x0[a0 * 2 + 0]``, ``x0[a0 * 2 + 1]`` loaded by two
 statements, the sums written by one.  The generic lowering issues one 4-byte access per
 statement; here the single-element Loads of a read-only buffer at ``X + 0 .. X + U-1`` become
-one vector load (``ld.global.nc.v{V}``, V = min(U, 16 / element bytes), so a warp moves
-whole 128-byte lines per instruction) issued at the first of them, and single-value Writes at
+one vector load (V = min(U, 16 / element bytes), so a warp moves whole 128-byte lines per
+instruction) issued at the first of them, and single-value Writes at
 ``X + 0 .. X + U-1`` one vector store issued at the last of them (every value is computed by
 then).  The values, their order of computation and the IR's arithmetic are unchanged, so the
 results are bit-identical to the generic lowering.
@@ -14,6 +14,11 @@ results are bit-identical to the generic lowering.
 X must be ``a * m`` with m a multiple of V (so element X + jV sits on a V-element boundary);
 the guard also checks at run time that every vectorised buffer's base pointer is aligned to
 V elements, else the generic lowering of the same IR runs (a caller may pass an offset view).
+
+The body exists twice.  The recorded launch has one CTA more than meta.json's (it finds no
+elements); such a launch may begin while the stream's previous kernel still writes the inputs,
+so its vector loads are ``ld.global``.  meta.json's own launch is an ordinary one, its inputs are
+constant for its lifetime, and its vector loads stay ``ld.global.nc``.
 """
 
 from __future__ import annotations
@@ -112,10 +117,28 @@ class Pointwise(TunedKernel):
             em.ins(f"@{p} bra {generic}")
 
     def emit_tuned(self) -> None:
-        from thompiler.lowering import address
         em, w = self.em, self.w
         self.pdl_trigger()
+        p, ordinary = em.tmp("pred"), em.label("ordinary_launch")
+        em.ins(f"setp.ne.u32 {p}, {self.special('%nctaid.x')}, {self.k.grid[0] + 1}")
         self.pdl_wait()
+        em.ins(f"@{p} bra {ordinary}")
+        self._body("ld.global")
+        em.ins(f"bra {self.exit}")
+        em.place(ordinary)
+        w.consts.clear()
+        w.coherent = False
+        self._body("ld.global.nc")
+        w.coherent = True
+
+    def sidecar(self) -> dict:
+        g = self.k.grid
+        return {"grid": [g[0] + 1, *g[1:]], "block": list(self.k.block), "smem_bytes": self.k.dynamic_smem_bytes,
+                "pdl_meta": False}
+
+    def _body(self, ld: str) -> None:
+        from thompiler.lowering import address
+        em, w = self.em, self.w
         pos = {id(s): i for i, s in enumerate(self.stmts)}
 
         def load_hook(w_, load) -> bool:
@@ -129,7 +152,7 @@ class Pointwise(TunedKernel):
             idx = (ir.BinaryExpr("+", x, ir.Literal(j, "int")),) if j else (x,)
             _, addr, ty, _ = address.access(w_, p.name, idx)
             regs = [em.value(s.names[0], ty.reg) for s in members]
-            em.ins(f"ld.global.nc.v{len(regs)}.{ty.mov} {{{', '.join(regs)}}}, [{addr}]")
+            em.ins(f"{ld}.v{len(regs)}.{ty.mov} {{{', '.join(regs)}}}, [{addr}]")
             return True
 
         def write_hook(w_, wr) -> bool:

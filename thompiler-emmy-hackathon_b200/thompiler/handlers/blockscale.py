@@ -116,7 +116,7 @@ def emit_block_scale_load(w: "Walker", s: ir.BlockScaleLoad) -> None:
         b = em.tmp("b32")
         if prm is not None:
             a = address.global_address(w, prm, idx)
-            em.ins(f"ld.global{'.nc' if not prm.written else ''}.u8 {b}, [{a}]")
+            em.ins(f"ld.global{'' if prm.written or w.coherent else '.nc'}.u8 {b}, [{a}]")
         else:
             elem = address.flat_index(w, arr.extents, idx, arr.name)
             a = address.shared_element_address(w, arr, elem, "NONE")

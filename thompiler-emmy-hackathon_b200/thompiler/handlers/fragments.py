@@ -284,7 +284,7 @@ def _coordinate_operand(w: "Walker", s: ir.FragmentApply, nregs: int, e: int, ar
     if prm is None:
         raise ValueError(f"FragmentApply bias: {buf!r} is not a kernel parameter")
     addr = address.global_address(w, prm, idx)
-    ld = "ld.global" if prm.written else "ld.global.nc"      # a buffer the kernel writes: coherent loads
+    ld = "ld.global" if prm.written or w.coherent else "ld.global.nc"    # a buffer that is written: coherent loads
     if prm.ty is F32:
         em.ins(f"{ld}.f32 {out}, [{addr}]")
     elif prm.ty is F16:

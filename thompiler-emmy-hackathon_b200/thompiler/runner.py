@@ -248,6 +248,7 @@ class LaunchPlan:
     counters: list = field(default_factory=list)    # self-resetting arrival counters (module globals)
     pdl: bool = False                               # the tuned body waits (griddepcontrol.wait) before
                                                     # global accesses: launches may overlap the previous kernel
+                                                    # (meta.json's too, unless the record says pdl_meta: false)
 
 
 def plan_launch(module: Module, kmeta: dict, honour_meta: bool = False) -> LaunchPlan:
@@ -259,7 +260,7 @@ def plan_launch(module: Module, kmeta: dict, honour_meta: bool = False) -> Launc
     if "grid" not in side or honour_meta:
         err = side.get("error_word") if "grid" not in side else None
         return LaunchPlan(tuple(kmeta["grid"]), tuple(kmeta["block"]), int(kmeta.get("smem_bytes", 0)), False,
-                          ir_maps, None, err, counters, bool(side.get("pdl", False)))
+                          ir_maps, None, err, counters, bool(side.get("pdl_meta", side.get("pdl", False))))
     return LaunchPlan(tuple(side["grid"]), tuple(side["block"]), int(side.get("smem_bytes", 0)), True,
                       list(side.get("tmaps", [])) + ir_maps, side.get("tmap_ptrs"), side.get("error_word"),
                       counters, bool(side.get("pdl", False)))
