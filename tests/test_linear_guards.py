@@ -1,0 +1,76 @@
+"""What the fused linear product's kernels refuse by themselves, on the CPU: operands off the 16-byte
+boundary that their copies need, whatever meta.json says of alignment, and launch geometries that the
+package's own does not allow."""
+
+import json
+import re
+from types import SimpleNamespace
+
+import pytest
+
+from thompiler import ir, load, runner, schedules, synth
+from thompiler.compiler import compile_kernel
+from thompiler.emitter import read_sidecar
+from thompiler.families.tuning import TUNING
+
+KERNELS = ("stream", "rows", "split", "pair")
+
+
+def _package(out, M, N, K, grid, epilogue=None, inputs=None):
+    """A linear product without ``align`` records, launched with ``grid`` CTAs by meta.json."""
+    return synth._layer_write(out, "linear", "linear", "k_linear",
+                              schedules.linear_body(M, N, K, "f16", False, epilogue),
+                              {"x": ((M, K), "f16", None), "w": ((N, K), "f16", None), **(inputs or {})},
+                              {"linear": ((M, N), "f16", None)}, grid, 128, 2e-2, 2e-3, smem=2 * 64 * 64 * 2)
+
+
+def _info(d):
+    return load.load(str(next(d.glob("*.ir.json"))))
+
+
+def _extra(M, N):
+    """An epilogue that adds a vector over the columns, and its input."""
+    epi = ir.Lambda(("z", "row", "col"), (ir.Load(("e",), "extra", (schedules.clamped(ir.Var("col"), N),), schedules.F32T),
+                                          schedules.assign("y", "add", "z", "e")), ("y",))
+    return epi, {"extra": ((N,), "f32", None)}
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_kernel_checks_its_operands(tmp_path, monkeypatch, kernel):
+    """Before any branch to a path that copies from them, x and w are tested and sent to the refusal."""
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    ptx = compile_kernel(_info(_package(tmp_path / "p", 16, 512, 512, 64)))
+    assert read_sidecar(ptx)["family"].endswith("linear-" + kernel)
+    body = ptx[ptx.index(".entry"):]
+    to = set()
+    for name in ("x", "w"):
+        m = re.search(rf"and\.b64 (%rd\d+), %g_{name}, 15;\s*setp\.ne\.u64 (%p\d+), \1, 0;\s*@\2 bra (\$\w+);", body)
+        assert m, name
+        assert not re.search(r"\bbra\b|cp\.async|ld\.global", body[:m.start()].replace(f"bra {m[3]}", ""))
+        to.add(m[3])
+    (bad,) = to
+    assert re.match(r"\s*(griddepcontrol\.wait;\s*)?mov\.u64 %rd\d+, thc_error;\s*atom\.global\.or\.b32 %r\d+, \[%rd\d+\], 16;\s*ret;",
+                    body[body.index(bad + ":") + len(bad) + 1:])
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_call_is_refused_without_align_in_meta(tmp_path, monkeypatch, kernel):
+    """The launch record carries the boundaries: ``Launch`` refuses before anything is issued."""
+    if not runner.LIB_PATH.exists():
+        pytest.skip("runner library not built")
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    epi, more = _extra(16, 512)
+    d = _package(tmp_path / "p", 16, 512, 512, 64, epi, more)
+    kmeta = json.loads((d / "meta.json").read_text())["kernels"][0]
+    assert not any("align" in a for a in kmeta["args"])
+    side = read_sidecar(compile_kernel(_info(d)))
+    plan = runner.plan_launch(SimpleNamespace(sidecar=side), kmeta)
+    plan.tmaps = []
+    wide = {"x", "w"} | ({"extra", "linear"} if kernel in ("split", "pair") else set())
+    assert {n for n, a in plan.align.items() if a == 16} == wide
+    k = runner.Launch(SimpleNamespace(handle=1, name="k_linear", module=SimpleNamespace(handle=0)), plan, kmeta, None)
+    good = {n: 4096 * (i + 1) for i, n in enumerate(kmeta["arg_order"])}
+    for name in wide:
+        with pytest.raises(runner.RunnerError, match=f"buffer '{name}' .* not 16-byte aligned") as e:
+            k(dict(good, **{name: good[name] + 8}))
+        assert e.value.stage == "request"

@@ -107,6 +107,15 @@ class TunedKernel:
         em.ins("ret")
         em.place(skip)
 
+    def check_aligned(self, names: list[str], to: int, bad: str) -> None:
+        """Branch to ``bad`` unless each buffer starts on a multiple of ``to`` bytes."""
+        em, q = self.em, self.em.tmp("pred")
+        for name in names:
+            a = em.tmp("b64")
+            em.ins(f"and.b64 {a}, {em.buffer_reg(name)}, {to - 1}")
+            em.ins(f"setp.ne.u64 {q}, {a}, 0")
+            em.ins(f"@{q} bra {bad}")
+
     def special(self, reg: str) -> str:
         r = self.em.tmp("b32")
         self.em.ins(f"mov.u32 {r}, {reg}")

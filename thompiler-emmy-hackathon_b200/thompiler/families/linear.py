@@ -127,15 +127,10 @@ class Replay:
                     return False
         return True
 
-    def check_alignment(self, bad: str) -> None:
-        """Branch to ``bad`` unless every source takes 16-byte accesses (the runner refuses such calls)."""
-        em = self.f.em
-        q = em.tmp("pred")
-        for name in sorted({s[0] for s in self.sources}):
-            a = em.tmp("b64")
-            em.ins(f"and.b64 {a}, {em.buffer_reg(name)}, 15")
-            em.ins(f"setp.ne.u64 {q}, {a}, 0")
-            em.ins(f"@{q} bra {bad}")
+    @property
+    def names(self) -> list[str]:
+        """The buffers that are fetched."""
+        return sorted({s[0] for s in self.sources})
 
     def unpacked(self, regs: list[str], i: int, ty: Ty) -> str:
         """Element ``i`` of packed ``regs`` as its load would leave it: an f32 value, or f16's b16."""
@@ -288,16 +283,20 @@ class LinearPair(TcMatmulPair):
         em.module(".global .align 4 .u32 thc_error")
         em.module(".extern .shared .align 1024 .b8 smem_pool[]")
         em.entry_attrs.append(f".reqnctapercluster {cluster}, 1, 1")
-        q = em.tmp("pred")
+        q, bad = em.tmp("pred"), em.label("unserved")
+        self.check_aligned([self.a.name, self.b.name], 16, bad)     # in any launch: the generic path's copies too
         em.ins(f"setp.ne.u32 {q}, {self.special('%ntid.x')}, {threads}")
         em.ins(f"@{q} bra {generic}")
-        bad = em.label("unserved")
         em.ins(f"setp.lt.u32 {q}, {self.special('%tid.x')}, 32")
         self.table = load_tmap_table(em, [b.name for b in (self.a, self.b, self.c)], bad, self.map_sets, q)
         if self.replay:
-            self.replay.check_alignment(bad)
+            self.check_aligned(self.replay.names, 16, bad)
         self.refuse(bad, 4)
         return bad
+
+    def sidecar(self) -> dict:
+        names = [self.a.name, self.b.name, self.c.name] + (self.replay.names if self.replay else [])
+        return dict(super().sidecar(), align=dict.fromkeys(names, 16))
 
     # ---- barriers, tensor memory and maps ----------------------------------------------------
 
@@ -513,6 +512,24 @@ class ByElement(TunedKernel):
         self.p = p
         self.replay = Replay(self, p) if p.epilogue is not None else None
 
+    def sidecar(self) -> dict:
+        return {"grid": [self.plan.ctas, 1, 1], "smem_bytes": self.plan.smem, "error_word": "thc_error",
+                "align": {self.p.x.name: 16, self.p.w.name: 16}}
+
+    def guard_launch(self, generic: str, threads: int) -> None:
+        """To ``generic``: another block than ``threads``.  Refused: another grid, and, in any launch (the
+        generic path copies 16 bytes at a time, too), operands off their boundary."""
+        em = self.em
+        em.module(".global .align 4 .u32 thc_error")
+        em.module(".extern .shared .align 1024 .b8 smem_pool[]")
+        q, bad = em.tmp("pred"), em.label("unserved")
+        self.check_aligned([self.p.x.name, self.p.w.name], 16, bad)
+        em.ins(f"setp.ne.u32 {q}, {self.special('%ntid.x')}, {threads}")
+        em.ins(f"@{q} bra {generic}")
+        em.ins(f"setp.ne.u32 {q}, {self.special('%nctaid.x')}, {self.plan.ctas}")
+        em.ins(f"@{q} bra {bad}")
+        self.refuse(bad, 4)
+
     def _tokens(self, x: str, m: str, n: str, left: str, inside: str | None, count: int,
                 into: list | None = None) -> list:
         """Tokens x, x + 1, .. of the tile (rows m, m + 1, .. of C): [(row, stored?, sources)], with the
@@ -629,22 +646,13 @@ class LinearRows(ByElement):
 
     def sidecar(self) -> dict:
         pl = self.plan
-        return {"grid": [pl.ctas, 1, 1], "block": [PRODUCERS + 32, 1, 1], "smem_bytes": pl.smem,
-                "error_word": "thc_error", "cluster": [pl.S, 1, 1], "tile": [BM, pl.BT, BK], "stages": pl.stages}
+        return dict(super().sidecar(), block=[PRODUCERS + 32, 1, 1], cluster=[pl.S, 1, 1], tile=[BM, pl.BT, BK],
+                    stages=pl.stages)
 
     def guard(self, generic: str) -> None:
-        em = self.em
-        em.module(".global .align 4 .u32 thc_error")
-        em.module(".extern .shared .align 1024 .b8 smem_pool[]")
         if self.plan.S > 1:
-            em.entry_attrs.append(f".reqnctapercluster {self.plan.S}, 1, 1")
-        q = em.tmp("pred")
-        em.ins(f"setp.ne.u32 {q}, {self.special('%ntid.x')}, {PRODUCERS + 32}")
-        em.ins(f"@{q} bra {generic}")
-        bad = em.label("other_grid")
-        em.ins(f"setp.ne.u32 {q}, {self.special('%nctaid.x')}, {self.plan.ctas}")
-        em.ins(f"@{q} bra {bad}")
-        self.refuse(bad, 4)
+            self.em.entry_attrs.append(f".reqnctapercluster {self.plan.S}, 1, 1")
+        self.guard_launch(generic, PRODUCERS + 32)
 
     def emit_tuned(self) -> None:  # noqa: C901 - one kernel, written out in order
         em, t, ins, place, lab = self.em, self.em.tmp, self.em.ins, self.em.place, self.em.label
@@ -1142,19 +1150,10 @@ class LinearStream(ByElement):
         self.plan = plan
 
     def sidecar(self) -> dict:
-        return {"grid": [self.plan.ctas, 1, 1], "block": [256, 1, 1], "smem_bytes": self.plan.smem,
-                "error_word": "thc_error"}
+        return dict(super().sidecar(), block=[256, 1, 1])
 
     def guard(self, generic: str) -> None:
-        em = self.em
-        em.module(".extern .shared .align 1024 .b8 smem_pool[]")
-        q = em.tmp("pred")
-        em.ins(f"setp.ne.u32 {q}, {self.special('%ntid.x')}, 256")
-        em.ins(f"@{q} bra {generic}")
-        bad = em.label("other_grid")
-        em.ins(f"setp.ne.u32 {q}, {self.special('%nctaid.x')}, {self.plan.ctas}")
-        em.ins(f"@{q} bra {bad}")
-        self.refuse(bad, 4)
+        self.guard_launch(generic, 256)
 
     def emit_tuned(self) -> None:
         em, t, ins, place, lab = self.em, self.em.tmp, self.em.ins, self.em.place, self.em.label

@@ -249,6 +249,7 @@ class LaunchPlan:
     pdl: bool = False                               # the tuned body waits (griddepcontrol.wait) before
                                                     # global accesses: launches may overlap the previous kernel
                                                     # (meta.json's too, unless the record says pdl_meta: false)
+    align: dict = field(default_factory=dict)       # buffer -> the boundary, in bytes, that it has to start on
 
 
 def plan_launch(module: Module, kmeta: dict, honour_meta: bool = False) -> LaunchPlan:
@@ -258,12 +259,12 @@ def plan_launch(module: Module, kmeta: dict, honour_meta: bool = False) -> Launc
     ir_maps = list(side.get("ir_tmaps", []))
     counters = list(side.get("counters", []))
     if "grid" not in side or honour_meta:
-        err = side.get("error_word") if "grid" not in side else None
         return LaunchPlan(tuple(kmeta["grid"]), tuple(kmeta["block"]), int(kmeta.get("smem_bytes", 0)), False,
-                          ir_maps, None, err, counters, bool(side.get("pdl_meta", side.get("pdl", False))))
+                          ir_maps, None, side.get("error_word"), counters,
+                          bool(side.get("pdl_meta", side.get("pdl", False))))
     return LaunchPlan(tuple(side["grid"]), tuple(side["block"]), int(side.get("smem_bytes", 0)), True,
                       list(side.get("tmaps", [])) + ir_maps, side.get("tmap_ptrs"), side.get("error_word"),
-                      counters, bool(side.get("pdl", False)))
+                      counters, bool(side.get("pdl", False)), dict(side.get("align", {})))
 
 
 def encode_tensor_map(spec: dict, base: int) -> bytes:
@@ -312,15 +313,16 @@ class Launch:
     """One kernel's launches on device pointers.  What stays the same from call to call is a C record made
     once, so ``launch(ptrs, stream)`` packs the pointers and makes one C call (with its tensor maps'
     binding, when the plan has any).  ``plan``'s grid, block, shared memory and overlap are read again
-    whenever they are replaced; a buffer that meta.json wants aligned is refused when it is not."""
+    whenever they are replaced; a buffer that meta.json or the launch record wants aligned is refused when
+    it is not."""
 
     def __init__(self, function: Function, plan: LaunchPlan, kmeta: dict, tmaps: TensorMaps | None):
         self.function, self.plan, self.order, self.tmaps = function, plan, tuple(kmeta["arg_order"]), tmaps
         n = len(self.order)
         self._get = operator.itemgetter(*self.order) if n > 1 else lambda ptrs: tuple(ptrs[x] for x in self.order)
         self._pack = struct.Struct(f"@{max(1, n)}Q").pack if n else lambda: bytes(8)
-        align = {a["name"]: a.get("align", 0) for a in kmeta["args"]}
-        self._align = (ctypes.c_uint32 * max(1, n))(*[align.get(x, 0) for x in self.order])
+        align, own = {a["name"]: a.get("align", 0) for a in kmeta["args"]}, getattr(plan, "align", {})
+        self._align = (ctypes.c_uint32 * max(1, n))(*[max(align.get(x, 0), own.get(x, 0)) for x in self.order])
         self._call = library().thr_launch_prepared
         self._geometry, self._descs = None, []
 
