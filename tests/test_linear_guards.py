@@ -74,3 +74,18 @@ def test_call_is_refused_without_align_in_meta(tmp_path, monkeypatch, kernel):
         with pytest.raises(runner.RunnerError, match=f"buffer '{name}' .* not 16-byte aligned") as e:
             k(dict(good, **{name: good[name] + 8}))
         assert e.value.stage == "request"
+
+
+@pytest.mark.parametrize("kernel", ["", *KERNELS])
+@pytest.mark.parametrize("M,N,K,grid", [(40, 72, 4096, 2), (130, 72, 4096, 6), (40, 200, 8192, 4), (300, 200, 2048, 20),
+                                        (64, 64, 4096, 1), (300, 64, 4096, 5), (2048, 576, 512, 288), (600, 960, 512, 150)])
+def test_clusters_divide_metas_grid(tmp_path, monkeypatch, kernel, M, N, K, grid):
+    """A cluster's shape belongs to the entry, so meta.json's launch runs in it too."""
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    ptx = compile_kernel(_info(_package(tmp_path / "p", M, N, K, grid)))
+    shapes = [int(x) for x in re.findall(r"\.reqnctapercluster (\d+)", ptx)]
+    assert all(grid % s == 0 for s in shapes), shapes
+    side = read_sidecar(ptx) or {}
+    assert side.get("cluster", [1])[0] in (shapes or [1])
+    if not shapes and M > 24:                             # neither a cluster's kernel nor the one for a handful of rows
+        assert "linear-rows" in side["family"] if "family" in side else "griddepcontrol" not in ptx

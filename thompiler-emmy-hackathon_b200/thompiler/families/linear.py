@@ -51,6 +51,10 @@ class Product:
         # the generic path's slabs, where they are static arrays of their own
         self.static_smem = 0 if kernel.dynamic_smem_bytes else (3 if gated else 2) * 64 * 64 * 2
 
+    def launches_in(self, cluster: int) -> bool:
+        """Does meta.json's launch divide into clusters of this size?  They belong to the entry, so to every launch."""
+        return self.kernel.grid[0] % cluster == 0
+
     @classmethod
     def read(cls, kernel: KernelInfo) -> "Product | None":
         x, w, c = (kernel.param(n) for n in ("x", "w", "linear"))
@@ -1105,7 +1109,7 @@ class RowsPlan:
                 break
             for S in (1, 2, 4, 8):
                 pl = cls(p, BT, S)
-                if pl.possible:
+                if pl.possible and p.launches_in(S):
                     out.append((pl.estimate(p), S, tiles_m, pl))
         return min(out, key=lambda x: x[:3])[3] if out else None
 
@@ -1373,8 +1377,9 @@ class StreamPlan:
         return 1.53 + ((p.w.nbytes / 6.46e6) ** 4 + turns ** 4) ** 0.25 + more
 
 
-def choose(p: Product) -> TunedKernel:
-    """The kernel and plan whose estimated time is least.
+def choose(p: Product) -> TunedKernel | None:
+    """The kernel and plan whose estimated time is least, of those whose clusters meta.json's grid divides
+    into (None: there is none).
 
     The estimates' forms follow what bounds each kernel; their constants are least-squares fits (of log
     time) to 1,745 timings on a B200 of every plan at M = 1 .. 1024, (N, K) from 512 x 512 to 8192 x 8192,
@@ -1384,8 +1389,10 @@ def choose(p: Product) -> TunedKernel:
     1 x 512 x 512 1.7 / 2.5 / - / 5.3; 1 x 4096 x 4096 6.1 / 6.8 / - / 21; 16 x 4096 x 4096 7.7 / 7.0 / - / 17;
     128 x 4096 x 4096 - / 10.3 / 12.0 / 16.5; 512 x 4096 x 8192 - / 32.1 / 28.4 / 31.4; 835 x 440 x 4048 gated
     - / 29.8 / 11.8 / 24.2; 1024 x 4096 x 4096 - / 28.8 / - / 26.3; 2048 x 4096 x 4096 - / - / - / 51."""
-    pair = LinearPair(p)
-    plans = [(pair.estimate(), "pair", lambda: pair)]
+    plans = []
+    if p.launches_in(2):
+        pair = LinearPair(p)
+        plans.append((pair.estimate(), "pair", lambda: pair))
     rows, stream = RowsPlan.best(p), StreamPlan.of(p)
     if rows is not None:
         plans.append((rows.estimate(p), "rows", lambda: LinearRows(p, rows)))
@@ -1393,10 +1400,10 @@ def choose(p: Product) -> TunedKernel:
         plans.append((stream.estimate(p), "stream", lambda: LinearStream(p, stream)))
     from thompiler.families.linear_split import LinearSplit, SplitPlan
     split = SplitPlan.best(p)
-    if split is not None:
+    if split is not None and p.launches_in(4):
         plans.append((split.estimate(p), "split", lambda: LinearSplit(p, split)))
     forced = [x for x in plans if x[1] == TUNING.linear_kernel]
-    return min(forced or plans, key=lambda x: x[0])[2]()
+    return min(forced or plans, key=lambda x: x[0])[2]() if plans else None
 
 
 def recognise(kernel: KernelInfo):
