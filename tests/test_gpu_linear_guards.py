@@ -1,10 +1,12 @@
 """Linear products whose package is launched with a grid that clusters do not divide, under their own
-launch and meta.json's, against the float64 product."""
+launch and meta.json's, against the float64 product; and products of very long rows."""
 
 import pytest
 
 from test_linear_guards import _package
+from thompiler import synth
 from thompiler.device import DeviceKernel
+from thompiler.families.tuning import TUNING
 
 pytestmark = pytest.mark.gpu
 
@@ -30,5 +32,29 @@ def test_any_grid_of_metas(tmp_path, M, N, K, grid, meta):
     torch.cuda.synchronize()
     want, allowed = _bound(x, w)
     assert ((y.double() - want).abs() <= allowed).all()
+    assert k.error_word() == 0
+    k.close()
+
+
+@pytest.mark.parametrize("M,N,K,kernel", [(16, 64, 16 << 20, ""), (16, 64, 16 << 20, "pair"), (1, 24, 16 << 20, ""),
+                                          (256, 64, (5 << 20) + 8, "")])
+def test_long_rows(tmp_path, monkeypatch, M, N, K, kernel):
+    """Rows past the reach of an address' immediate offset.  Entries of -1, 0 and 1: about 4 K / 9 products, fewer
+    than 2^24, are not zero, so f32 holds every partial sum exactly, whatever the order."""
+    import torch
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    k = DeviceKernel(next(synth.linear_package(tmp_path / "p", M, N, K, out_dtype="f32").glob("*.ir.json")))
+    g = torch.Generator(device="cuda").manual_seed(K + M)
+
+    def entries(rows):
+        return torch.randint(-1, 2, (rows, K), device="cuda", generator=g, dtype=torch.int8).half()
+    x, w = entries(M), entries(N)
+    y = torch.full((M, N), float("nan"), device="cuda")
+    k({"x": x.data_ptr(), "w": w.data_ptr(), "linear": y.data_ptr()}, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    want = torch.zeros(M, N, device="cuda", dtype=torch.float64)
+    for at in range(0, K, 1 << 20):
+        want += x[:, at:at + (1 << 20)].double() @ w[:, at:at + (1 << 20)].double().t()
+    assert torch.equal(y.double(), want)
     assert k.error_word() == 0
     k.close()

@@ -89,3 +89,32 @@ def test_clusters_divide_metas_grid(tmp_path, monkeypatch, kernel, M, N, K, grid
     assert side.get("cluster", [1])[0] in (shapes or [1])
     if not shapes and M > 24:                             # neither a cluster's kernel nor the one for a handful of rows
         assert "linear-rows" in side["family"] if "family" in side else "griddepcontrol" not in ptx
+
+
+@pytest.mark.parametrize("kernel", ["", *KERNELS])
+@pytest.mark.parametrize("M,N,K,more", [(16, 64, 16 << 20, {}), (256, 64, 5 << 20, {}), (1, 64, 1 << 27, {}),
+                                        (20, 16, 1 << 28, {}), (3, 64, 1 << 26, dict(gated=True)), (200, 64, 4 << 20, {}),
+                                        (1, 1 << 30, 8, dict(residual=True, out_dtype="f32"))], ids=str)
+def test_offsets_fit_their_fields(tmp_path, monkeypatch, kernel, M, N, K, more):
+    """Immediate offsets of addresses are signed 32-bit numbers, and so fit the operands of 32-bit
+    instructions, at the longest rows too."""
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    ptx = compile_kernel(_info(synth.linear_package(tmp_path / "p", M, N, K, **more)))
+    side = read_sidecar(ptx) or {}
+    assert "linear" in side.get("family", "") or K > 64 << 20
+    # a wait lasts about a second: no CTA-pair tile of more than 2^20 K blocks
+    assert K <= 64 << 20 or side.get("cluster", [1])[0] == 1
+    assert max(int(x) for x in re.findall(r"\+(\d+)\]", ptx)) < 2 ** 31
+    for op, n in re.findall(r"\t(?:@!?%p\d+ )?(\w+\.[\w.]*(?:u32|s32|b32)) [^;]*?, (\d+)(?:, %\w+)?;", ptx):
+        assert int(n) < 2 ** 32, (op, n)
+
+
+def test_wide_f32_rows_of_an_epilogue(tmp_path, monkeypatch):
+    """An f32 array of C's shape whose rows are 4 GB: its row pitch is no 32-bit number."""
+    monkeypatch.setattr(TUNING, "linear_kernel", "pair")
+    M, N = 2, 1 << 30
+    epi = ir.Lambda(("z", "row", "col"), (ir.Load(("e",), "extra", (schedules.clamped(ir.Var("row"), M), ir.Var("col")),
+                                                  schedules.F32T), schedules.assign("y", "add", "z", "e")), ("y",))
+    ptx = compile_kernel(_info(_package(tmp_path / "p", M, N, 8, 1 << 24, epi, {"extra": ((M, N), "f32", None)})))
+    tuned = ptx[:ptx.index("generic lowering of the same IR")]
+    assert "tcgen05-linear-pair" in ptx and not re.search(rf"\.u32 [^;]*\b{4 * N};", tuned)

@@ -51,6 +51,12 @@ class Product:
         # the generic path's slabs, where they are static arrays of their own
         self.static_smem = 0 if kernel.dynamic_smem_bytes else (3 if gated else 2) * 64 * 64 * 2
 
+    @property
+    def tile_ends(self) -> bool:
+        """Does a tile's K loop end well within the second that the kernels' waits last?  2^20 blocks of the
+        CTA-pair kernels, at up to 0.4 us each, take 0.4 s."""
+        return self.K <= BK << 20
+
     def launches_in(self, cluster: int) -> bool:
         """Does meta.json's launch divide into clusters of this size?  They belong to the entry, so to every launch."""
         return self.kernel.grid[0] % cluster == 0
@@ -390,8 +396,8 @@ class LinearPair(TcMatmulPair):
             a, off = t("b64"), t("b64")
             ins(f"mad.wide.u32 {a}, {self.col}, {nb}, {em.buffer_reg(name)}")
             if not cols_only:
-                ins(f"mul.wide.u32 {off}, {self.row}, {p.N * nb}")
-                ins(f"add.u64 {a}, {a}, {off}")
+                ins(f"mul.wide.u32 {off}, {self.row}, {p.N}")
+                ins(f"mad.lo.u64 {a}, {off}, {nb}, {a}")
             if first:
                 ins(f"add.u64 {a}, {a}, {first * nb}")
             self.at[src] = a
@@ -506,6 +512,7 @@ EXCHANGE_LIMIT = 64 * 1024                   # shared memory for the partial sum
 PRODUCERS = 256
 MMA_WARP = PRODUCERS // 32
 ROW_STEP = PRODUCERS // 8                    # rows that the producers copy a piece of at a time
+OFFSET_LIMIT = 2 ** 31                       # an address' immediate offset is a signed 32-bit number
 
 
 class ByElement(TunedKernel):
@@ -1075,6 +1082,7 @@ class RowsPlan:
         self.kblocks = -(-p.K // BK)
         self.tiles_m, self.tiles_n = -(-p.M // BT), -(-p.N // BM)
         self.ctas = self.tiles_m * self.tiles_n * S
+        self.reach = (max(BT, BM) - 1) * p.K * 2     # from a thread's first row of a tile to its last
         self.stage_bytes = self.G * ROW_SLAB + BT * BK * 2
         self.exchange = self.G * BT * BM * 4 if S > 1 else 0
         self.tmem_cols = max(32, 1 << (self.G * BT - 1).bit_length())
@@ -1093,7 +1101,7 @@ class RowsPlan:
     @property
     def possible(self) -> bool:
         return (self.stages >= 2 and self.S <= self.kblocks and self.exchange <= EXCHANGE_LIMIT
-                and self.G * self.BT <= 512
+                and self.G * self.BT <= 512 and self.reach < OFFSET_LIMIT
                 and self.ctas <= (2 * SM_COUNT if self.smem <= SMEM_LIMIT // 2 - 1024 else
                                   SM_COUNT if self.S < 4 else 128))
 
@@ -1367,6 +1375,8 @@ class StreamPlan:
 
     @classmethod
     def of(cls, p: Product) -> "StreamPlan | None":
+        if 8 * p.K * 2 + 1024 >= OFFSET_LIMIT:     # from a lane's row of w to its second, eight further on
+            return None
         return cls(p) if p.M <= 24 else None       # 32 x 4096 x 4096: 12.7 us, the rows kernel 8.0
 
     def estimate(self, p: Product) -> float:
@@ -1379,7 +1389,7 @@ class StreamPlan:
 
 def choose(p: Product) -> TunedKernel | None:
     """The kernel and plan whose estimated time is least, of those whose clusters meta.json's grid divides
-    into (None: there is none).
+    into and which serve rows of this length (None: there is none).
 
     The estimates' forms follow what bounds each kernel; their constants are least-squares fits (of log
     time) to 1,745 timings on a B200 of every plan at M = 1 .. 1024, (N, K) from 512 x 512 to 8192 x 8192,
@@ -1390,7 +1400,7 @@ def choose(p: Product) -> TunedKernel | None:
     128 x 4096 x 4096 - / 10.3 / 12.0 / 16.5; 512 x 4096 x 8192 - / 32.1 / 28.4 / 31.4; 835 x 440 x 4048 gated
     - / 29.8 / 11.8 / 24.2; 1024 x 4096 x 4096 - / 28.8 / - / 26.3; 2048 x 4096 x 4096 - / - / - / 51."""
     plans = []
-    if p.launches_in(2):
+    if p.launches_in(2) and p.tile_ends:
         pair = LinearPair(p)
         plans.append((pair.estimate(), "pair", lambda: pair))
     rows, stream = RowsPlan.best(p), StreamPlan.of(p)
@@ -1400,7 +1410,7 @@ def choose(p: Product) -> TunedKernel | None:
         plans.append((stream.estimate(p), "stream", lambda: LinearStream(p, stream)))
     from thompiler.families.linear_split import LinearSplit, SplitPlan
     split = SplitPlan.best(p)
-    if split is not None and p.launches_in(4):
+    if split is not None and p.launches_in(4) and p.tile_ends:
         plans.append((split.estimate(p), "split", lambda: LinearSplit(p, split)))
     forced = [x for x in plans if x[1] == TUNING.linear_kernel]
     return min(forced or plans, key=lambda x: x[0])[2]() if plans else None
