@@ -118,3 +118,19 @@ def test_wide_f32_rows_of_an_epilogue(tmp_path, monkeypatch):
     ptx = compile_kernel(_info(_package(tmp_path / "p", M, N, 8, 1 << 24, epi, {"extra": ((M, N), "f32", None)})))
     tuned = ptx[:ptx.index("generic lowering of the same IR")]
     assert "tcgen05-linear-pair" in ptx and not re.search(rf"\.u32 [^;]*\b{4 * N};", tuned)
+
+
+@pytest.mark.parametrize("kernel", [*KERNELS, "heads"])
+def test_a_refused_launch_waits_for_the_previous_kernel(tmp_path, monkeypatch, kernel):
+    """A kernel behind a refused launch waits for that launch alone; were it to end at once, the kernel behind
+    it would run beside the one before it."""
+    monkeypatch.setattr(TUNING, "linear_kernel", kernel)
+    ptx = compile_kernel(_info(synth.rope_package(tmp_path / "p", 2, 64, 4, 2, 128) if kernel == "heads" else
+                               synth.linear_package(tmp_path / "p", 16, 512, 512)))
+    lines = [ln.strip() for ln in ptx.splitlines()]
+    records = [i for i, ln in enumerate(lines) if "atom.global.or.b32" in ln and ln.endswith(", 16;")
+               and lines[i + 1] == "ret;"]
+    assert records
+    for i in records:
+        start = max(j for j in range(i) if lines[j].endswith(":"))
+        assert lines[start + 1] == "griddepcontrol.wait;", lines[start:i + 1]

@@ -36,6 +36,7 @@ class TunedKernel:
         # of linear-stream launches in a graph read the previous launch's input)
         self.w.coherent = True
         self.pdl = False            # set by pdl_wait: the tuned body waits for the previous grid
+        self.refusals: list[tuple[str, int]] = []
 
     # programmatic dependent launch ----------------------------------------------
     def pdl_trigger(self) -> None:
@@ -81,6 +82,7 @@ class TunedKernel:
         w.consts.clear()
         w.body(self.k.body)
         em.ins("ret")
+        self._emit_refusals()
         side = self.sidecar()
         if side is not None:
             # keep what the generic path's statements recorded (IR-level tensor maps)
@@ -95,17 +97,21 @@ class TunedKernel:
 
     # helpers ----------------------------------------------------------------
     def refuse(self, bad: str, code: int) -> None:
-        """Place ``bad``: record ``code`` in the module's error word and leave.  For a launch in the tuned
-        geometry that the tuned body cannot serve: the generic lowering needs meta.json's."""
+        """At ``bad``, the module's end: record ``code`` in the module's error word and leave.  For a launch in
+        the tuned geometry that the tuned body cannot serve: the generic lowering needs meta.json's."""
+        self.em.module(".global .align 4 .u32 thc_error")
+        self.refusals.append((bad, code))
+
+    def _emit_refusals(self) -> None:
         em = self.em
-        em.module(".global .align 4 .u32 thc_error")
-        skip, a = em.label("served"), em.tmp("b64")
-        em.ins(f"bra {skip}")
-        em.place(bad)
-        em.ins(f"mov.u64 {a}, thc_error")
-        em.ins(f"atom.global.or.b32 {em.tmp('b32')}, [{a}], {1 << code}")
-        em.ins("ret")
-        em.place(skip)
+        for bad, code in self.refusals:
+            em.place(bad)
+            if self.pdl:             # the next kernel waits for this grid alone: it must not end before the last one
+                em.ins("griddepcontrol.wait")
+            a = em.tmp("b64")
+            em.ins(f"mov.u64 {a}, thc_error")
+            em.ins(f"atom.global.or.b32 {em.tmp('b32')}, [{a}], {1 << code}")
+            em.ins("ret")
 
     def check_aligned(self, names: list[str], to: int, bad: str) -> None:
         """Branch to ``bad`` unless each buffer starts on a multiple of ``to`` bytes."""
