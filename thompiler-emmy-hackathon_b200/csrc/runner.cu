@@ -334,13 +334,16 @@ int tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const cha
     // another stream may rewrite a set.  A launch in flight on buffers T could then match a set
     // caught half-way from its old addresses O to the new ones N if every T[i] is O[i] or N[i]:
     // such a set is not re-encoded while that launch may run.
+    // (A captured graph may be replayed at any time: the sets that it reads are always in flight.)
     auto in_flight = [&](TmapSet &o) -> bool {
+        if (o.pinned) return true;
         if (!o.read_pending) return false;
         cudaError_t q = cudaEventQuery(o.read);
         if (q == cudaSuccess) o.read_pending = false;
-        return o.read_pending || o.pinned;
+        return o.read_pending;
     };
-    auto confusable = [&](int v) -> int {         // a set in flight that v's rewrite could alias, or -1
+    // a set in flight (for_ever: by a captured graph) that v's rewrite could alias, or -1
+    auto confusable = [&](int v, bool for_ever) -> int {
         const std::vector<uint64_t> &old_ = r->s[v].ptrs;
         if (old_.empty()) return -1;
         for (int k = 0; k < r->sets; ++k) {
@@ -348,21 +351,25 @@ int tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const cha
             if (k == v || o.ptrs.empty()) continue;
             bool mix = true;
             for (int i = 0; i < ntmaps && mix; ++i) mix = o.ptrs[i] == old_[i] || o.ptrs[i] == want[i];
-            if (mix && in_flight(o)) return k;
+            if (mix && (for_ever ? o.pinned : in_flight(o))) return k;
         }
         return -1;
     };
     int victim = -1;
     for (int k = 0; k < r->sets; ++k)
-        if (!r->s[k].pinned && confusable(k) < 0 && (victim < 0 || r->s[k].stamp < r->s[victim].stamp)) victim = k;
+        if (!r->s[k].pinned && confusable(k, false) < 0 && (victim < 0 || r->s[k].stamp < r->s[victim].stamp)) victim = k;
     if (victim < 0) {                             // every free set could be aliased: wait for the reader
-        for (int k = 0; k < r->sets; ++k)
-            if (!r->s[k].pinned && (victim < 0 || r->s[k].stamp < r->s[victim].stamp)) victim = k;
-        if (victim < 0)
+        bool unpinned = false;
+        for (int k = 0; k < r->sets; ++k) {
+            unpinned = unpinned || !r->s[k].pinned;
+            if (!r->s[k].pinned && confusable(k, true) < 0 && (victim < 0 || r->s[k].stamp < r->s[victim].stamp))
+                victim = k;
+        }
+        if (!unpinned)
             return fail(THR_ERR_REQUEST, "tensor maps: all %d sets of the module are read by captured graphs", r->sets);
-        for (int c; (c = confusable(victim)) >= 0;) {
-            if (r->s[c].pinned)
-                return fail(THR_ERR_REQUEST, "tensor maps: re-encoding a set could alias one a captured graph reads");
+        if (victim < 0)
+            return fail(THR_ERR_REQUEST, "tensor maps: re-encoding a set could alias one a captured graph reads");
+        for (int c; (c = confusable(victim, false)) >= 0;) {
             cudaError_t e = cudaEventSynchronize(r->s[c].read);
             if (e != cudaSuccess) return cuda_fail(e, "waiting for a tensor-map reader");
             r->s[c].read_pending = false;
