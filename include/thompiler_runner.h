@@ -158,9 +158,12 @@ int thr_run_batch(const thr_run_desc *runs, int nruns, double timeout_s);
  * is, it re-encodes the least recently used one with stream-ordered copies on `stream`, after
  * the last launch that read that set.  Call thr_tmap_launched right after issuing the launch
  * (same stream) so a later re-encoding waits for it.  A set read by a launch captured into a
- * CUDA graph is kept for good; a set must be encoded, and its upload complete, before a capture
+ * CUDA graph is kept for good (and a call on new buffers refused once every set is, or could be
+ * mistaken for one that is); a set must be encoded, and its upload complete, before a capture
  * reads it (launch once on the same buffers and synchronise first).  Maps in separate globals
- * (one per spec) form a single set. */
+ * (one per spec) form a single set.  Threads that launch one module this way hold a lock of their
+ * own from the binding to the report, or another one's binding may re-encode the set in between;
+ * thr_launch_prepared, thr_run_ex and thr_run_batch hold the module's. */
 int thr_tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const char *ptr_table,
                   const uint64_t *args, int nargs, uint64_t stream, int *set);
 int thr_tmap_launched(uint64_t module, int set, uint64_t stream);

@@ -8,6 +8,7 @@ import pytest
 from thompiler import runner, synth
 from thompiler.device import DeviceKernel
 from thompiler.families.kit import TMAP_SETS
+from thompiler.families.tuning import TUNING
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +107,64 @@ def test_no_set_left_is_refused(kernel):
         assert (c.double() - a.double() @ b.double().t()).abs().max().item() < 1e-4
     assert kernel.error_word() == 0
     del graph
+
+
+def test_threads_share_the_last_free_set(tmp_path, monkeypatch):
+    """Graphs keep every set but one, and two threads call the kernel on buffers of their own, each on its own
+    stream: a call's maps stay its own from their binding to its launch.  (A launch whose set is taken from it
+    records bit 4 of the error word and writes nothing.)"""
+    import threading
+
+    import torch
+    from thompiler.families.linear import LinearPair
+    monkeypatch.setattr(TUNING, "linear_kernel", "pair")
+    monkeypatch.setattr(LinearPair, "map_sets", 32)
+    rows, cols, depth, calls = 64, 128, 64, 400
+    k = DeviceKernel(next(synth.linear_package(tmp_path / "p", rows, cols, depth, out_dtype="f32").glob("*.ir.json")))
+    assert k.family == "tcgen05-linear-pair" and k.module.sidecar["tmap_sets"] == 32
+
+    def buffers(n):
+        """Entries of -1, 0 and 1: exact sums."""
+        draw = lambda *shape: torch.randint(-1, 2, (n, *shape), device="cuda").half()   # noqa: E731
+        return draw(rows, depth), draw(cols, depth), torch.empty(n, rows, cols, device="cuda")
+
+    def call(x, w, y, stream):
+        k({"x": x.data_ptr(), "w": w.data_ptr(), "linear": y.data_ptr()}, stream)
+    kept = list(zip(*buffers(31)))
+    for t in kept:
+        call(*t, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for t in kept:
+            call(*t, torch.cuda.current_stream().cuda_stream)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    own = [buffers(calls) for _ in streams]
+    own = [(x, w, y.fill_(float("nan"))) for x, w, y in own]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            for x, w, y in zip(*own[i]):
+                call(x, w, y, streams[i].cuda_stream)
+            streams[i].synchronize()
+        except Exception as e:                                # noqa: BLE001 - reported by the test
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    assert k.error_word() == 0
+    for x, w, y in own:
+        assert torch.equal(y, x.float() @ w.float().transpose(1, 2))
+    for x, w, y in kept:
+        y.fill_(float("nan"))
+    graph.replay()
+    torch.cuda.synchronize()
+    for x, w, y in kept:
+        assert torch.equal(y, x.float() @ w.float().t())
+    del graph
+    k.close()

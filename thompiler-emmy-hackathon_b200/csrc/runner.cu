@@ -18,6 +18,7 @@
 #include <cstdio>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <thread>
@@ -229,25 +230,31 @@ struct TmapRing {
     uint64_t table = 0;                   // the pointer table, 0 if none
     uint64_t clock = 0;
     std::vector<TmapSet> s;
+    std::recursive_mutex mu;              // held from a launch's binding until it is reported (bound_launch)
 };
 
-std::map<uint64_t, TmapRing> g_rings;     // by module handle
-std::mutex g_ring_mu;
+std::map<uint64_t, std::shared_ptr<TmapRing>> g_rings;     // by module handle
+std::mutex g_ring_mu;                     // of g_rings itself
 
 bool stream_capturing(cudaStream_t st) {
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
     return cudaStreamIsCapturing(st, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone;
 }
 
-int ring_of(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const char *ptr_table, TmapRing **out) {
+int ring_of(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const char *ptr_table,
+            std::shared_ptr<TmapRing> *out) {
+    for (int i = 0; i < ntmaps; ++i)
+        if (!tmaps[i].global) return fail(THR_ERR_REQUEST, "tensor map %d names no global", i);
+    std::lock_guard<std::mutex> lk(g_ring_mu);
     auto it = g_rings.find(module);
     if (it != g_rings.end()) {
-        if (it->second.nmaps != ntmaps) return fail(THR_ERR_REQUEST, "tensor maps: %d specs for a module of %d",
-                                                    ntmaps, it->second.nmaps);
-        *out = &it->second;
+        if (it->second->nmaps != ntmaps) return fail(THR_ERR_REQUEST, "tensor maps: %d specs for a module of %d",
+                                                     ntmaps, it->second->nmaps);
+        *out = it->second;
         return THR_OK;
     }
-    TmapRing r;
+    auto made = std::make_shared<TmapRing>();
+    TmapRing &r = *made;
     r.nmaps = ntmaps;
     bool one = true;
     for (int i = 1; i < ntmaps; ++i) one = one && !strcmp(tmaps[i].global, tmaps[0].global);
@@ -282,17 +289,18 @@ int ring_of(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const char 
         r.table = g;
     }
     r.s.resize(r.sets);
-    *out = &g_rings.emplace(module, std::move(r)).first->second;
+    g_rings.emplace(module, made);
+    *out = made;
     return THR_OK;
 }
 
 // Make the set encoded for the mapped buffers (args[tmaps[i].arg]) current for a launch on `st`.
 int tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const char *ptr_table,
               const uint64_t *args, int nargs, cudaStream_t st, int *set_out) {
-    std::lock_guard<std::mutex> lk(g_ring_mu);
-    TmapRing *r = nullptr;
+    std::shared_ptr<TmapRing> r;
     int s = ring_of(module, tmaps, ntmaps, ptr_table, &r);
     if (s) return s;
+    std::lock_guard<std::recursive_mutex> lk(r->mu);
     std::vector<uint64_t> want(ntmaps);
     for (int i = 0; i < ntmaps; ++i) {
         if (tmaps[i].arg < 0 || tmaps[i].arg >= nargs) return fail(THR_ERR_REQUEST, "tensor map %d: bad argument", i);
@@ -424,10 +432,15 @@ int tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const cha
 
 // A launch that reads set `k` was just issued on `st`.
 int tmap_launched(uint64_t module, int k, cudaStream_t st) {
-    std::lock_guard<std::mutex> lk(g_ring_mu);
-    auto it = g_rings.find(module);
-    if (it == g_rings.end() || k < 0 || k >= it->second.sets) return fail(THR_ERR_REQUEST, "tensor maps: set %d", k);
-    TmapSet &t = it->second.s[k];
+    std::shared_ptr<TmapRing> r;
+    {
+        std::lock_guard<std::mutex> lk(g_ring_mu);
+        auto it = g_rings.find(module);
+        if (it != g_rings.end()) r = it->second;
+    }
+    if (!r || k < 0 || k >= r->sets) return fail(THR_ERR_REQUEST, "tensor maps: set %d", k);
+    std::lock_guard<std::recursive_mutex> lk(r->mu);
+    TmapSet &t = r->s[k];
     if (stream_capturing(st)) {
         t.pinned = true;
         return THR_OK;
@@ -440,11 +453,31 @@ int tmap_launched(uint64_t module, int k, cudaStream_t st) {
     return THR_OK;
 }
 
+// One launch that reads maps: the set for args[] bound on `bind_st`, go() issues the launch on `st`, and the launch is
+// reported.  The ring is held throughout: in between, another thread's binding could re-encode the set.
+template <class Go>
+int bound_launch(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const char *ptr_table, const uint64_t *args,
+                 int nargs, cudaStream_t bind_st, cudaStream_t st, Go go) {
+    if (!ntmaps) return go();
+    std::shared_ptr<TmapRing> r;
+    int s = ring_of(module, tmaps, ntmaps, ptr_table, &r), set = -1;
+    if (s) return s;
+    std::lock_guard<std::recursive_mutex> lk(r->mu);
+    if ((s = tmap_bind(module, tmaps, ntmaps, ptr_table, args, nargs, bind_st, &set)) || (s = go())) return s;
+    return tmap_launched(module, set, st);
+}
+
 void drop_ring(uint64_t module) {
-    std::lock_guard<std::mutex> lk(g_ring_mu);
-    auto it = g_rings.find(module);
-    if (it == g_rings.end()) return;
-    for (TmapSet &t : it->second.s) {
+    std::shared_ptr<TmapRing> r;
+    {
+        std::lock_guard<std::mutex> lk(g_ring_mu);
+        auto it = g_rings.find(module);
+        if (it == g_rings.end()) return;
+        r = it->second;
+        g_rings.erase(it);
+    }
+    std::lock_guard<std::recursive_mutex> lk(r->mu);
+    for (TmapSet &t : r->s) {
         if (t.uploaded) {
             cudaEventSynchronize(t.uploaded);
             cudaEventDestroy(t.uploaded);
@@ -452,7 +485,6 @@ void drop_ring(uint64_t module) {
         if (t.read) cudaEventDestroy(t.read);
         if (t.staging) cudaFreeHost(t.staging);
     }
-    g_rings.erase(it);
 }
 
 // Wait for `ev` at most timeout_s seconds.  A request's work often ends within a millisecond
@@ -673,7 +705,7 @@ int thr_run_ex(uint64_t module, uint64_t function, const uint32_t grid[3], const
                             : cudaMemsetAsync(p, 0, args[i].nbytes, st);
         if (e != cudaSuccess) return cuda_fail(e, "staging a run argument");
     }
-    int set = -1;
+    int set = -1;                              // here, so that an upload is none of the timed launches'
     if (ntmaps && (s = tmap_bind(module, tmaps, ntmaps, ptr_table, dev.data(), nargs, st, &set))) return s;
     auto rezero = [&]() -> int {
         for (int i = 0; i < nargs; ++i)
@@ -690,10 +722,12 @@ int thr_run_ex(uint64_t module, uint64_t function, const uint32_t grid[3], const
     int rc = THR_OK;
     for (int k = 0; k < total && rc == THR_OK; ++k) {
         if ((rc = rezero())) break;
-        cudaEventRecord(ev[2 * k], st);
-        rc = thr_launch(function, grid, block, smem_bytes, dev.data(), nargs, stream);
-        if (rc == THR_OK && ntmaps) rc = tmap_launched(module, set, st);
-        cudaEventRecord(ev[2 * k + 1], st);
+        rc = bound_launch(module, tmaps, ntmaps, ptr_table, dev.data(), nargs, st, st, [&]() -> int {
+            cudaEventRecord(ev[2 * k], st);
+            int l = thr_launch(function, grid, block, smem_bytes, dev.data(), nargs, stream);
+            cudaEventRecord(ev[2 * k + 1], st);
+            return l;
+        });
     }
     if (rc == THR_OK) rc = wait_event(ev[2 * total - 1], timeout_s);
     if (rc == THR_OK) {
@@ -750,20 +784,18 @@ int thr_run_batch(const thr_run_desc *runs, int nruns, double timeout_s) {
             if (e != cudaSuccess) rc = cuda_fail(e, "staging a batch argument");
         }
         if (rc) break;
-        int set = -1;
-        if (d.ntmaps && (rc = tmap_bind(d.module, d.tmaps, d.ntmaps, d.ptr_table, dev.data(), d.nargs, sin, &set)))
-            break;
         cudaEvent_t staged, ran;
         if (!event(&staged) || !event(&ran)) {
             rc = fail(THR_ERR_CUDA, "cudaEventCreate");
             break;
         }
-        cudaEventRecord(staged, sin);
-        cudaStreamWaitEvent(scmp, staged, 0);
-        if ((rc = thr_launch(d.function, d.grid, d.block, d.smem_bytes, dev.data(), d.nargs,
-                             (uint64_t)(uintptr_t)scmp)))
-            break;
-        if (d.ntmaps && (rc = tmap_launched(d.module, set, scmp))) break;
+        rc = bound_launch(d.module, d.tmaps, d.ntmaps, d.ptr_table, dev.data(), d.nargs, sin, scmp, [&]() -> int {
+            cudaEventRecord(staged, sin);
+            cudaStreamWaitEvent(scmp, staged, 0);
+            return thr_launch(d.function, d.grid, d.block, d.smem_bytes, dev.data(), d.nargs,
+                              (uint64_t)(uintptr_t)scmp);
+        });
+        if (rc) break;
         cudaEventRecord(ran, scmp);
         cudaStreamWaitEvent(sout, ran, 0);
         for (int i = 0; i < d.nargs && rc == THR_OK; ++i)
@@ -799,8 +831,6 @@ int thr_tmap_bind(uint64_t module, const thr_tmap_spec *tmaps, int ntmaps, const
     if (s) return s;
     if (!module || ntmaps <= 0 || !tmaps || !args || nargs <= 0 || !set)
         return fail(THR_ERR_REQUEST, "thr_tmap_bind: bad arguments");
-    for (int i = 0; i < ntmaps; ++i)
-        if (!tmaps[i].global) return fail(THR_ERR_REQUEST, "thr_tmap_bind: tensor map %d names no global", i);
     return tmap_bind(module, tmaps, ntmaps, ptr_table, args, nargs, (cudaStream_t)(uintptr_t)stream, set);
 }
 
@@ -815,13 +845,14 @@ int thr_launch_prepared(const thr_launch_desc *d, const uint64_t *args, uint64_t
             if (d->align[i] > 1 && (args[i] & (d->align[i] - 1)))
                 return fail(THR_ERR_REQUEST, "argument %d at 0x%llx is not %u-byte aligned", i,
                             (unsigned long long)args[i], d->align[i]);
-    int set = -1, s = THR_OK;
-    if (d->ntmaps > 0 &&
-        (s = thr_tmap_bind(d->module, d->tmaps, d->ntmaps, d->ptr_table, args, d->nargs, stream, &set)))
-        return s;
-    s = thr_launch_ex(d->function, d->grid, d->block, d->smem_bytes, args, d->nargs, stream, d->flags);
-    if (!s && d->ntmaps > 0) s = thr_tmap_launched(d->module, set, stream);
-    return s;
+    int s = ensure_driver();
+    if (s) return s;
+    if (d->ntmaps < 0 || (d->ntmaps && (!d->module || !d->tmaps)))
+        return fail(THR_ERR_REQUEST, "thr_launch_prepared: bad tensor maps");
+    cudaStream_t st = (cudaStream_t)(uintptr_t)stream;
+    return bound_launch(d->module, d->tmaps, d->ntmaps, d->ptr_table, args, d->nargs, st, st, [&]() -> int {
+        return thr_launch_ex(d->function, d->grid, d->block, d->smem_bytes, args, d->nargs, stream, d->flags);
+    });
 }
 
 int thr_tensor_map(void *out128, int dtype_code, int rank, uint64_t base, const uint64_t *dims,
