@@ -1,5 +1,5 @@
 """Linear products whose package is launched with a grid that clusters do not divide, under their own
-launch and meta.json's, against the float64 product; and products of very long rows."""
+launch and meta.json's, against the float64 product; products of very long rows, and of very many columns."""
 
 import pytest
 
@@ -56,5 +56,22 @@ def test_long_rows(tmp_path, monkeypatch, M, N, K, kernel):
     for at in range(0, K, 1 << 20):
         want += x[:, at:at + (1 << 20)].double() @ w[:, at:at + (1 << 20)].double().t()
     assert torch.equal(y.double(), want)
+    assert k.error_word() == 0
+    k.close()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 50264, 264), (25, 50264, 264), (64, 128256, 64), (300, 37904, 72)])
+def test_many_columns(tmp_path, M, N, K):
+    """The widths of an output head, past the columns that the kernel for few rows takes."""
+    import torch
+    k = DeviceKernel(next(synth.linear_package(tmp_path / "p", M, N, K).glob("*.ir.json")))
+    g = torch.Generator(device="cuda").manual_seed(N)
+    x = torch.randn(M, K, device="cuda", generator=g).half()
+    w = (torch.randn(N, K, device="cuda", generator=g) * K ** -0.5).half()
+    y = torch.full((M, N), float("nan"), device="cuda", dtype=torch.float16)
+    k({"x": x.data_ptr(), "w": w.data_ptr(), "linear": y.data_ptr()}, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    want, allowed = _bound(x, w)
+    assert ((y.double() - want).abs() <= allowed).all()
     assert k.error_word() == 0
     k.close()
