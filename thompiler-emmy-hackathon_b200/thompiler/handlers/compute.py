@@ -2,7 +2,8 @@
 
 Load / Write move one value or a group of consecutive values (a vector
 access of at most 16 bytes).  Global reads of buffers the kernel never
-writes go through the read-only non-coherent path (``ld.global.nc``).
+writes go through the read-only non-coherent path (``ld.global.nc``), but
+not in a tuned module, which may overlap the kernel that writes them.
 Assign lowers one elementwise op with ``.rn`` arithmetic (bit-exact against
 CPU float math), ``exp`` as ``ex2.approx(x * log2 e)`` (the reference's
 lowering, thompiler/handlers/compute.py:77-83 of the reference), ``relu`` as
